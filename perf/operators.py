@@ -228,8 +228,7 @@ def _plain_beam(c):
     x, scores, eos = c['logits'].float(), c['scores'], c['eos']
     B, W, V = x.shape
     top = x.amax(-1, keepdim=True)
-    lse = top + torch.exp(x - top).sum(-1, keepdim=True).log()
-    cand = scores[..., None] + (x - lse)
+    cand = scores[..., None] + ((x - top) - torch.exp(x - top).sum(-1, keepdim=True).log())
     done = torch.full_like(cand, float('-inf'))
     done[..., eos] = scores
     cand = torch.where(c['finished'][..., None], done, cand)
