@@ -22,6 +22,25 @@ _i64 = ctypes.c_int64
 _int = ctypes.c_int
 _flt = ctypes.c_float
 
+
+
+class DecayWalkArgs(ctypes.Structure):
+    """bdm_decay_walk_args of include/bdm_b200.h."""
+    _fields_ = ([(n, _vp) for n in ('a', 'b', 'c', 'out', 'log_decay', 'lengths', 'state_in', 'state_out', 'status')]
+                + [(n, _i64 * 3) for n in ('a_stride', 'b_stride', 'c_stride', 'out_stride')]
+                + [('batch', _i64), ('time', _i64)]
+                + [(n, _int) for n in ('heads', 'a_heads', 'b_heads', 'c_heads', 'width_ab', 'width_c', 'dtype',
+                                       'out_dtype', 'reverse', 'state_in_transposed', 'state_out_transposed')]
+                + [(n, _flt) for n in ('scale', 'state_in_mul', 'state_out_mul')])
+
+
+class DecayStepArgs(ctypes.Structure):
+    """bdm_decay_step_args of include/bdm_b200.h."""
+    _fields_ = ([(n, _vp) for n in ('q', 'k', 'v', 'log_decay', 'state', 'out')]
+                + [(n, _i64 * 2) for n in ('q_stride', 'k_stride', 'v_stride')] + [('batch', _i64)]
+                + [(n, _int) for n in ('heads', 'kv_heads', 'key_width', 'value_width', 'dtype')] + [('scale', _flt)])
+
+
 # name -> (restype, argtypes); mirrors include/bdm_b200.h
 SIGNATURES = {
     'bdm_status_string': (ctypes.c_char_p, [_int]),
@@ -82,6 +101,14 @@ SIGNATURES = {
     'bdm_norm_gate_f32': (_int, [_vp, _i64, _i64, _vp, _i64, _vp, _vp, _flt, _int, _int, _vp, _vp]),
     'bdm_decode_step': (_int, [_vp, _vp, _vp, _vp, _vp, _vp, _vp, _vp, _vp, _vp, _i64, _i64, _int, _int, _int, _int,
                                _int, _int, _int, _flt, _vp, _int, _vp, _vp, _i64, _vp, _vp, _flt, _int, _vp, _vp]),
+    'bdm_decay_walk_workspace_bytes': (_i64, [ctypes.POINTER(DecayWalkArgs)]),
+    'bdm_decay_walk': (_int, [ctypes.POINTER(DecayWalkArgs), _vp, _i64, _vp]),
+    'bdm_decay_group_sum': (_int, [_vp, _i64, _int, _int, _int, _int, _vp, _vp]),
+    'bdm_decay_step': (_int, [ctypes.POINTER(DecayStepArgs), _vp]),
+    'bdm_beam_select_workspace_bytes': (_i64, [_i64, _int, _i64]),
+    'bdm_beam_select': (_int, [_vp, _i64, _i64, _int, _i64, _int, _vp, _vp, _i64, _int, _vp, _vp, _vp, _vp, _vp, _i64,
+                               _vp]),
+    'bdm_reorder_rows': (_int, [_vp, _vp, _vp, _int, _vp, _i64, _int, _vp, _vp]),
 }
 
 _lib = None

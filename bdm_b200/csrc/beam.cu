@@ -1,0 +1,569 @@
+// Beam search: selection over beams x vocabulary, and the in-place reordering of decoder states.
+#include "common.cuh"
+
+namespace bdm {
+namespace {
+
+constexpr int kThreads = 256;
+constexpr int kWarps = kThreads / 32;
+constexpr int kMaxBeams = 32;
+constexpr int kList = 1024;  // candidates a CTA collects before it falls back to repeated maxima
+
+using u64 = unsigned long long;
+
+// Order of floats as unsigned integers, -0 as +0; NaN never gets here.
+__device__ __forceinline__ uint32_t ordered(float x) {
+    const uint32_t u = __float_as_uint(x + 0.f);
+    return u & 0x80000000u ? ~u : u | 0x80000000u;
+}
+__device__ __forceinline__ float unordered(uint32_t u) {
+    return __uint_as_float(u & 0x80000000u ? u & 0x7fffffffu : ~u);
+}
+// Larger value first, then lower index; 0 is no candidate (its index would be 2^32 - 1 and its value NaN).
+__device__ __forceinline__ u64 make_key(float x, uint32_t index) { return (u64)ordered(x) << 32 | (uint32_t)~index; }
+__device__ __forceinline__ float key_value(u64 k) { return unordered((uint32_t)(k >> 32)); }
+__device__ __forceinline__ uint32_t key_index(u64 k) { return ~(uint32_t)k; }
+
+// Sorts one key per lane, largest in lane 0.
+__device__ __forceinline__ u64 warp_sort_desc(u64 x) {
+    const int lane = threadIdx.x & 31;
+#pragma unroll
+    for (int size = 2; size <= 32; size <<= 1)
+#pragma unroll
+        for (int d = size >> 1; d > 0; d >>= 1) {
+            const u64 y = __shfl_xor_sync(0xffffffffu, x, d);
+            const bool up = (lane & size) == 0, low = (lane & d) == 0;
+            x = (up == low) == (x > y) ? x : y;
+        }
+    return x;
+}
+__device__ __forceinline__ u64 warp_max(u64 x) {
+#pragma unroll
+    for (int o = 16; o > 0; o >>= 1) {
+        const u64 y = __shfl_xor_sync(0xffffffffu, x, o);
+        x = x > y ? x : y;
+    }
+    return x;
+}
+
+struct TopShared {
+    u64 list[kList];
+    u64 best[kMaxBeams];
+    u64 warp[kWarps];
+    int count;
+};
+
+__device__ u64 block_max(u64 m, TopShared &sh) {
+    m = warp_max(m);
+    __syncthreads();
+    if ((threadIdx.x & 31) == 0) sh.warp[threadIdx.x >> 5] = m;
+    __syncthreads();
+#pragma unroll
+    for (int w = 0; w < kWarps; ++w) m = sh.warp[w] > m ? sh.warp[w] : m;
+    return m;
+}
+
+// The K largest of all threads' keys key(0) .. key(E-1) (0 = none), in descending order in sh.best (0 where
+// there are fewer).  Keys are distinct.  The K-th largest of one warp's 32 thread maxima bounds the K-th
+// largest of the CTA's keys from below; the keys above the largest such bound (a few times K) go to a list
+// and are ranked there.  When the list overflows (a few threads hold most of the largest keys), K rounds of
+// a CTA-wide maximum take its place.
+template <int E, typename F> __device__ void block_topk(int K, TopShared &sh, F key) {
+    const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
+    u64 mx = 0;
+#pragma unroll
+    for (int e = 0; e < E; ++e) {
+        const u64 x = key(e);
+        mx = x > mx ? x : mx;
+    }
+    const u64 sorted = warp_sort_desc(mx);
+    const u64 kth = __shfl_sync(0xffffffffu, sorted, K - 1);
+    if (lane == 0) sh.warp[warp] = kth;
+    if (tid == 0) sh.count = 0;
+    if (tid < K) sh.best[tid] = 0;
+    __syncthreads();
+    u64 bound = 1;
+#pragma unroll
+    for (int w = 0; w < kWarps; ++w) bound = sh.warp[w] > bound ? sh.warp[w] : bound;
+    if (mx >= bound)
+#pragma unroll
+        for (int e = 0; e < E; ++e) {
+            const u64 x = key(e);
+            if (x >= bound) {
+                const int at = atomicAdd(&sh.count, 1);
+                if (at < kList) sh.list[at] = x;
+            }
+        }
+    __syncthreads();
+    const int n = sh.count;
+    if (n <= kList) {
+        for (int i = tid; i < n; i += kThreads) {
+            const u64 x = sh.list[i];
+            int rank = 0;
+            for (int j = 0; j < n && rank < K; ++j) rank += sh.list[j] > x;
+            if (rank < K) sh.best[rank] = x;
+        }
+        __syncthreads();
+        return;
+    }
+    u64 last = ~0ull;
+    for (int r = 0; r < K; ++r) {
+        u64 m = 0;
+#pragma unroll
+        for (int e = 0; e < E; ++e) {
+            const u64 x = key(e);
+            if (x < last && x > m) m = x;
+        }
+        last = block_max(m, sh);
+        if (tid == 0) sh.best[r] = last;
+        if (last == 0) break;
+    }
+    __syncthreads();
+}
+
+// ------------------------------------------------------------- per row slices
+
+// Per (row, split): the slice's maximum, the sum of exp(x - max), and its K largest logits by (value,
+// lower index).
+struct Slice {
+    float max, sum;
+};
+
+template <typename T> struct Vec;
+template <> struct Vec<float> {
+    static constexpr int n = 4;
+};
+template <> struct Vec<bf16> {
+    static constexpr int n = 8;
+};
+
+template <typename T> __device__ __forceinline__ void unpack(const uint4 &r, float *x);
+template <> __device__ __forceinline__ void unpack<float>(const uint4 &r, float *x) {
+    x[0] = __uint_as_float(r.x), x[1] = __uint_as_float(r.y), x[2] = __uint_as_float(r.z), x[3] = __uint_as_float(r.w);
+}
+template <> __device__ __forceinline__ void unpack<bf16>(const uint4 &r, float *x) {
+    const uint32_t w[4] = {r.x, r.y, r.z, r.w};
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+        x[2 * i] = __uint_as_float(w[i] << 16);
+        x[2 * i + 1] = __uint_as_float(w[i] & 0xffff0000u);
+    }
+}
+
+// E logits per thread.  VECTOR: rows start on 16-byte boundaries.
+template <typename T, int E, bool VECTOR>
+__global__ void __launch_bounds__(kThreads)
+    beam_slice_kernel(const T *__restrict__ logits, int64_t ld, int vocab, int K, int splits, Slice *__restrict__ stat,
+                      u64 *__restrict__ lists) {
+    __shared__ TopShared sh;
+    __shared__ float redf[kWarps];
+    const int64_t row = blockIdx.x / splits;
+    const int split = (int)(blockIdx.x % splits);
+    const int base = split * (E * kThreads);
+    const T *src = logits + row * ld;
+    constexpr int V = VECTOR ? Vec<T>::n : 1;
+    float x[E];
+    auto index = [&](int e) { return base + (e / V * kThreads + (int)threadIdx.x) * V + e % V; };
+#pragma unroll
+    for (int e = 0; e < E; e += V) {
+        const int i = index(e);
+        if (VECTOR && i + V <= vocab) {
+            unpack<T>(*reinterpret_cast<const uint4 *>(src + i), x + e);
+        } else {
+#pragma unroll
+            for (int u = 0; u < V; ++u) x[e + u] = i + u < vocab ? Elem<T>::to_float(src[i + u]) : -INFINITY;
+        }
+    }
+    // maximum; NaN and +inf make the whole row's log-probabilities NaN
+    float m = -INFINITY;
+    bool bad = false;
+#pragma unroll
+    for (int e = 0; e < E; ++e) {
+        m = fmaxf(m, x[e]);
+        bad |= !(x[e] < INFINITY);
+    }
+#pragma unroll
+    for (int o = 16; o > 0; o >>= 1) m = fmaxf(m, __shfl_xor_sync(0xffffffffu, m, o));
+    if ((threadIdx.x & 31) == 0) redf[threadIdx.x >> 5] = m;
+    bad = __syncthreads_or(bad);
+#pragma unroll
+    for (int w = 0; w < kWarps; ++w) m = fmaxf(m, redf[w]);
+    float s = 0.f;
+    if (m > -INFINITY && !bad)
+#pragma unroll
+        for (int e = 0; e < E; ++e) s += expf(x[e] - m);
+    s = warp_sum(s);
+    __syncthreads();
+    if ((threadIdx.x & 31) == 0) redf[threadIdx.x >> 5] = s;
+    __syncthreads();
+    if (threadIdx.x == 0) {
+        s = 0.f;
+        for (int w = 0; w < kWarps; ++w) s += redf[w];
+        stat[row * splits + split] = Slice{bad ? NAN : m, s};
+    }
+    if (bad) return;  // the row has no candidate of its own: its list is not read
+    block_topk<E>(K, sh, [&](int e) {
+        const int i = index(e);
+        return i < vocab ? make_key(x[e], (uint32_t)i) : 0ull;
+    });
+    if (threadIdx.x < K) lists[(row * splits + split) * K + threadIdx.x] = sh.best[threadIdx.x];
+}
+
+// ------------------------------------------------------------------- merging
+
+// Largest value of the type below x (x finite).
+template <typename T> __device__ __forceinline__ float next_below(float x);
+template <> __device__ __forceinline__ float next_below<float>(float x) { return nextafterf(x, -INFINITY); }
+template <> __device__ __forceinline__ float next_below<bf16>(float x) {
+    if (x == 0.f) return -__uint_as_float(0x00010000u);
+    const uint32_t u = __float_as_uint(x);
+    return __uint_as_float(x > 0.f ? u - 0x10000u : u + 0x10000u);
+}
+
+struct Row {
+    float score, max, logsum;
+    int kind;  // 0: finite log-probabilities, 1: every candidate is -inf, 2: finished
+};
+
+// score + log softmax.  The maximum goes first: a row at the type's lowest value keeps its uniform weights.
+__device__ __forceinline__ float candidate(const Row &r, float logit) {
+    const float c = r.score + ((logit - r.max) - r.logsum);
+    return c == c ? c : -INFINITY;  // NaN ranks as -inf
+}
+
+// One CTA per batch row: joins the rows' softmax sums, ranks their candidates by (value, lower flat
+// index) and writes the new beams.
+template <typename T>
+__global__ void __launch_bounds__(kThreads)
+    beam_merge_kernel(const T *__restrict__ logits, int64_t ld, const float *__restrict__ scores,
+                      const uint8_t *__restrict__ finished, int64_t eos, int beams, int vocab, int splits, int stable,
+                      const Slice *__restrict__ stat, const u64 *__restrict__ lists, float *__restrict__ out_scores,
+                      int64_t *__restrict__ out_parents, int64_t *__restrict__ out_tokens,
+                      uint8_t *__restrict__ out_finished) {
+    __shared__ TopShared sh;
+    __shared__ Row rows[kMaxBeams];
+    __shared__ u64 kept[kMaxBeams];
+    __shared__ int reach[kMaxBeams];
+    const int64_t b = blockIdx.x;
+    const int K = beams, tid = threadIdx.x;
+    if (tid < beams) {
+        const int64_t row = b * beams + tid;
+        Row r;
+        r.score = scores[row];
+        float m = -INFINITY, s = 0.f;
+        bool bad = false;
+        for (int i = 0; i < splits; ++i) {
+            const Slice t = stat[row * splits + i];
+            bad |= t.max != t.max;
+            m = fmaxf(m, t.max);
+        }
+        for (int i = 0; i < splits; ++i) {
+            const Slice t = stat[row * splits + i];
+            if (t.max > -INFINITY) s += t.sum * expf(t.max - m);
+        }
+        r.max = m;
+        r.logsum = logf(s);
+        r.kind = bad || m == -INFINITY || r.score != r.score || r.score == -INFINITY;
+        if (finished && finished[row]) r.kind = 2;
+        rows[tid] = r;
+        kept[tid] = 0;
+    }
+    __syncthreads();
+    // rows 0 .. beams-1, per row splits * K listed keys (K made-up ones for kinds 1 and 2)
+    const int per = splits * K, total = beams * per;
+    constexpr int E = 8;
+    u64 limit[E];
+    auto entry = [&](int i) -> u64 {
+        const int w = i / per, j = i % per;
+        const Row r = rows[w];
+        const uint32_t flat = (uint32_t)w * (uint32_t)vocab;
+        if (r.kind == 0) {
+            const u64 x = lists[(b * beams + w) * per + j];
+            return x ? make_key(candidate(r, key_value(x)), flat + key_index(x)) : 0ull;
+        }
+        if (j >= K) return 0ull;
+        if (r.kind == 1) return j < vocab ? make_key(-INFINITY, flat + j) : 0ull;
+        // finished: the end token keeps the score, then the lowest other tokens
+        if (j == 0) return make_key(r.score == r.score ? r.score : -INFINITY, flat + (uint32_t)eos);
+        const int t = j - 1 < (int)eos ? j - 1 : j;
+        return t < vocab ? make_key(-INFINITY, flat + t) : 0ull;
+    };
+    auto select = [&]() {
+        if (tid < beams) kept[tid] = 0;
+        for (int i0 = 0; i0 < total; i0 += kThreads * (E - 1)) {
+#pragma unroll
+            for (int e = 0; e < E - 1; ++e) {
+                const int i = i0 + e * kThreads + tid;
+                limit[e] = i < total ? entry(i) : 0ull;
+            }
+            __syncthreads();
+            limit[E - 1] = tid < K ? kept[tid] : 0ull;
+            block_topk<E>(K, sh, [&](int e) { return limit[e]; });
+            if (tid < K) kept[tid] = sh.best[tid];
+            __syncthreads();
+        }
+    };
+    select();
+    // Rounding may give unlisted logits (below the row's list) the value of a listed one and a lower index.
+    // That can matter only where the type's next value below the list's last logit already rounds to the same
+    // candidate, and that candidate reaches the selection: such a row is read again, by candidate.
+    // (the row then has K listed candidates at or above the last kept value)
+    if (tid < beams) reach[tid] = 0;
+    __syncthreads();
+    const uint32_t kth = (uint32_t)(kept[K - 1] >> 32);
+    for (int i = tid; i < total; i += kThreads)
+        if (rows[i / per].kind == 0 && (uint32_t)(entry(i) >> 32) >= kth) atomicAdd(&reach[i / per], 1);
+    __syncthreads();
+    for (int w = 0; w < beams; ++w) {
+        const Row r = rows[w];
+        if (reach[w] < K || vocab <= K) continue;
+        u64 lowest = ~0ull;  // the row's K-th largest logit
+        for (int k = 0; k < K; ++k) {
+            u64 m = 0;
+            for (int j = tid; j < per; j += kThreads) {
+                const u64 x = lists[(b * beams + w) * per + j];
+                if (x < lowest && x > m) m = x;
+            }
+            lowest = block_max(m, sh);
+        }
+        const float x = key_value(lowest);
+        if (!(x > -INFINITY)) continue;
+        const float c = candidate(r, x);
+        if (candidate(r, next_below<T>(x)) != c) continue;
+        // the row's K best by candidate, merged with the other rows' candidates kept so far
+        const uint32_t flat = (uint32_t)w * (uint32_t)vocab;
+        u64 last = ~0ull;
+        u64 mine = 0;  // thread k < K: the row's k-th
+        for (int k = 0; k < K; ++k) {
+            u64 m = 0;
+            for (int i = tid; i < vocab; i += kThreads) {
+                const u64 y = make_key(candidate(r, Elem<T>::to_float(logits[(b * beams + w) * ld + i])),
+                                       flat + i);
+                if (y < last && y > m) m = y;
+            }
+            last = block_max(m, sh);
+            if (tid == k) mine = last;
+        }
+        u64 other = tid < K ? kept[tid] : 0ull;
+        if (other && key_index(other) / (uint32_t)vocab == (uint32_t)w) other = 0;  // its own are in `mine`
+        __syncthreads();
+        block_topk<2>(K, sh, [&](int e) { return e ? mine : other; });
+        if (tid < K) kept[tid] = sh.best[tid];
+        __syncthreads();
+    }
+    if (tid < 32) {
+        const bool on = tid < K;
+        const u64 x = on ? kept[tid] : 0ull;
+        const uint32_t at = key_index(x);
+        const int parent = on ? (int)(at / (uint32_t)vocab) : -1 - tid;
+        const int64_t token = on ? at % (uint32_t)vocab : 0;
+        int slot = tid;
+        if (stable) {
+            // the first child of a parent takes its slot, the others the free slots in turn
+            const unsigned all = 0xffffffffu;
+            const unsigned same = __match_any_sync(all, parent);
+            const bool first = (same & ((1u << tid) - 1)) == 0;
+            unsigned taken = on ? 1u << parent : 0u;
+#pragma unroll
+            for (int o = 16; o > 0; o >>= 1) taken |= __shfl_xor_sync(all, taken, o);
+            const unsigned later = __ballot_sync(all, on && !first);
+            if (on) {
+                if (first) {
+                    slot = parent;
+                } else {
+                    unsigned open = ~taken;
+                    for (int n = __popc(later & ((1u << tid) - 1)); n > 0; --n) open &= open - 1;
+                    slot = __ffs(open) - 1;
+                }
+            }
+        }
+        if (on) {
+            const int64_t o = b * beams + slot;
+            out_scores[o] = key_value(x);
+            out_parents[o] = parent;
+            out_tokens[o] = token;
+            if (out_finished)
+                out_finished[o] = (finished && finished[b * beams + parent]) || (eos >= 0 && token == eos);
+        }
+    }
+}
+
+// Logits per thread of the slice kernel and the splits of a row.
+struct BeamPlan {
+    int e, splits;
+};
+BeamPlan beam_plan(int64_t rows, int64_t vocab) {
+    BeamPlan p;
+    // 32 logits per thread where the rows alone fill the GPU, fewer (more CTAs per row) where they do not
+    p.e = rows * ceil_div(vocab, 32 * kThreads) >= kNumSMs ? 32 : 8;
+    p.splits = (int)ceil_div(vocab, p.e * kThreads);
+    return p;
+}
+
+// ------------------------------------------------------------------ reordering
+
+constexpr int kMaxTensors = 32;
+struct Tensors {
+    void *base[kMaxTensors];
+    int64_t stride[kMaxTensors];  // bytes between rows
+    int64_t units[kMaxTensors];   // access units per row
+    int64_t first[kMaxTensors + 1];  // first tile of each tensor
+    int count;
+};
+
+constexpr int kUnroll = 4;  // columns a thread moves at a time
+
+// In place: each thread owns columns of one group's rows and reads all of them that move before it writes
+// any, so permutations and copies need no second buffer.
+template <typename U, int W>
+__global__ void __launch_bounds__(kThreads)
+    reorder_rows_kernel(const Tensors t, const int64_t *__restrict__ parents, int beams, int64_t groups, int *status) {
+    int k = 0;
+    while (k + 1 < t.count && (int64_t)blockIdx.x >= t.first[k + 1]) ++k;
+    const int64_t tile = blockIdx.x - t.first[k];
+    const int64_t group = tile % groups, col0 = tile / groups * (kThreads * kUnroll) + threadIdx.x;
+    int src[W];
+    bool any = false;
+#pragma unroll
+    for (int i = 0; i < W; ++i) {
+        src[i] = i;
+        if (i < beams) {
+            const int64_t s = parents[group * beams + i];
+            if (s >= 0 && s < beams)
+                src[i] = (int)s;
+            else if (status && threadIdx.x == 0)
+                atomicOr(status, 0x8);  // the row keeps its state
+            any |= src[i] != i;
+        }
+    }
+    if (!any) return;
+    char *base = static_cast<char *>(t.base[k]) + group * beams * t.stride[k];
+    const int64_t stride = t.stride[k], units = t.units[k];
+    constexpr int kAt = W <= 4 ? kUnroll : (W <= 8 ? 2 : 1);  // columns in registers at a time
+#pragma unroll
+    for (int u0 = 0; u0 < kUnroll; u0 += kAt) {
+        U x[kAt][W];
+#pragma unroll
+        for (int u = 0; u < kAt; ++u)
+#pragma unroll
+            for (int i = 0; i < W; ++i)
+                if (src[i] != i && col0 + (u0 + u) * kThreads < units)
+                    x[u][i] = *(reinterpret_cast<const U *>(base + src[i] * stride) + col0 + (u0 + u) * kThreads);
+#pragma unroll
+        for (int u = 0; u < kAt; ++u)
+#pragma unroll
+            for (int i = 0; i < W; ++i)
+                if (src[i] != i && col0 + (u0 + u) * kThreads < units)
+                    *(reinterpret_cast<U *>(base + i * stride) + col0 + (u0 + u) * kThreads) = x[u][i];
+    }
+}
+
+template <typename U>
+int reorder_launch(Tensors t, const int64_t *row_bytes, const int64_t *parents, int64_t groups, int beams, int *status,
+                   cudaStream_t st) {
+    int64_t tiles = 0;
+    for (int i = 0; i < t.count; ++i) {
+        t.units[i] = row_bytes[i] / (int64_t)sizeof(U);
+        t.first[i] = tiles;
+        tiles += groups * ceil_div(t.units[i], kThreads * kUnroll);
+    }
+    t.first[t.count] = tiles;
+    if (tiles > 0x7fffffff) return BDM_ERR_UNSUPPORTED;
+    if (tiles == 0) return BDM_OK;
+    if (beams <= 4)
+        reorder_rows_kernel<U, 4><<<(unsigned)tiles, kThreads, 0, st>>>(t, parents, beams, groups, status);
+    else if (beams <= 8)
+        reorder_rows_kernel<U, 8><<<(unsigned)tiles, kThreads, 0, st>>>(t, parents, beams, groups, status);
+    else if (beams <= 16)
+        reorder_rows_kernel<U, 16><<<(unsigned)tiles, kThreads, 0, st>>>(t, parents, beams, groups, status);
+    else
+        reorder_rows_kernel<U, 32><<<(unsigned)tiles, kThreads, 0, st>>>(t, parents, beams, groups, status);
+    return launch_status();
+}
+
+}  // namespace
+}  // namespace bdm
+
+extern "C" int64_t bdm_beam_select_workspace_bytes(int64_t batch, int beams, int64_t vocab) {
+    using namespace bdm;
+    if (batch < 0 || beams <= 0 || vocab <= 0 || beams > kMaxBeams || vocab * beams >= 0xffffffffll) return -1;
+    const BeamPlan p = beam_plan(batch * beams, vocab);
+    return batch * beams * p.splits * ((int64_t)beams * 8 + 8);
+}
+
+extern "C" int bdm_beam_select(const void *logits, int64_t ld, int64_t batch, int beams, int64_t vocab, int dtype,
+                               const float *scores, const uint8_t *finished, int64_t eos_token, int stable_slots,
+                               float *out_scores, int64_t *out_parents, int64_t *out_tokens, uint8_t *out_finished,
+                               void *workspace, int64_t workspace_bytes, void *stream) {
+    using namespace bdm;
+    if (batch < 0 || beams <= 0 || vocab <= 0 || ld < 0 || eos_token < -1 || eos_token >= vocab) return BDM_ERR_INVALID;
+    if (finished && eos_token < 0) return BDM_ERR_INVALID;
+    if (!valid_dtype(dtype)) return BDM_ERR_DTYPE;
+    if (beams > kMaxBeams || vocab * beams >= 0xffffffffll) return BDM_ERR_UNSUPPORTED;
+    if (batch == 0) return BDM_OK;
+    if (!logits || !scores || !out_scores || !out_parents || !out_tokens) return BDM_ERR_INVALID;
+    const int64_t rows = batch * beams;
+    const BeamPlan p = beam_plan(rows, vocab);
+    if (!workspace || workspace_bytes < bdm_beam_select_workspace_bytes(batch, beams, vocab)) return BDM_ERR_WORKSPACE;
+    if (rows * p.splits > 0x7fffffff) return BDM_ERR_UNSUPPORTED;
+    cudaStream_t st = as_stream(stream);
+    u64 *lists = static_cast<u64 *>(workspace);
+    Slice *stat = reinterpret_cast<Slice *>(lists + rows * p.splits * beams);
+    const unsigned grid = (unsigned)(rows * p.splits);
+    BDM_DISPATCH_DTYPE(dtype, T, {
+        const T *x = static_cast<const T *>(logits);
+        const bool vec = (reinterpret_cast<uintptr_t>(logits) & 15) == 0 && (ld * (int64_t)sizeof(T)) % 16 == 0;
+        if (p.e == 32) {
+            if (vec)
+                beam_slice_kernel<T, 32, true><<<grid, kThreads, 0, st>>>(x, ld, (int)vocab, beams, p.splits, stat, lists);
+            else
+                beam_slice_kernel<T, 32, false><<<grid, kThreads, 0, st>>>(x, ld, (int)vocab, beams, p.splits, stat, lists);
+        } else {
+            if (vec)
+                beam_slice_kernel<T, 8, true><<<grid, kThreads, 0, st>>>(x, ld, (int)vocab, beams, p.splits, stat, lists);
+            else
+                beam_slice_kernel<T, 8, false><<<grid, kThreads, 0, st>>>(x, ld, (int)vocab, beams, p.splits, stat, lists);
+        }
+        if (int rc = launch_status()) return rc;
+        beam_merge_kernel<T><<<(unsigned)batch, kThreads, 0, st>>>(x, ld, scores, finished, eos_token, beams, (int)vocab,
+                                                                  p.splits, stable_slots, stat, lists, out_scores,
+                                                                  out_parents, out_tokens, out_finished);
+    });
+    return launch_status();
+}
+
+extern "C" int bdm_reorder_rows(void *const *bases, const int64_t *row_strides, const int64_t *row_bytes, int count,
+                                const int64_t *parents, int64_t groups, int beams, int *status, void *stream) {
+    using namespace bdm;
+    if (count < 0 || groups < 0 || beams <= 0) return BDM_ERR_INVALID;
+    if (beams > kMaxBeams) return BDM_ERR_UNSUPPORTED;
+    if (count == 0 || groups == 0) return BDM_OK;
+    if (!bases || !row_strides || !row_bytes || !parents) return BDM_ERR_INVALID;
+    for (int i = 0; i < count; ++i)
+        if (row_bytes[i] < 0 || row_strides[i] < row_bytes[i] || (row_bytes[i] && !bases[i])) return BDM_ERR_INVALID;
+    cudaStream_t st = as_stream(stream);
+    for (int width : {16, 4, 1}) {  // the widest access each tensor's rows allow
+        Tensors t{};
+        int64_t bytes[kMaxTensors];
+        auto flush = [&]() {
+            const int rc = t.count == 0 ? BDM_OK
+                           : width == 16 ? reorder_launch<uint4>(t, bytes, parents, groups, beams, status, st)
+                           : width == 4  ? reorder_launch<uint32_t>(t, bytes, parents, groups, beams, status, st)
+                                         : reorder_launch<uint8_t>(t, bytes, parents, groups, beams, status, st);
+            t.count = 0;
+            return rc;
+        };
+        for (int i = 0; i < count; ++i) {
+            const uint64_t bits = reinterpret_cast<uintptr_t>(bases[i]) | (uint64_t)row_strides[i] | (uint64_t)row_bytes[i];
+            const int fits = bits % 16 == 0 ? 16 : (bits % 4 == 0 ? 4 : 1);
+            if (fits != width || row_bytes[i] == 0) continue;
+            t.base[t.count] = bases[i];
+            t.stride[t.count] = row_strides[i];
+            bytes[t.count++] = row_bytes[i];
+            if (t.count == kMaxTensors)
+                if (int rc = flush()) return rc;
+        }
+        if (int rc = flush()) return rc;
+    }
+    return BDM_OK;
+}

@@ -1,0 +1,106 @@
+// Shared pieces of the decay-attention walk: parameters, the segmentation of the time axis, and the
+// state a segment starts from.
+//
+// Walk (per batch row and head, lam = exp(log_decay)), n valid tokens:
+//   forward:  out_t = scale * (sum_{s<=t} lam^(t-s) (a_t.b_s) c_s + lam^(t+1)   a_t X)
+//             Y     = lam^n X + sum_s lam^(n-1-s) b_s c_s^T
+//   reverse:  out_t = scale * (sum_{s>=t} lam^(s-t) (a_t.b_s) c_s + lam^(n-1-t) a_t X)
+//             Y     = lam^n X + sum_s lam^(s+1)   b_s c_s^T
+// X = state_in * state_in_mul, state_out = Y * state_out_mul.  o = forward(q, k, v); the gradients are
+// the same walk: dq = forward(do, v, k), dk = reverse(v, do, q), dv = reverse(k, q, do).
+//
+// In a chunk of kChunk tokens starting at t0, row r = t - t0 of n' = min(kChunk, n - t0) valid ones, the
+// exponents are: inside t-s (or s-t); reading the carried state r+1 (n'-1-r); writing it n'-1-r (r+1);
+// carrying it n'.  The time axis is cut into segments of whole chunks when there are too few (row, head)
+// pairs for the SMs: a first launch leaves every segment's own state (X = 0) in the workspace, and the
+// main launch starts each segment from the given state and its predecessors'.
+#pragma once
+
+#include "common.cuh"
+
+namespace bdm {
+namespace walk {
+
+constexpr int kChunk = 64;
+constexpr int kMaxWidth = 128;  // of a, b and of c: what one CTA's tiles hold
+// Below this log-decay a power is zero in FP32 from the first token on; clamping keeps 0 * -inf away.
+constexpr float kLogFloor = -1.0e4f;
+
+struct Params {
+    const void *a, *b, *c;
+    int64_t as[3], bs[3], cs[3], os[3];  // strides of batch, token, head (elements)
+    int ag, bg, cg;                      // heads sharing one head of a, b, c
+    void *out;
+    const float *log_decay;
+    const int64_t *lengths;
+    const float *state_in;
+    float *state_out;
+    float in_mul, out_mul;
+    int in_t, out_t;  // state stored [wc, wab] instead of [wab, wc]
+    float *seg;       // segment states, [batch*heads, nseg, wc, wab]
+    int64_t batch, time;
+    int heads, wab, wc, reverse;
+    float scale;
+    int nseg, cps;  // segments, chunks per segment
+    int *status;
+};
+
+__device__ __forceinline__ float head_log_decay(const Params &p, int h) {
+    const float g = p.log_decay[h];
+    return g < kLogFloor ? kLogFloor : g;
+}
+__device__ __forceinline__ int64_t row_tokens(const Params &p, int64_t b) {
+    if (!p.lengths) return p.time;
+    const int64_t n = p.lengths[b];
+    return n < 0 ? 0 : (n > p.time ? p.time : n);
+}
+
+// One segment of one row: its chunks [c0, c1), the row's chunks, and its place in the walk.
+struct Span {
+    int64_t n, c0, c1, chunks;
+    bool last;  // the walk ends here: this segment writes the final state
+};
+__device__ __forceinline__ Span span_of(const Params &p, int64_t n, int seg) {
+    Span s;
+    s.n = n;
+    s.chunks = (n + kChunk - 1) / kChunk;
+    s.c0 = (int64_t)seg * p.cps;
+    s.c1 = s.c0 + p.cps;
+    if (s.c0 > s.chunks) s.c0 = s.chunks;
+    if (s.c1 > s.chunks) s.c1 = s.chunks;
+    if (p.reverse || s.chunks == 0)
+        s.last = seg == 0;
+    else
+        s.last = s.c1 == s.chunks && s.c0 < s.c1;
+    return s;
+}
+
+// Element (i of wab, j of wc) of the state the segment starts from.
+__device__ __forceinline__ float start_state(const Params &p, const Span &s, int64_t bh, int seg, float g, int i, int j) {
+    const int64_t size = (int64_t)p.wab * p.wc;
+    float x = 0.f;
+    if (p.state_in) {
+        const int64_t end = s.c1 * kChunk < s.n ? s.c1 * kChunk : s.n;
+        const int64_t far = p.reverse ? s.n - end : s.c0 * kChunk;
+        const float v = p.state_in[bh * size + (p.in_t ? (int64_t)j * p.wab + i : (int64_t)i * p.wc + j)] * p.in_mul;
+        x = far ? v * expf(g * (float)far) : v;
+    }
+    if (p.nseg > 1) {
+        // predecessors in walk order, nearest last; all but the row's last segment are whole
+        const float *z = p.seg + (bh * p.nseg) * size + (int64_t)j * p.wab + i;
+        const float step = expf(g * (float)((int64_t)p.cps * kChunk));
+        float acc = 0.f;
+        if (!p.reverse) {
+            for (int q = 0; q < seg; ++q) acc = acc * step + z[q * size];
+        } else {
+            const int lastseg = (int)((s.chunks + p.cps - 1) / p.cps) - 1;
+            for (int q = lastseg; q > seg; --q) acc = acc * step + z[q * size];
+        }
+        x += acc;
+    }
+    return x;
+}
+
+}  // namespace walk
+
+}  // namespace bdm

@@ -1,0 +1,283 @@
+"""Decay attention: linear attention with a decay for each head, for prompts, training and single tokens.
+
+Per batch row and head, with lam = exp(log_decay[h]):
+
+    S_t = lam S_{t-1} + k_t v_t^T        o_t = scale * q_t S_t
+
+``decay_attention`` runs whole sequences chunk by chunk (differentiable), ``decay_attention_step`` one
+token against a resident state, and ``DecayAttention`` is the mixer layer around them, with the same
+``forward`` / ``prefill`` / ``step`` / ``create_state`` calls as the bank memory layer, so a language
+model can interleave the two (``HybridLanguageModel``).  There is no reference counterpart.
+"""
+from __future__ import annotations
+
+import ctypes
+import math
+from contextlib import nullcontext
+
+import torch
+from torch import nn
+from torch.nn import functional as F
+
+from . import _lib, ops
+
+
+def _on(device):
+    """The launches below go to the device of their tensors."""
+    return nullcontext() if device.index == torch.cuda.current_device() else torch.cuda.device(device)
+
+
+def _rows(x):
+    """Columns of a head contiguous; every other stride is free."""
+    return x if x.stride(-1) == 1 or x.shape[-1] == 1 else x.contiguous()
+
+
+_I3 = ctypes.c_int64 * 3
+_I2 = ctypes.c_int64 * 2
+
+
+def _walk(a, b, c, log_decay, lengths, *, heads, scale, reverse=False, out_dtype=None, state_in=None, state_in_mul=1.0,
+          state_in_transposed=False, state_out=None, state_out_mul=1.0, state_out_transposed=False):
+    """One bdm_decay_walk over [B, T, heads of the operand, width] tensors; returns out [B, T, heads, width of c]."""
+    batch, time = a.shape[:2]
+    out = torch.empty((batch, time, heads, c.shape[-1]), dtype=out_dtype or a.dtype, device=a.device)
+    w = _lib.DecayWalkArgs(
+        a.data_ptr(), b.data_ptr(), c.data_ptr(), out.data_ptr(), log_decay.data_ptr(), ops._ptr(lengths),
+        ops._ptr(state_in), ops._ptr(state_out), ops._scan_status_of(a.device).word.data_ptr(),
+        _I3(*a.stride()[:3]), _I3(*b.stride()[:3]), _I3(*c.stride()[:3]), _I3(*out.stride()[:3]), batch, time, heads,
+        a.shape[2], b.shape[2], c.shape[2], a.shape[3], c.shape[3], ops.dtype_code(a.dtype),
+        ops.dtype_code(out.dtype), int(reverse), int(state_in_transposed), int(state_out_transposed), scale,
+        state_in_mul, state_out_mul)
+    lib = _lib.load()
+    nbytes = lib.bdm_decay_walk_workspace_bytes(ctypes.byref(w))
+    if nbytes < 0:
+        raise ValueError('invalid decay-attention geometry')
+    ws = torch.empty(nbytes, dtype=torch.uint8, device=a.device) if nbytes else None
+    _lib.check(lib.bdm_decay_walk(ctypes.byref(w), ops._ptr(ws), nbytes, ops._stream(a.device)), 'bdm_decay_walk')
+    return out
+
+
+def _group_sum(part, kv_heads, dtype):
+    """[B, T, H, D] FP32 gradients per query head -> [B, T, kv_heads, D] in ``dtype``."""
+    batch, time, heads, width = part.shape
+    out = torch.empty((batch, time, kv_heads, width), dtype=dtype, device=part.device)
+    _lib.check(_lib.load().bdm_decay_group_sum(part.data_ptr(), batch * time, kv_heads, heads // kv_heads, width,
+                                               ops.dtype_code(dtype), out.data_ptr(), ops._stream(part.device)),
+               'bdm_decay_group_sum')
+    return out
+
+
+class _DecayAttention(torch.autograd.Function):
+    @staticmethod
+    def forward(ctx, q, k, v, log_decay, initial_state, lengths, scale):
+        q, k, v = _rows(q), _rows(k), _rows(v)
+        heads = q.shape[2]
+        state = torch.empty((q.shape[0], heads, q.shape[3], v.shape[3]), dtype=torch.float32, device=q.device)
+        with _on(q.device):
+            out = _walk(q, k, v, log_decay, lengths, heads=heads, scale=scale, state_in=initial_state, state_out=state)
+        ctx.save_for_backward(q, k, v, log_decay, initial_state, lengths)
+        ctx.scale = scale
+        ctx.set_materialize_grads(False)
+        return out, state
+
+    @staticmethod
+    @torch.autograd.function.once_differentiable
+    def backward(ctx, do, dstate):
+        q, k, v, log_decay, s0, lengths = ctx.saved_tensors
+        scale, heads, kv_heads, dt = ctx.scale, q.shape[2], k.shape[2], q.dtype
+        if do is None and dstate is None:
+            return (None,) * 7
+        do = _rows(do) if do is not None else torch.zeros_like(v[:, :, :1]).expand(-1, -1, heads, -1)
+        dstate = dstate.contiguous() if dstate is not None else None
+        need = ctx.needs_input_grad
+        dq = dk = dv = ds0 = None
+        shared = kv_heads != heads
+        walk = dict(heads=heads, scale=scale)
+        back = dict(walk, reverse=True, state_in=dstate, state_in_mul=1.0 / scale,
+                    out_dtype=torch.float32 if shared else dt)
+        with _on(q.device):
+            ops.check_scan_status(q.device)
+            if need[0]:
+                dq = _walk(do, v, k, log_decay, lengths, state_in=s0, state_in_transposed=True, **walk)
+            if need[1]:
+                dk = _walk(v, do, q, log_decay, lengths, state_in_transposed=True, **back)
+                dk = _group_sum(dk, kv_heads, dt) if shared else dk
+            if need[2] or need[4]:
+                ds0 = torch.empty((q.shape[0], heads, q.shape[3], v.shape[3]), dtype=torch.float32,
+                                  device=q.device) if need[4] else None
+                dv = _walk(k, q, do, log_decay, lengths, state_out=ds0, state_out_mul=scale, **back)
+                dv = _group_sum(dv, kv_heads, dt) if shared else dv
+        return dq, dk, dv if need[2] else None, None, ds0, None, None
+
+
+def _check_heads(q, k, v, log_decay, scale):
+    ops._cuda(q, k, v, log_decay)
+    if q.dtype != k.dtype or q.dtype != v.dtype:
+        raise ValueError('q, k and v must share one dtype')
+    ops.dtype_code(q.dtype)
+    if any(t.device != q.device for t in (k, v, log_decay)):
+        raise ValueError('q, k, v and log_decay must be on one device')
+    heads, kv_heads, dk = q.shape[-2], k.shape[-2], q.shape[-1]
+    if k.shape[-1] != dk or v.shape[-2] != kv_heads or k.shape[:-2] != q.shape[:-2] or v.shape[:-2] != q.shape[:-2]:
+        raise ValueError('k must be [..., kv_heads, key width of q] and v [..., kv_heads, value width], '
+                         'with the leading sizes of q')
+    if min(heads, kv_heads, dk, v.shape[-1]) < 1 or heads % kv_heads:
+        raise ValueError('the heads of q must be a multiple of the heads of k and v')
+    if log_decay.dtype != torch.float32 or tuple(log_decay.shape) != (heads,) or not log_decay.is_contiguous():
+        raise ValueError(f'log_decay must be a contiguous float32 [{heads}] tensor')
+    if log_decay.requires_grad and torch.is_grad_enabled():
+        raise ValueError('log_decay is a constant: it gets no gradient')
+    scale = dk ** -0.5 if scale is None else float(scale)
+    if not math.isfinite(scale) or scale == 0.0:
+        raise ValueError('scale must be finite and not 0')
+    return scale
+
+
+def _check_state(name, state, shape, device):
+    if state.dtype != torch.float32 or tuple(state.shape) != shape or state.device != device or not state.is_contiguous():
+        raise ValueError(f'{name} must be a contiguous float32 {list(shape)} tensor on {device}')
+
+
+def decay_attention(q, k, v, log_decay, *, scale=None, initial_state=None, lengths=None, return_state=False):
+    """Linear attention with a decay for each head over whole sequences.
+
+    q [B, T, H, dk], k [B, T, G, dk], v [B, T, G, dv] in float32 or bfloat16 (any strides; head h of q uses
+    head h // (H // G) of k and v); log_decay [H] float32, log of the decay per token, at most 0 in use;
+    dk, dv <= 128.  ``lengths`` (int64 [B]): tokens of row b from lengths[b] on are padding: not read, their
+    outputs and gradients 0, and the state stops before them.  ``scale`` defaults to dk ** -0.5.
+
+    Returns o [B, T, H, dv] in q's dtype, and with ``return_state`` (o, state [B, H, dk, dv] float32), the
+    state after each row's last valid token, starting from ``initial_state`` (zero if None).
+    Differentiable in q, k, v and initial_state, through o and the state.
+    """
+    if q.ndim != 4 or k.ndim != 4 or v.ndim != 4:
+        raise ValueError('q, k and v must be [batch, time, heads, width]')
+    scale = _check_heads(q, k, v, log_decay, scale)
+    batch = q.shape[0]
+    if initial_state is not None:
+        _check_state('initial_state', initial_state, (batch, q.shape[2], q.shape[3], v.shape[3]), q.device)
+    if lengths is not None and (lengths.dtype != torch.int64 or tuple(lengths.shape) != (batch,)
+                                or lengths.device != q.device or not lengths.is_contiguous()):
+        raise ValueError(f'lengths must be a contiguous int64 [{batch}] tensor on {q.device}')
+    if q.shape[3] > 128 or v.shape[3] > 128:
+        raise NotImplementedError('decay_attention supports head widths up to 128')
+    ops.check_scan_status(q.device)
+    out, state = _DecayAttention.apply(q, k, v, log_decay, initial_state, lengths, scale)
+    return (out, state) if return_state else out
+
+
+def decay_attention_step(q, k, v, log_decay, state, *, scale=None):
+    """One token per row: ``state`` [B, H, dk, dv] (float32) is advanced in place; returns o [B, H, dv].
+
+    q [B, H, dk], k [B, G, dk], v [B, G, dv] as one token of ``decay_attention``; dk <= 1024, any dv.
+    Not differentiable; requires no_grad or inference_mode where an input would need a gradient.
+    """
+    if q.ndim != 3 or k.ndim != 3 or v.ndim != 3:
+        raise ValueError('q, k and v must be [batch, heads, width]')
+    scale = _check_heads(q, k, v, log_decay, scale)
+    if torch.is_grad_enabled() and (q.requires_grad or k.requires_grad or v.requires_grad or state.requires_grad):
+        raise RuntimeError('decay_attention_step requires no_grad or inference_mode')
+    batch, heads, dk = q.shape
+    dv = v.shape[2]
+    _check_state('state', state, (batch, heads, dk, dv), q.device)
+    if dk > 1024:
+        raise NotImplementedError('decay_attention_step supports key widths up to 1024')
+    q, k, v = _rows(q), _rows(k), _rows(v)
+    out = torch.empty((batch, heads, dv), dtype=q.dtype, device=q.device)
+    a = _lib.DecayStepArgs(q.data_ptr(), k.data_ptr(), v.data_ptr(), log_decay.data_ptr(), state.data_ptr(),
+                           out.data_ptr(), _I2(*q.stride()[:2]), _I2(*k.stride()[:2]), _I2(*v.stride()[:2]), batch,
+                           heads, k.shape[1], dk, dv, ops.dtype_code(q.dtype), scale)
+    with _on(q.device):
+        _lib.check(_lib.load().bdm_decay_step(ctypes.byref(a), ops._stream(q.device)), 'bdm_decay_step')
+    return out
+
+
+class DecayAttention(nn.Module):
+    """Mixer layer of decay attention, a drop-in beside ``BankedDeltaMemory`` in a language-model block.
+
+    One projection gives q, k (SiLU, unit norm per head), v and an output gate; the heads' outputs are
+    RMS-normalised per head, gated by a sigmoid and projected back.  The decays are fixed: 1 - 2^-e with e
+    spread evenly over [min_exponent, max_exponent] across the heads.  ``forward`` / ``prefill`` / ``step``
+    / ``create_state`` mirror the bank memory layer's; the state is FP32 [B, H, key width, value width].
+    """
+
+    def __init__(self, dim, num_heads, *, key_width=None, value_width=None, kv_heads=None, min_exponent=3.0,
+                 max_exponent=9.0, norm_eps=1e-5, seed=0):
+        super().__init__()
+        kv_heads = num_heads if kv_heads is None else kv_heads
+        if min(dim, num_heads, kv_heads) < 1 or num_heads % kv_heads:
+            raise ValueError('num_heads must be a positive multiple of kv_heads')
+        if (key_width is None or value_width is None) and dim % num_heads:
+            raise ValueError('dim must be divisible by num_heads')
+        self.dim, self.num_heads, self.kv_heads = dim, num_heads, kv_heads
+        self.key_width, self.value_width = key_width or dim // num_heads, value_width or dim // num_heads
+        if self.key_width > 128 or self.value_width > 128:
+            raise NotImplementedError('decay attention supports head widths up to 128')
+        self.norm_eps = norm_eps
+        self._splits = [num_heads * self.key_width, kv_heads * self.key_width, kv_heads * self.value_width,
+                        num_heads * self.value_width]
+        with torch.random.fork_rng(devices=[]):  # init_weights below seeds them: the caller's generator stays
+            self.in_proj = nn.Linear(dim, sum(self._splits), bias=False)
+            self.o_proj = nn.Linear(num_heads * self.value_width, dim, bias=False)
+        self.norm_weight = nn.Parameter(torch.ones(num_heads * self.value_width))
+        exponent = torch.linspace(float(min_exponent), float(max_exponent), num_heads, dtype=torch.float64)
+        self._log_decay = torch.log1p(-torch.exp2(-exponent)).float()  # a constant: FP32 whatever the module's dtype
+        self._decay_on = {}
+        self.init_weights(initialization_seed=seed)
+
+    def init_weights(self, *, initialization_seed=0):
+        with torch.random.fork_rng(devices=[]):
+            torch.manual_seed(initialization_seed)
+            for w in (self.in_proj.weight, self.o_proj.weight):
+                nn.init.trunc_normal_(w, std=w.shape[1] ** -0.5, a=-3 * w.shape[1] ** -0.5, b=3 * w.shape[1] ** -0.5)
+        nn.init.ones_(self.norm_weight)
+
+    def log_decay(self, device):
+        """The heads' log-decays [H] on ``device`` (uploaded once per device)."""
+        if device not in self._decay_on:
+            with torch.inference_mode(False):
+                self._decay_on[device] = self._log_decay.to(device)
+        return self._decay_on[device]
+
+    def create_state(self, batch, *, device=None):
+        """A zero state for ``batch`` rows."""
+        device = self.in_proj.weight.device if device is None else device
+        return torch.zeros(batch, self.num_heads, self.key_width, self.value_width, device=device)
+
+    def _heads(self, hidden):
+        q, k, v, gate = self.in_proj(hidden).split(self._splits, -1)
+        lead = hidden.shape[:-1]
+        unit = lambda x, n: F.normalize(F.silu(x.reshape(*lead, n, self.key_width)), dim=-1, eps=1e-6)  # noqa: E731
+        return unit(q, self.num_heads), unit(k, self.kv_heads), v.reshape(*lead, self.kv_heads, self.value_width), gate
+
+    def _output(self, o, gate):
+        x = o.float()
+        x = (x * torch.rsqrt(x.square().mean(-1, keepdim=True) + self.norm_eps)).flatten(-2)
+        return self.o_proj((x * self.norm_weight.float() * torch.sigmoid(gate.float())).to(gate.dtype))
+
+    def forward(self, hidden, *, lengths=None):
+        """[B, T, dim] -> [B, T, dim] from a zero state; differentiable."""
+        q, k, v, gate = self._heads(hidden)
+        return self._output(decay_attention(q, k, v, self.log_decay(hidden.device), lengths=lengths), gate)
+
+    def prefill(self, hidden, state=None, *, lengths=None, state_dtype=None):
+        """Process a prefix [B, T, dim] -> (output, state); continues from ``state`` if given.
+
+        The state is always FP32: ``state_dtype`` (which picks the bank caches' storage) has no effect.
+        """
+        if torch.is_grad_enabled():
+            raise RuntimeError('prefill requires no_grad or inference_mode')
+        q, k, v, gate = self._heads(hidden)
+        o, state = decay_attention(q, k, v, self.log_decay(hidden.device), initial_state=state, lengths=lengths,
+                                   return_state=True)
+        return self._output(o, gate), state
+
+    def step(self, hidden, state):
+        """One token per row [B, 1, dim] -> (output [B, 1, dim], state); ``state`` is advanced in place."""
+        if torch.is_grad_enabled():
+            raise RuntimeError('step requires no_grad or inference_mode')
+        if hidden.ndim != 3 or hidden.shape[1] != 1:
+            raise ValueError('step takes one token per row: [batch, 1, dim]')
+        q, k, v, gate = self._heads(hidden[:, 0])
+        o = decay_attention_step(q, k, v, self.log_decay(hidden.device), state)
+        return self._output(o, gate)[:, None], state

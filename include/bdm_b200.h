@@ -461,6 +461,89 @@ BDM_API int bdm_decode_token_step(const void *proj, int64_t batch, int64_t ld, i
                                   const void *norm_weight, const void *norm_bias, float eps, int norm_mode,
                                   void *out, void *stream);
 
+/*
+ * Recurrent-decoder operators (no reference counterpart).
+ *
+ * Decay attention: linear attention with a decay lam = exp(log_decay[h]) for each head.  bdm_decay_walk is
+ * one walk over every row's n tokens (n = lengths[row] clamped to [0, time], or time), with a, b of
+ * width_ab and c of width_c columns per head:
+ *   forward (reverse = 0): out_t = scale * (sum_{s<=t} lam^(t-s) (a_t.b_s) c_s + lam^(t+1) a_t X)
+ *                          Y     = lam^n X + sum_s lam^(n-1-s) b_s c_s^T
+ *   reverse (reverse = 1): out_t = scale * (sum_{s>=t} lam^(s-t) (a_t.b_s) c_s + lam^(n-1-t) a_t X)
+ *                          Y     = lam^n X + sum_s lam^(s+1) b_s c_s^T
+ *   X = state_in * state_in_mul (0 if null), state_out = Y * state_out_mul (skipped if null).
+ * The attention is the forward walk of (q, k, v); its gradients are dq = forward(do, v, k),
+ * dk = reverse(v, do, q) and dv = reverse(k, q, do).  Outputs of rows past n are 0; nothing is read there.
+ * Strides are in elements, in the order batch, token, head; columns are contiguous.  Head h uses head
+ * h / (heads / x_heads) of operand x.  States are FP32 [batch, heads, width_ab, width_c], or with
+ * *_transposed [batch, heads, width_c, width_ab].  Products, sums and states are FP32.
+ * width_ab, width_c <= 128.  status (optional int): 0x4 is ORed in if a bounded wait gave up.
+ */
+typedef struct bdm_decay_walk_args {
+    const void *a, *b, *c;
+    void *out;
+    const float *log_decay;
+    const int64_t *lengths;
+    const float *state_in;
+    float *state_out;
+    int *status;
+    int64_t a_stride[3], b_stride[3], c_stride[3], out_stride[3];
+    int64_t batch, time;
+    int heads, a_heads, b_heads, c_heads;
+    int width_ab, width_c;
+    int dtype, out_dtype; /* out_dtype: dtype, or BDM_F32 */
+    int reverse;
+    int state_in_transposed, state_out_transposed;
+    float scale, state_in_mul, state_out_mul;
+} bdm_decay_walk_args;
+
+/* Workspace bytes of a walk (segment states; 0 for most shapes), -1 for invalid arguments. */
+BDM_API int64_t bdm_decay_walk_workspace_bytes(const bdm_decay_walk_args *args);
+BDM_API int bdm_decay_walk(const bdm_decay_walk_args *args, void *workspace, int64_t workspace_bytes, void *stream);
+
+/* out[t, g, d] (dtype) = sum_s part[t, g * group + s, d] (FP32, in order of s): gradients of shared heads. */
+BDM_API int bdm_decay_group_sum(const float *part, int64_t tokens, int groups, int group, int width, int dtype, void *out,
+                                void *stream);
+
+/*
+ * One token per row of decay attention: state <- lam state + k v^T in place (FP32 [batch, heads,
+ * key_width, value_width]), out = scale q state [batch, heads, value_width] (dtype).  Strides: batch, head.
+ */
+typedef struct bdm_decay_step_args {
+    const void *q, *k, *v;
+    const float *log_decay;
+    float *state;
+    void *out;
+    int64_t q_stride[2], k_stride[2], v_stride[2];
+    int64_t batch;
+    int heads, kv_heads, key_width, value_width, dtype;
+    float scale;
+} bdm_decay_step_args;
+BDM_API int bdm_decay_step(const bdm_decay_step_args *args, void *stream);
+
+/*
+ * Beam selection.  logits: batch * beams rows of vocab (dtype), ld apart (0: one row for all), scores [batch, beams] FP32.  Candidate (w, t) is
+ * scores[w] + ((logit - max) - log sum exp(. - max)) in FP32; a finished row's only candidate is (w, eos_token) with its
+ * score, the others are -inf.  NaN candidates (a row with NaN, +inf or no finite logit) rank as -inf.  The
+ * `beams` best per batch row, ties to the lower w * vocab + t, in descending order; with stable_slots the
+ * best child of each parent takes the parent's place and the others the free places in turn.
+ * finished (optional, bytes) needs eos_token >= 0; out_finished (optional) = the parent's | (token == eos).
+ * beams <= 32, beams * vocab < 2^32.
+ */
+BDM_API int64_t bdm_beam_select_workspace_bytes(int64_t batch, int beams, int64_t vocab);
+BDM_API int bdm_beam_select(const void *logits, int64_t ld, int64_t batch, int beams, int64_t vocab, int dtype,
+                            const float *scores, const uint8_t *finished, int64_t eos_token, int stable_slots,
+                            float *out_scores, int64_t *out_parents, int64_t *out_tokens, uint8_t *out_finished,
+                            void *workspace, int64_t workspace_bytes, void *stream);
+
+/*
+ * In place, for every tensor: row (g, i) <- row (g, parents[g, i]) of its groups * beams rows of row_bytes
+ * bytes, row_strides bytes apart.  bases, row_strides and row_bytes are host arrays of `count` entries.  A
+ * parent out of range keeps the row and ORs 0x8 into status (optional).  beams <= 32.
+ */
+BDM_API int bdm_reorder_rows(void *const *bases, const int64_t *row_strides, const int64_t *row_bytes, int count,
+                             const int64_t *parents, int64_t groups, int beams, int *status, void *stream);
+
 #ifdef __cplusplus
 }
 #endif
