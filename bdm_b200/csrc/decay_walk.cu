@@ -273,7 +273,7 @@ int64_t simt_segments(int64_t ctas, int64_t chunks, int sms) {
     return s < 1 ? 1 : s;
 }
 
-int plan(const bdm_decay_walk_args &w, Params &p, int sms) {
+int plan(const bdm_decay_walk_args &w, Params &p, bool &tc, int sms) {
     p.a = w.a, p.b = w.b, p.c = w.c, p.out = w.out;
     for (int i = 0; i < 3; ++i) {
         p.as[i] = w.a_stride[i];
@@ -293,7 +293,9 @@ int plan(const bdm_decay_walk_args &w, Params &p, int sms) {
     p.status = w.status;
     p.seg = nullptr;
     const int64_t chunks = ceil_div(w.time, kChunk) > 0 ? ceil_div(w.time, kChunk) : 1;
-    int64_t nseg = simt_segments(w.batch * w.heads * ceil_div(w.width_c, kCols), chunks, sms);
+    tc = decay_walk_tc_takes(w);
+    const int64_t nseg = tc ? decay_walk_tc_segments(w.batch * w.heads, chunks, sms)
+                            : simt_segments(w.batch * w.heads * ceil_div(w.width_c, kCols), chunks, sms);
     p.cps = (int)ceil_div(chunks, nseg);
     p.nseg = (int)ceil_div(chunks, p.cps);
     return BDM_OK;
@@ -325,7 +327,8 @@ extern "C" int64_t bdm_decay_walk_workspace_bytes(const bdm_decay_walk_args *w) 
     int sms = 0;
     if (device_setup(sms)) return -1;
     Params p{};
-    if (plan(*w, p, sms)) return -1;
+    bool tc = false;
+    if (plan(*w, p, tc, sms)) return -1;
     return seg_bytes(p);
 }
 
@@ -338,14 +341,17 @@ extern "C" int bdm_decay_walk(const bdm_decay_walk_args *w, void *workspace, int
     int sms = 0;
     if (int rc = device_setup(sms)) return rc;
     Params p{};
-    if (int rc = plan(*w, p, sms)) return rc;
+    bool tc = false;
+    if (int rc = plan(*w, p, tc, sms)) return rc;
     const int64_t need = seg_bytes(p);
     if (need > workspace_bytes || (need && !workspace)) return BDM_ERR_WORKSPACE;
     p.seg = static_cast<float *>(workspace);
     cudaStream_t st = as_stream(stream);
     for (int pass = p.nseg > 1 ? 0 : 1; pass < 2; ++pass) {
         int rc;
-        if (w->dtype == BDM_F32)
+        if (tc)
+            rc = decay_walk_tc_launch(*w, p, pass == 0, st);
+        else if (w->dtype == BDM_F32)
             rc = simt_launch<float, float>(p, pass == 0, st);
         else if (w->out_dtype == BDM_F32)
             rc = simt_launch<bf16, float>(p, pass == 0, st);

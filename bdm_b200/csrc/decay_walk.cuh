@@ -103,4 +103,9 @@ __device__ __forceinline__ float start_state(const Params &p, const Span &s, int
 
 }  // namespace walk
 
+// The tensor-core walk (decay_walk_tc.cu): BF16 operands that TMA can address.
+bool decay_walk_tc_takes(const bdm_decay_walk_args &w);
+int64_t decay_walk_tc_segments(int64_t rows, int64_t chunks, int sms);
+int decay_walk_tc_launch(const bdm_decay_walk_args &w, const walk::Params &p, bool state_only, cudaStream_t st);
+
 }  // namespace bdm

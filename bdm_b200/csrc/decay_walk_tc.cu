@@ -1,0 +1,590 @@
+// Decay attention on the tensor cores: the walk of decay_walk.cuh for BF16 operands.
+//
+// One CTA walks the 64-token chunks of one segment of one (row, head).  Everything is computed transposed,
+// so that the state's and the outputs' value columns are the 128 lanes of tensor memory and every product
+// has M = 128:
+//   A    = Qa Kb^T                 [i, j]   operands as TMA leaves them (K-major)
+//   P    = A * lam^(i-j), masked   -> BF16 in shared memory, [i][j]
+//   O1^T = Vc^T P^T                [dv, i]  Vc read MN-major
+//   O2^T = S^T Qa^T                [dv, i]  S^T is a BF16 operand in tensor memory
+//   T^T  = V'^T Kb                 [dv, dk] V' = lam^. Vc as three BF16 terms in tensor memory, Kb MN-major
+//   out  = scale (O1 + lam^. O2),   S <- lam^n S + T
+// The state itself stays in registers in FP32.  Roundings to BF16: P and the copy of S that is read (one
+// rounding each, as large as the output's own); V' is split into three terms (24 bits), so that T, and with
+// it the state over any number of chunks, is exact to FP32.
+//
+// Roles (16 warps): 0-7 scale V' and carry the state (thread = value column, half of the key columns),
+// 8-11 the outputs, 12-13 P, 14 TMA, 15 MMA.  Every wait is bounded; one that gives up sets the status bit
+// and lets the CTA drain.
+#include "decay_walk.cuh"
+#include "tcgen05.cuh"
+
+#include <cuda.h>
+
+#include <mutex>
+
+namespace bdm {
+namespace {
+
+using namespace walk;
+
+constexpr int kThreads = 512;
+constexpr int kBox = 64 * 128;  // bytes of a TMA box: 64 tokens x 64 BF16 columns
+constexpr int kStateWarps = 8, kOutWarp = 8, kScoreWarp = 12, kTmaWarp = 14, kMmaWarp = 15;
+constexpr int kMaxStages = 8;
+constexpr int kSmemMax = 227 * 1024;
+constexpr unsigned long long kWaitNs = 2000000000ull;
+
+// tensor memory columns
+constexpr uint32_t kColA = 0, kColO1 = 64, kColO2 = 128, kColT = 192, kColS = 320, kColV = 384;
+
+struct Maps {
+    CUtensorMap a, b, c;
+};
+struct TcParams {
+    Params p;
+    int amul[3], bmul[3];  // 0 where the operand's batch (head) is shared by all: a, b, c
+    int stages;
+};
+
+struct Bars {
+    uint64_t full[kMaxStages], empty[kMaxStages];
+    uint64_t sready, tdone, adone, pready, odone, ofree;
+};
+
+__device__ __forceinline__ uint32_t pack_bf16(float lo, float hi) {
+    uint32_t r;
+    asm("cvt.rn.bf16x2.f32 %0, %1, %2;\n" : "=r"(r) : "f"(hi), "f"(lo));
+    return r;
+}
+__device__ __forceinline__ float bf16_lo(uint32_t r) { return __uint_as_float(r << 16); }
+__device__ __forceinline__ float bf16_hi(uint32_t r) { return __uint_as_float(r & 0xffff0000u); }
+
+// The state the segment starts from, key columns [k0, k0 + KC) of value column `col` (see start_state).
+template <int KC>
+__device__ __forceinline__ void start_states(const Params &p, const Span &s, int64_t bh, int seg, float g, int k0, int col,
+                                             float (&S)[KC]) {
+    const int64_t size = (int64_t)p.wab * p.wc;
+    if (p.nseg > 1) {
+        const float step = expf(g * (float)((int64_t)p.cps * kChunk));
+        const int far = p.reverse ? (int)((s.chunks + p.cps - 1) / p.cps) - 1 : 0;
+        const int count = p.reverse ? far - seg : seg;
+        const float *z = p.seg + (bh * p.nseg + far) * size + (int64_t)col * p.wab + k0;
+        for (int q = 0; q < count; ++q, z += p.reverse ? -size : size)
+#pragma unroll
+            for (int i = 0; i < KC; ++i)
+                if (k0 + i < p.wab) S[i] = fmaf(S[i], step, z[i]);
+    }
+    if (p.state_in) {
+        const int64_t end = s.c1 * kChunk < s.n ? s.c1 * kChunk : s.n;
+        const int64_t far = p.reverse ? s.n - end : s.c0 * kChunk;
+        const float w = (far ? expf(g * (float)far) : 1.f) * p.in_mul;
+        const float *x = p.state_in + bh * size;
+#pragma unroll
+        for (int i = 0; i < KC; ++i)
+            if (k0 + i < p.wab)
+                S[i] = fmaf(w, x[p.in_t ? (int64_t)col * p.wab + k0 + i : (int64_t)(k0 + i) * p.wc + col], S[i]);
+    }
+}
+
+// DKB, VB: 64-column boxes of a / b and of c.
+template <int DKB, int VB, typename OT, bool STATE_ONLY>
+__global__ void __launch_bounds__(kThreads, 1) decay_walk_tc_kernel(const TcParams tp, const __grid_constant__ Maps maps) {
+    extern __shared__ char raw[];
+    __shared__ Bars bar;
+    __shared__ float pw[kChunk + 1];
+    __shared__ uint32_t tmem_slot;
+    __shared__ volatile int dead;
+    const Params &p = tp.p;
+    const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+    char *smem = reinterpret_cast<char *>((reinterpret_cast<uintptr_t>(raw) + 1023) & ~(uintptr_t)1023);
+    constexpr int kStage = (STATE_ONLY ? DKB + VB : 2 * DKB + VB) * kBox;
+    constexpr int kOffB = STATE_ONLY ? 0 : DKB * kBox, kOffC = kOffB + DKB * kBox;
+    constexpr int DK = DKB * 64;
+    const int stages = tp.stages;
+    char *sP = smem + stages * kStage;
+
+    int64_t id = blockIdx.x;
+    const int seg = (int)(id % p.nseg);
+    const int64_t bh = id / p.nseg;
+    const int64_t b = bh / p.heads;
+    const int h = (int)(bh % p.heads);
+    const float g = head_log_decay(p, h);
+    const Span sp = span_of(p, row_tokens(p, b), seg);
+    const int steps = (int)(sp.c1 - sp.c0);
+
+    if (threadIdx.x <= kChunk) pw[threadIdx.x] = threadIdx.x ? expf(g * (float)threadIdx.x) : 1.f;
+    if (threadIdx.x == 0) {
+        dead = 0;
+        for (int i = 0; i < stages; ++i) {
+            tc::mbar_init(&bar.full[i], 1);
+            tc::mbar_init(&bar.empty[i], 1);
+        }
+        tc::mbar_init(&bar.sready, kStateWarps);
+        tc::mbar_init(&bar.tdone, 1);
+        tc::mbar_init(&bar.adone, 1);
+        tc::mbar_init(&bar.pready, 2);
+        tc::mbar_init(&bar.odone, 1);
+        tc::mbar_init(&bar.ofree, 4);
+        tc::mbar_fence_init();
+    }
+    if (warp == kMmaWarp) tc::tmem_alloc(&tmem_slot, 512);
+    tc::fence_before_sync();
+    __syncthreads();
+    tc::fence_after_sync();
+    const uint32_t tmem = tmem_slot;
+
+    // bounded wait; false once any wait of the CTA has given up
+    auto wait = [&](uint64_t *m, unsigned parity) -> bool {
+        if (tc::mbar_test(m, parity)) return true;
+        if (dead) return false;
+        const unsigned long long t0 = tc::global_ns();
+        for (long long i = 0; i < (1ll << 26); ++i) {
+            if (tc::mbar_test(m, parity)) return true;
+            if ((i & 63) == 63 && (dead || tc::global_ns() - t0 > kWaitNs)) break;
+        }
+        dead = 1;
+        return false;
+    };
+    // the same for a whole warp, with one answer for its lanes
+    auto wait_warp = [&](uint64_t *m, unsigned parity) -> bool { return __all_sync(0xffffffffu, wait(m, parity)); };
+    auto chunk_of = [&](int n) -> int64_t { return p.reverse ? sp.c1 - 1 - n : sp.c0 + n; };
+    auto valid_of = [&](int64_t ch) -> int {
+        const int64_t left = sp.n - ch * kChunk;
+        return (int)(left < kChunk ? left : kChunk);
+    };
+
+    if (warp < kStateWarps) {
+        // ------------------------------------------------------- V' and the state
+        const int quad = warp & 3, half = warp >> 2;
+        const int col = quad * 32 + lane;                  // value column = tensor-memory lane
+        const uint32_t lanes = (uint32_t)(quad * 32) << 16;
+        constexpr int KC = DK / 2;                         // key columns of this thread
+        const int k0 = half * KC;
+        const bool mine = quad < 2 * VB;
+        float S[KC];
+#pragma unroll
+        for (int i = 0; i < KC; ++i) S[i] = 0.f;
+        if (!STATE_ONLY && col < p.wc) start_states<KC>(p, sp, bh, seg, g, k0, col, S);
+        bool ok = true;
+        int before = 0;  // valid tokens of the previous chunk
+        for (int n = 0; n <= steps && ok; ++n) {
+            const int st = n % stages;
+            const int64_t ch = chunk_of(n);
+            const int valid = n < steps ? valid_of(ch) : 0;
+            uint32_t v3[3][8];
+            // 16 tokens of V' as packed BF16 terms: j0 .. j0 + 15
+            auto scale16 = [&](int j0) {
+                const char *src = smem + st * kStage + kOffC + (col >> 6) * kBox + (col & 7) * 2;
+                const int chunk = (col & 63) >> 3;
+#pragma unroll
+                for (int u = 0; u < 8; ++u) {
+                    float x[2];
+#pragma unroll
+                    for (int e = 0; e < 2; ++e) {
+                        const int j = j0 + 2 * u + e;
+                        const unsigned short raw16 =
+                            *reinterpret_cast<const unsigned short *>(src + j * 128 + ((chunk ^ (j & 7)) << 4));
+                        const float f = __uint_as_float((uint32_t)raw16 << 16);
+                        const int w = p.reverse ? j + 1 : valid - 1 - j;
+                        x[e] = j < valid ? f * pw[w < 0 ? 0 : w] : 0.f;
+                    }
+                    const uint32_t hi = pack_bf16(x[0], x[1]);
+                    const float r0 = x[0] - bf16_lo(hi), r1 = x[1] - bf16_hi(hi);
+                    const uint32_t mid = pack_bf16(r0, r1);
+                    v3[0][u] = hi;
+                    v3[1][u] = mid;
+                    v3[2][u] = pack_bf16(r0 - bf16_lo(mid), r1 - bf16_hi(mid));
+                }
+            };
+            auto store16 = [&](int j0) {
+#pragma unroll
+                for (int t = 0; t < 3; ++t) tc::tmem_st8(tmem + lanes + kColV + t * 32 + j0 / 2, v3[t]);
+            };
+            if (n < steps) {
+                ok = wait_warp(&bar.full[st], (n / stages) & 1);
+                if (!ok) break;
+                if (valid < kChunk && ch * kChunk + valid < p.time) {
+                    // tokens past the row's length may hold anything: zero them for the products over j
+                    uint4 *kb = reinterpret_cast<uint4 *>(smem + st * kStage + kOffB);
+                    for (int i = threadIdx.x; i < (DKB + VB) * kBox / 16; i += kStateWarps * 32)
+                        if ((i % (kBox / 16)) / 8 >= valid) kb[i] = make_uint4(0, 0, 0, 0);
+                    tc::fence_async_smem();
+                }
+                if (mine) scale16(half * 32);
+            }
+            if (n > 0) {
+                ok = wait_warp(&bar.tdone, (n - 1) & 1);
+                if (!ok) break;
+                tc::fence_after_sync();
+            }
+            if (n < steps && mine) {
+                store16(half * 32);
+                scale16(half * 32 + 16);
+                store16(half * 32 + 16);
+            }
+            if (n > 0 && mine) {
+                const float carry = pw[before];
+#pragma unroll
+                for (int i = 0; i < KC; i += 16) {
+                    float t[16];
+                    tc::tmem_ld16(tmem + lanes + kColT + k0 + i, t);
+                    tc::tmem_wait_ld();
+#pragma unroll
+                    for (int e = 0; e < 16; ++e) S[i + e] = fmaf(carry, S[i + e], t[e]);
+                }
+            }
+            before = valid;
+            if (n == steps) break;
+            if (!STATE_ONLY) {
+                if (n > 0) {
+                    ok = wait_warp(&bar.odone, (n - 1) & 1);  // the last chunk's reads of S are over
+                    if (!ok) break;
+                    tc::fence_after_sync();
+                }
+                if (mine)
+#pragma unroll
+                    for (int i = 0; i < KC; i += 16) {
+                        uint32_t r[8];
+#pragma unroll
+                        for (int e = 0; e < 8; ++e) r[e] = pack_bf16(S[i + 2 * e], S[i + 2 * e + 1]);
+                        tc::tmem_st8(tmem + lanes + kColS + (k0 + i) / 2, r);
+                    }
+            }
+            tc::tmem_wait_st();
+            tc::fence_before_sync();
+            __syncwarp();
+            if (lane == 0) tc::mbar_arrive(&bar.sready);
+        }
+        if (ok && col < p.wc) {
+            const int64_t size = (int64_t)p.wab * p.wc;
+            if (STATE_ONLY) {
+                float *z = p.seg + (bh * p.nseg + seg) * size + (int64_t)col * p.wab;
+#pragma unroll
+                for (int i = 0; i < KC; ++i)
+                    if (k0 + i < p.wab) z[k0 + i] = S[i];
+            } else if (p.state_out && sp.last) {
+                float *z = p.state_out + bh * size;
+#pragma unroll
+                for (int i = 0; i < KC; ++i)
+                    if (k0 + i < p.wab)
+                        z[p.out_t ? (int64_t)col * p.wab + k0 + i : (int64_t)(k0 + i) * p.wc + col] = S[i] * p.out_mul;
+            }
+        }
+    } else if (warp < kScoreWarp) {
+        // ------------------------------------------------------------- outputs
+        if constexpr (!STATE_ONLY) {
+            const int quad = warp & 3;
+            const int col = quad * 32 + lane;
+            const uint32_t lanes = (uint32_t)(quad * 32) << 16;
+            const bool on = col < p.wc;
+            OT *out = static_cast<OT *>(p.out) + b * p.os[0] + h * p.os[2] + col;
+            for (int n = 0; n < steps; ++n) {
+                if (!wait_warp(&bar.odone, n & 1)) break;
+                tc::fence_after_sync();
+                float x[64];
+                if (quad < 2 * VB) {
+                    float y[16];
+#pragma unroll
+                    for (int i = 0; i < 64; i += 16) tc::tmem_ld16(tmem + lanes + kColO2 + i, *reinterpret_cast<float(*)[16]>(x + i));
+                    const int64_t ch = chunk_of(n);
+                    const int valid = valid_of(ch);
+                    tc::tmem_wait_ld();
+#pragma unroll
+                    for (int i = 0; i < 64; i += 16) {
+                        tc::tmem_ld16(tmem + lanes + kColO1 + i, y);
+                        tc::tmem_wait_ld();
+#pragma unroll
+                        for (int e = 0; e < 16; ++e) {
+                            const int r = i + e;
+                            const int w = p.reverse ? (valid - 1 - r < 0 ? 0 : valid - 1 - r) : r + 1;
+                            x[r] = p.scale * fmaf(pw[w], x[r], y[e]);
+                        }
+                    }
+                }
+                tc::fence_before_sync();
+                __syncwarp();
+                if (lane == 0) tc::mbar_arrive(&bar.ofree);
+                if (on) {
+                    const int64_t t0 = chunk_of(n) * kChunk;
+                    const int valid = valid_of(chunk_of(n));
+                    const int rows = (int)(p.time - t0 < kChunk ? p.time - t0 : kChunk);
+                    OT *o = out + t0 * p.os[1];
+#pragma unroll
+                    for (int r = 0; r < 64; ++r)
+                        if (r < rows) o[r * p.os[1]] = Elem<OT>::from_float(r < valid ? x[r] : 0.f);
+                }
+            }
+            // whole chunks past the row's length
+            int64_t z0 = sp.chunks * kChunk, z1 = p.time;
+            const int64_t s0 = (int64_t)seg * p.cps * kChunk, s1 = s0 + (int64_t)p.cps * kChunk;
+            if (z0 < s0) z0 = s0;
+            if (z1 > s1) z1 = s1;
+            if (on)
+                for (int64_t t = z0; t < z1; ++t) out[t * p.os[1]] = Elem<OT>::from_float(0.f);
+        }
+    } else if (warp < kTmaWarp) {
+        // -------------------------------------------------- decayed scores P (rows 0..63)
+        if constexpr (!STATE_ONLY) {
+            const int quad = warp & 3;  // 0 or 1
+            const int row = quad * 32 + lane;
+            const uint32_t lanes = (uint32_t)(quad * 32) << 16;
+            for (int n = 0; n < steps; ++n) {
+                if (!wait_warp(&bar.adone, n & 1)) break;
+                tc::fence_after_sync();
+                const int valid = valid_of(chunk_of(n));  // scores of later tokens may be anything
+                uint32_t r[32];
+#pragma unroll
+                for (int i = 0; i < 64; i += 16) {
+                    float x[16];
+                    tc::tmem_ld16(tmem + lanes + kColA + i, x);
+                    tc::tmem_wait_ld();
+#pragma unroll
+                    for (int e = 0; e < 16; ++e) {
+                        const int d = p.reverse ? i + e - row : row - (i + e);
+                        const float w = pw[d < 0 ? 0 : d];
+                        x[e] = d >= 0 && i + e < valid ? x[e] * w : 0.f;
+                    }
+#pragma unroll
+                    for (int e = 0; e < 8; ++e) r[i / 2 + e] = pack_bf16(x[2 * e], x[2 * e + 1]);
+                }
+                if (n > 0 && !wait_warp(&bar.odone, (n - 1) & 1)) break;
+#pragma unroll
+                for (int c = 0; c < 8; ++c)
+                    *reinterpret_cast<uint4 *>(sP + row * 128 + ((c ^ (row & 7)) << 4)) =
+                        make_uint4(r[4 * c], r[4 * c + 1], r[4 * c + 2], r[4 * c + 3]);
+                tc::fence_async_smem();
+                tc::fence_before_sync();
+                __syncwarp();
+                if (lane == 0) tc::mbar_arrive(&bar.pready);
+            }
+        }
+    } else if (warp == kTmaWarp) {
+        // ------------------------------------------------------------------ loads
+        if (lane == 0) {
+            int issued = 0;
+            for (int n = 0; n < steps; ++n) {
+                const int st = n % stages;
+                if (n >= stages && !wait(&bar.empty[st], ((n / stages) - 1) & 1)) break;
+                char *dst = smem + st * kStage;
+                const int t0 = (int)(chunk_of(n) * kChunk);
+                tc::mbar_arrive_expect_tx(&bar.full[st], kStage);
+                if (!STATE_ONLY)
+#pragma unroll
+                    for (int i = 0; i < DKB; ++i)
+                        tc::tma_load_4d(dst + i * kBox, &maps.a, i * 64, t0, (h / p.ag) * tp.bmul[0], (int)b * tp.amul[0],
+                                        &bar.full[st]);
+#pragma unroll
+                for (int i = 0; i < DKB; ++i)
+                    tc::tma_load_4d(dst + kOffB + i * kBox, &maps.b, i * 64, t0, (h / p.bg) * tp.bmul[1],
+                                    (int)b * tp.amul[1], &bar.full[st]);
+#pragma unroll
+                for (int i = 0; i < VB; ++i)
+                    tc::tma_load_4d(dst + kOffC + i * kBox, &maps.c, i * 64, t0, (h / p.cg) * tp.bmul[2],
+                                    (int)b * tp.amul[2], &bar.full[st]);
+                issued = n + 1;
+            }
+            // no copy may be in flight when the CTA ends, whatever happened to its consumers
+            for (int n = issued > stages ? issued - stages : 0; n < issued; ++n)
+                tc::mbar_wait(&bar.full[n % stages], (n / stages) & 1, kWaitNs);
+        }
+    } else {
+        // --------------------------------------------------------------- products
+        if (lane == 0) {
+            constexpr uint32_t idQK = tc::idesc_bf16(128, 64);
+            constexpr uint32_t idO1 = tc::idesc_bf16(128, 64) | tc::kIdescMnA;
+            constexpr uint32_t idO2 = tc::idesc_bf16(128, 64);
+            constexpr uint32_t idT = tc::idesc_bf16(128, DK) | tc::kIdescMnB;
+            const uint32_t base = tc::smem_u32(smem), pbase = tc::smem_u32(sP);
+            auto scores = [&](int n) {  // rows 64..127 of the product are whatever follows the tile
+                const uint32_t qa = base + (n % stages) * kStage, kb = qa + kOffB;
+#pragma unroll
+                for (int k = 0; k < DK / 16; ++k)
+                    tc::mma_bf16(tmem + kColA, tc::smem_desc_sw128(qa + (k / 4) * kBox + (k % 4) * 32),
+                                 tc::smem_desc_sw128(kb + (k / 4) * kBox + (k % 4) * 32), idQK, k > 0);
+                tc::mma_commit(&bar.adone);
+            };
+            bool ok = true;
+            int done = 0;
+            if (!STATE_ONLY && steps > 0) {
+                ok = wait(&bar.full[0], 0);
+                if (ok) scores(0);
+            }
+            for (int n = 0; n < steps && ok; ++n) {
+                const int st = n % stages;
+                const uint32_t qa = base + st * kStage, kb = qa + kOffB, vc = qa + kOffC;
+                if (!(ok = wait(&bar.sready, n & 1))) break;
+                tc::fence_after_sync();
+#pragma unroll
+                for (int t = 0; t < 3; ++t)
+#pragma unroll
+                    for (int k = 0; k < 4; ++k)
+                        tc::mma_bf16_tmem_a(tmem + kColT, tmem + kColV + t * 32 + k * 8,
+                                            tc::smem_desc_sw128_mn(kb + k * 2048, kBox), idT, t + k > 0);
+                tc::mma_commit(&bar.tdone);
+                if (!STATE_ONLY) {
+                    if (!(ok = wait(&bar.pready, n & 1))) break;
+                    if (n > 0 && !(ok = wait(&bar.ofree, (n - 1) & 1))) break;
+                    tc::fence_after_sync();
+                    if (n + 1 < steps) {
+                        if (!(ok = wait(&bar.full[(n + 1) % stages], ((n + 1) / stages) & 1))) break;
+                        scores(n + 1);
+                    }
+#pragma unroll
+                    for (int k = 0; k < DK / 16; ++k)
+                        tc::mma_bf16_tmem_a(tmem + kColO2, tmem + kColS + k * 8,
+                                            tc::smem_desc_sw128(qa + (k / 4) * kBox + (k % 4) * 32), idO2, k > 0);
+#pragma unroll
+                    for (int k = 0; k < 4; ++k)
+                        tc::mma_bf16(tmem + kColO1, tc::smem_desc_sw128_mn(vc + k * 2048, kBox),
+                                     tc::smem_desc_sw128(pbase + k * 32), idO1, k > 0);
+                    tc::mma_commit(&bar.odone);
+                }
+                tc::mma_commit(&bar.empty[st]);
+                done = n + 1;
+            }
+            // nor a product
+            if (done) tc::mbar_wait(&bar.empty[(done - 1) % stages], ((done - 1) / stages) & 1, kWaitNs);
+        }
+    }
+    __syncwarp();
+    tc::fence_before_sync();
+    __syncthreads();
+    if (threadIdx.x == 0 && dead && p.status) atomicOr(p.status, 0x4);
+    if (warp == kMmaWarp) {
+        tc::fence_after_sync();
+        tc::tmem_dealloc(tmem, 512);
+    }
+}
+
+using EncodeTiled = CUresult (*)(CUtensorMap *, CUtensorMapDataType, cuuint32_t, void *, const cuuint64_t *,
+                                 const cuuint64_t *, const cuuint32_t *, const cuuint32_t *, CUtensorMapInterleave,
+                                 CUtensorMapSwizzle, CUtensorMapL2promotion, CUtensorMapFloatOOBfill);
+
+EncodeTiled encode_tiled() {
+    static EncodeTiled fn = [] {
+        void *f = nullptr;
+        cudaDriverEntryPointQueryResult q{};
+        if (cudaGetDriverEntryPoint("cuTensorMapEncodeTiled", &f, cudaEnableDefault, &q) != cudaSuccess ||
+            q != cudaDriverEntryPointSuccess)
+            return static_cast<EncodeTiled>(nullptr);
+        return reinterpret_cast<EncodeTiled>(f);
+    }();
+    return fn;
+}
+
+struct Operand {
+    const void *ptr;
+    const int64_t *stride;
+    int width, heads;
+};
+
+// Columns, tokens, heads, batch; a dimension every index of which is the same memory becomes one of size 1.
+bool fits_tma(const Operand &o, int64_t time, int64_t batch) {
+    if (reinterpret_cast<uintptr_t>(o.ptr) & 15) return false;
+    const int64_t size[3] = {batch, time, o.heads};
+    for (int i = 0; i < 3; ++i) {
+        if (size[i] == 1) continue;
+        if (o.stride[i] == 0 && i != 1) continue;
+        if (o.stride[i] <= 0 || o.stride[i] % 8 || o.stride[i] * 2 >= ((int64_t)1 << 40)) return false;
+        if (size[i] > 0x7fffffff) return false;
+    }
+    return true;
+}
+bool encode(EncodeTiled fn, CUtensorMap *m, const Operand &o, int64_t time, int64_t batch, int &amul, int &bmul) {
+    amul = batch > 1 && o.stride[0] != 0;
+    bmul = o.heads > 1 && o.stride[2] != 0;
+    const cuuint64_t dims[4] = {(cuuint64_t)o.width, (cuuint64_t)time, (cuuint64_t)(bmul ? o.heads : 1),
+                                (cuuint64_t)(amul ? batch : 1)};
+    const cuuint64_t any = ((cuuint64_t)o.width * 2 + 15) / 16 * 16;  // of dimensions of size 1: nothing uses it
+    const cuuint64_t strides[3] = {time > 1 ? (cuuint64_t)o.stride[1] * 2 : any, bmul ? (cuuint64_t)o.stride[2] * 2 : any,
+                                   amul ? (cuuint64_t)o.stride[0] * 2 : any};
+    const cuuint32_t box[4] = {64, kChunk, 1, 1}, estr[4] = {1, 1, 1, 1};
+    return fn(m, CU_TENSOR_MAP_DATA_TYPE_BFLOAT16, 4, const_cast<void *>(o.ptr), dims, strides, box, estr,
+              CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B,
+              CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) == CUDA_SUCCESS;
+}
+
+template <int DKB, int VB> constexpr int stages_of(bool state_only) {
+    const int stage = (state_only ? DKB + VB : 2 * DKB + VB) * kBox;
+    int n = (kSmemMax - 1024 - 3072 - kBox) / stage;
+    return n > kMaxStages ? kMaxStages : n;
+}
+
+template <int DKB, int VB, typename OT, bool STATE_ONLY> int launch(TcParams &tp, const Maps &maps, cudaStream_t st) {
+    tp.stages = stages_of<DKB, VB>(STATE_ONLY);
+    const int smem = tp.stages * (STATE_ONLY ? DKB + VB : 2 * DKB + VB) * kBox + kBox + 1024;
+    auto kernel = decay_walk_tc_kernel<DKB, VB, OT, STATE_ONLY>;
+    constexpr int kMaxDevices = 64;
+    static std::mutex mu;
+    static bool set[kMaxDevices];
+    int dev = 0;
+    if (int rc = cuda_status(cudaGetDevice(&dev))) return rc;
+    if (dev < 0 || dev >= kMaxDevices) return BDM_ERR_UNSUPPORTED;
+    {
+        std::lock_guard<std::mutex> lock(mu);
+        if (!set[dev]) {
+            if (int rc = cuda_status(cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, smem))) return rc;
+            set[dev] = true;
+        }
+    }
+    const int64_t blocks = tp.p.batch * tp.p.heads * tp.p.nseg;
+    if (blocks > 0x7fffffff) return BDM_ERR_UNSUPPORTED;
+    kernel<<<(unsigned)blocks, kThreads, smem, st>>>(tp, maps);
+    return launch_status();
+}
+
+template <int DKB, int VB> int launch_types(TcParams &tp, const Maps &maps, bool out_f32, bool state_only, cudaStream_t st) {
+    if (state_only) return launch<DKB, VB, bf16, true>(tp, maps, st);
+    if (out_f32) return launch<DKB, VB, float, false>(tp, maps, st);
+    return launch<DKB, VB, bf16, false>(tp, maps, st);
+}
+
+}  // namespace
+
+bool decay_walk_tc_takes(const bdm_decay_walk_args &w) {
+    if (w.dtype != BDM_BF16 || w.time <= 0 || w.time > 0x7fffffff - kChunk) return false;
+    const Operand ops[3] = {{w.a, w.a_stride, w.width_ab, w.a_heads},
+                            {w.b, w.b_stride, w.width_ab, w.b_heads},
+                            {w.c, w.c_stride, w.width_c, w.c_heads}};
+    for (const Operand &o : ops)
+        if (!fits_tma(o, w.time, w.batch)) return false;
+    return encode_tiled() != nullptr;
+}
+
+// Segments of the time axis: the count that makes the two launches shortest, in units of one chunk of the
+// main walk.  A CTA has an SM to itself; its start and end cost about three chunks, a chunk of the state
+// launch about half of one, and a segment start reads all its predecessors' states.
+int64_t decay_walk_tc_segments(int64_t rows, int64_t chunks, int sms) {
+    int64_t best = 1;
+    double cost = 0;
+    for (int64_t s = 1; s <= chunks / 4 + 1 && s <= 64 && (s == 1 || rows * (s - 1) < sms); ++s) {
+        const int64_t cps = ceil_div(chunks, s), waves = ceil_div(rows * s, sms);
+        const double c = waves * (cps + 3.0 + (s > 1 ? 0.5 * cps + 5.0 + 0.2 * s : 0.0));
+        if (s == 1 || c < cost) cost = c, best = s;
+    }
+    return best;
+}
+
+int decay_walk_tc_launch(const bdm_decay_walk_args &w, const Params &p, bool state_only, cudaStream_t st) {
+    EncodeTiled fn = encode_tiled();
+    if (!fn) return BDM_ERR_UNSUPPORTED;
+    TcParams tp{};
+    tp.p = p;
+    Maps maps;
+    const Operand ops[3] = {{w.a, w.a_stride, w.width_ab, w.a_heads},
+                            {w.b, w.b_stride, w.width_ab, w.b_heads},
+                            {w.c, w.c_stride, w.width_c, w.c_heads}};
+    CUtensorMap *m[3] = {&maps.a, &maps.b, &maps.c};
+    for (int i = 0; i < 3; ++i)
+        if (!encode(fn, m[i], ops[i], w.time, w.batch, tp.amul[i], tp.bmul[i])) return BDM_ERR_UNSUPPORTED;
+    const bool f32 = w.out_dtype == BDM_F32;
+    if (p.wab > 64) {
+        if (p.wc > 64) return launch_types<2, 2>(tp, maps, f32, state_only, st);
+        return launch_types<2, 1>(tp, maps, f32, state_only, st);
+    }
+    if (p.wc > 64) return launch_types<1, 2>(tp, maps, f32, state_only, st);
+    return launch_types<1, 1>(tp, maps, f32, state_only, st);
+}
+
+}  // namespace bdm
