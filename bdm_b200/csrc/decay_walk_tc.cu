@@ -4,18 +4,19 @@
 // so that the state's and the outputs' value columns are the 128 lanes of tensor memory and every product
 // has M = 128:
 //   A    = Qa Kb^T                 [i, j]   operands as TMA leaves them (K-major)
-//   P    = A * lam^(i-j), masked   -> BF16 in shared memory, [i][j]
+//   P    = scale A * lam^(i-j), masked      -> BF16 in shared memory, [i][j]
 //   O1^T = Vc^T P^T                [dv, i]  Vc read MN-major
 //   O2^T = S^T Qa^T                [dv, i]  S^T is a BF16 operand in tensor memory
-//   T^T  = V'^T Kb                 [dv, dk] V' = lam^. Vc as three BF16 terms in tensor memory, Kb MN-major
-//   out  = scale (O1 + lam^. O2),   S <- lam^n S + T
+//   T^T  = V'^T Kb                 [dv, dk] V' = lam^. Vc as three BF16 terms in shared memory, both MN-major
+//   out  = O1 + scale lam^. O2,    S <- lam^n S + T
 // The state itself stays in registers in FP32.  Roundings to BF16: P and the copy of S that is read (one
 // rounding each, as large as the output's own); V' is split into three terms (24 bits), so that T, and with
 // it the state over any number of chunks, is exact to FP32.
 //
-// Roles (16 warps): 0-7 scale V' and carry the state (thread = value column, half of the key columns),
-// 8-11 the outputs, 12-13 P, 14 TMA, 15 MMA.  Every wait is bounded; one that gives up sets the status bit
-// and lets the CTA drain.
+// Roles (16 warps): 0-7 carry the state (thread = value column, half of the key columns) and scale V',
+// 8-11 the outputs, 12-13 P, 14 TMA, 15 MMA.  The cycle of a chunk is T(n) -> state update and V'(n+1) ->
+// T(n+1); O2, O1 and the next A fill the tensor pipe in between.  Every wait is bounded; one that gives up
+// sets the status bit and lets the CTA drain.
 #include "decay_walk.cuh"
 #include "tcgen05.cuh"
 
@@ -33,10 +34,11 @@ constexpr int kBox = 64 * 128;  // bytes of a TMA box: 64 tokens x 64 BF16 colum
 constexpr int kStateWarps = 8, kOutWarp = 8, kScoreWarp = 12, kTmaWarp = 14, kMmaWarp = 15;
 constexpr int kMaxStages = 8;
 constexpr int kSmemMax = 227 * 1024;
+constexpr long long kWaitCycles = 4000000000ll;  // about 2 s
 constexpr unsigned long long kWaitNs = 2000000000ull;
 
 // tensor memory columns
-constexpr uint32_t kColA = 0, kColO1 = 64, kColO2 = 128, kColT = 192, kColS = 320, kColV = 384;
+constexpr uint32_t kColA = 0, kColO1 = 64, kColO2 = 128, kColT = 192, kColS = 320;
 
 struct Maps {
     CUtensorMap a, b, c;
@@ -49,7 +51,7 @@ struct TcParams {
 
 struct Bars {
     uint64_t full[kMaxStages], empty[kMaxStages];
-    uint64_t sready, tdone, adone, pready, odone, ofree;
+    uint64_t vready, sready, tdone, adone, pready, odone, ofree;
 };
 
 __device__ __forceinline__ uint32_t pack_bf16(float lo, float hi) {
@@ -57,8 +59,46 @@ __device__ __forceinline__ uint32_t pack_bf16(float lo, float hi) {
     asm("cvt.rn.bf16x2.f32 %0, %1, %2;\n" : "=r"(r) : "f"(hi), "f"(lo));
     return r;
 }
+// Two FP32 values in one register pair, for the packed FP32 instructions.
+struct F2 {
+    unsigned long long v;
+};
+__device__ __forceinline__ F2 make2(float x, float y) {
+    F2 r;
+    asm("mov.b64 %0, {%1, %2};\n" : "=l"(r.v) : "f"(x), "f"(y));
+    return r;
+}
+__device__ __forceinline__ float2 split2(F2 a) {
+    float2 r;
+    asm("mov.b64 {%0, %1}, %2;\n" : "=f"(r.x), "=f"(r.y) : "l"(a.v));
+    return r;
+}
+__device__ __forceinline__ F2 fma2(F2 a, F2 b, F2 c) {
+    F2 r;
+    asm("fma.rn.f32x2 %0, %1, %2, %3;\n" : "=l"(r.v) : "l"(a.v), "l"(b.v), "l"(c.v));
+    return r;
+}
+__device__ __forceinline__ F2 mul2(F2 a, F2 b) {
+    F2 r;
+    asm("mul.rn.f32x2 %0, %1, %2;\n" : "=l"(r.v) : "l"(a.v), "l"(b.v));
+    return r;
+}
+__device__ __forceinline__ uint32_t pack2(F2 a) {
+    const float2 x = split2(a);
+    return pack_bf16(x.x, x.y);
+}
 __device__ __forceinline__ float bf16_lo(uint32_t r) { return __uint_as_float(r << 16); }
 __device__ __forceinline__ float bf16_hi(uint32_t r) { return __uint_as_float(r & 0xffff0000u); }
+__device__ __forceinline__ F2 unpack2(uint32_t r) { return make2(bf16_lo(r), bf16_hi(r)); }
+// Two values as three BF16 terms each.
+__device__ __forceinline__ void three_terms(F2 x, uint32_t &hi, uint32_t &mid, uint32_t &lo) {
+    const F2 minus = make2(-1.f, -1.f);
+    hi = pack2(x);
+    x = fma2(unpack2(hi), minus, x);
+    mid = pack2(x);
+    x = fma2(unpack2(mid), minus, x);
+    lo = pack2(x);
+}
 
 // The state the segment starts from, key columns [k0, k0 + KC) of value column `col` (see start_state).
 template <int KC>
@@ -92,7 +132,7 @@ template <int DKB, int VB, typename OT, bool STATE_ONLY>
 __global__ void __launch_bounds__(kThreads, 1) decay_walk_tc_kernel(const TcParams tp, const __grid_constant__ Maps maps) {
     extern __shared__ char raw[];
     __shared__ Bars bar;
-    __shared__ float pw[kChunk + 1];
+    __shared__ float pw[kChunk + 1], spw[kChunk + 2];  // lam^m, scale lam^m
     __shared__ uint32_t tmem_slot;
     __shared__ volatile int dead;
     const Params &p = tp.p;
@@ -103,6 +143,7 @@ __global__ void __launch_bounds__(kThreads, 1) decay_walk_tc_kernel(const TcPara
     constexpr int DK = DKB * 64;
     const int stages = tp.stages;
     char *sP = smem + stages * kStage;
+    char *sV = sP + kBox;  // V', three terms
 
     int64_t id = blockIdx.x;
     const int seg = (int)(id % p.nseg);
@@ -113,13 +154,17 @@ __global__ void __launch_bounds__(kThreads, 1) decay_walk_tc_kernel(const TcPara
     const Span sp = span_of(p, row_tokens(p, b), seg);
     const int steps = (int)(sp.c1 - sp.c0);
 
-    if (threadIdx.x <= kChunk) pw[threadIdx.x] = threadIdx.x ? expf(g * (float)threadIdx.x) : 1.f;
+    if (threadIdx.x <= kChunk) {
+        pw[threadIdx.x] = threadIdx.x ? expf(g * (float)threadIdx.x) : 1.f;
+        spw[threadIdx.x] = p.scale * pw[threadIdx.x];
+    }
     if (threadIdx.x == 0) {
         dead = 0;
         for (int i = 0; i < stages; ++i) {
             tc::mbar_init(&bar.full[i], 1);
             tc::mbar_init(&bar.empty[i], 1);
         }
+        tc::mbar_init(&bar.vready, kStateWarps);
         tc::mbar_init(&bar.sready, kStateWarps);
         tc::mbar_init(&bar.tdone, 1);
         tc::mbar_init(&bar.adone, 1);
@@ -137,11 +182,10 @@ __global__ void __launch_bounds__(kThreads, 1) decay_walk_tc_kernel(const TcPara
     // bounded wait; false once any wait of the CTA has given up
     auto wait = [&](uint64_t *m, unsigned parity) -> bool {
         if (tc::mbar_test(m, parity)) return true;
-        if (dead) return false;
-        const unsigned long long t0 = tc::global_ns();
-        for (long long i = 0; i < (1ll << 26); ++i) {
-            if (tc::mbar_test(m, parity)) return true;
-            if ((i & 63) == 63 && (dead || tc::global_ns() - t0 > kWaitNs)) break;
+        const long long t0 = clock64();
+        for (int i = 0; i < (1 << 28); ++i) {
+            if (tc::mbar_test_for(m, parity, 1000)) return true;
+            if ((i & 15) == 15 && (dead || clock64() - t0 > kWaitCycles)) break;
         }
         dead = 1;
         return false;
@@ -162,45 +206,22 @@ __global__ void __launch_bounds__(kThreads, 1) decay_walk_tc_kernel(const TcPara
         constexpr int KC = DK / 2;                         // key columns of this thread
         const int k0 = half * KC;
         const bool mine = quad < 2 * VB;
-        float S[KC];
+        F2 S[KC / 2];
+        {
+            float x[KC];
 #pragma unroll
-        for (int i = 0; i < KC; ++i) S[i] = 0.f;
-        if (!STATE_ONLY && col < p.wc) start_states<KC>(p, sp, bh, seg, g, k0, col, S);
+            for (int i = 0; i < KC; ++i) x[i] = 0.f;
+            if (!STATE_ONLY && col < p.wc) start_states<KC>(p, sp, bh, seg, g, k0, col, x);
+#pragma unroll
+            for (int i = 0; i < KC / 2; ++i) S[i] = make2(x[2 * i], x[2 * i + 1]);
+        }
         bool ok = true;
         int before = 0;  // valid tokens of the previous chunk
         for (int n = 0; n <= steps && ok; ++n) {
             const int st = n % stages;
             const int64_t ch = chunk_of(n);
             const int valid = n < steps ? valid_of(ch) : 0;
-            uint32_t v3[3][8];
-            // 16 tokens of V' as packed BF16 terms: j0 .. j0 + 15
-            auto scale16 = [&](int j0) {
-                const char *src = smem + st * kStage + kOffC + (col >> 6) * kBox + (col & 7) * 2;
-                const int chunk = (col & 63) >> 3;
-#pragma unroll
-                for (int u = 0; u < 8; ++u) {
-                    float x[2];
-#pragma unroll
-                    for (int e = 0; e < 2; ++e) {
-                        const int j = j0 + 2 * u + e;
-                        const unsigned short raw16 =
-                            *reinterpret_cast<const unsigned short *>(src + j * 128 + ((chunk ^ (j & 7)) << 4));
-                        const float f = __uint_as_float((uint32_t)raw16 << 16);
-                        const int w = p.reverse ? j + 1 : valid - 1 - j;
-                        x[e] = j < valid ? f * pw[w < 0 ? 0 : w] : 0.f;
-                    }
-                    const uint32_t hi = pack_bf16(x[0], x[1]);
-                    const float r0 = x[0] - bf16_lo(hi), r1 = x[1] - bf16_hi(hi);
-                    const uint32_t mid = pack_bf16(r0, r1);
-                    v3[0][u] = hi;
-                    v3[1][u] = mid;
-                    v3[2][u] = pack_bf16(r0 - bf16_lo(mid), r1 - bf16_hi(mid));
-                }
-            };
-            auto store16 = [&](int j0) {
-#pragma unroll
-                for (int t = 0; t < 3; ++t) tc::tmem_st8(tmem + lanes + kColV + t * 32 + j0 / 2, v3[t]);
-            };
+            uint4 raw[2 * VB];  // the chunk's values, 8 columns of a token each
             if (n < steps) {
                 ok = wait_warp(&bar.full[st], (n / stages) & 1);
                 if (!ok) break;
@@ -209,33 +230,52 @@ __global__ void __launch_bounds__(kThreads, 1) decay_walk_tc_kernel(const TcPara
                     uint4 *kb = reinterpret_cast<uint4 *>(smem + st * kStage + kOffB);
                     for (int i = threadIdx.x; i < (DKB + VB) * kBox / 16; i += kStateWarps * 32)
                         if ((i % (kBox / 16)) / 8 >= valid) kb[i] = make_uint4(0, 0, 0, 0);
-                    tc::fence_async_smem();
                 }
-                if (mine) scale16(half * 32);
+                // rows past `valid` are zero by now: their own thread, this one, has zeroed them
+                const uint4 *vc = reinterpret_cast<const uint4 *>(smem + st * kStage + kOffC);
+#pragma unroll
+                for (int u = 0; u < 2 * VB; ++u) raw[u] = vc[threadIdx.x + u * 256];
             }
             if (n > 0) {
                 ok = wait_warp(&bar.tdone, (n - 1) & 1);
                 if (!ok) break;
                 tc::fence_after_sync();
-            }
-            if (n < steps && mine) {
-                store16(half * 32);
-                scale16(half * 32 + 16);
-                store16(half * 32 + 16);
-            }
-            if (n > 0 && mine) {
-                const float carry = pw[before];
+                if (mine) {
+                    const F2 carry = make2(pw[before], pw[before]);
 #pragma unroll
-                for (int i = 0; i < KC; i += 16) {
-                    float t[16];
-                    tc::tmem_ld16(tmem + lanes + kColT + k0 + i, t);
-                    tc::tmem_wait_ld();
+                    for (int i = 0; i < KC; i += 16) {
+                        float t[16];
+                        tc::tmem_ld16(tmem + lanes + kColT + k0 + i, t);
+                        tc::tmem_wait_ld();
 #pragma unroll
-                    for (int e = 0; e < 16; ++e) S[i + e] = fmaf(carry, S[i + e], t[e]);
+                        for (int e = 0; e < 8; ++e) S[i / 2 + e] = fma2(carry, S[i / 2 + e], make2(t[2 * e], t[2 * e + 1]));
+                    }
                 }
             }
             before = valid;
             if (n == steps) break;
+            // V' has the layout of the tile: the same place in each term's buffer
+#pragma unroll
+            for (int u = 0; u < 2 * VB; ++u) {
+                const int i = threadIdx.x + u * 256;
+                const int j = (i % 512) / 8;
+                const int e = p.reverse ? j + 1 : valid - 1 - j;
+                const float w = pw[e < 0 ? 0 : e];
+                const F2 ww = make2(w, w);
+                uint4 t0, t1, t2;
+                three_terms(mul2(ww, unpack2(raw[u].x)), t0.x, t1.x, t2.x);
+                three_terms(mul2(ww, unpack2(raw[u].y)), t0.y, t1.y, t2.y);
+                three_terms(mul2(ww, unpack2(raw[u].z)), t0.z, t1.z, t2.z);
+                three_terms(mul2(ww, unpack2(raw[u].w)), t0.w, t1.w, t2.w);
+                uint4 *dst = reinterpret_cast<uint4 *>(sV) + i;
+                dst[0] = t0;
+                dst[VB * kBox / 16] = t1;
+                dst[2 * VB * kBox / 16] = t2;
+            }
+            tc::fence_async_smem();
+            tc::fence_before_sync();
+            __syncwarp();
+            if (lane == 0) tc::mbar_arrive(&bar.vready);
             if (!STATE_ONLY) {
                 if (n > 0) {
                     ok = wait_warp(&bar.odone, (n - 1) & 1);  // the last chunk's reads of S are over
@@ -244,31 +284,32 @@ __global__ void __launch_bounds__(kThreads, 1) decay_walk_tc_kernel(const TcPara
                 }
                 if (mine)
 #pragma unroll
-                    for (int i = 0; i < KC; i += 16) {
-                        uint32_t r[8];
+                    for (int i = 0; i < KC; i += 32) {
+                        uint32_t r[16];
 #pragma unroll
-                        for (int e = 0; e < 8; ++e) r[e] = pack_bf16(S[i + 2 * e], S[i + 2 * e + 1]);
-                        tc::tmem_st8(tmem + lanes + kColS + (k0 + i) / 2, r);
+                        for (int e = 0; e < 16; ++e) r[e] = pack2(S[i / 2 + e]);
+                        tc::tmem_st16(tmem + lanes + kColS + (k0 + i) / 2, r);
                     }
+                tc::tmem_wait_st();
+                tc::fence_before_sync();
+                __syncwarp();
+                if (lane == 0) tc::mbar_arrive(&bar.sready);
             }
-            tc::tmem_wait_st();
-            tc::fence_before_sync();
-            __syncwarp();
-            if (lane == 0) tc::mbar_arrive(&bar.sready);
         }
         if (ok && col < p.wc) {
             const int64_t size = (int64_t)p.wab * p.wc;
+            auto at = [&](int i) { return i & 1 ? split2(S[i / 2]).y : split2(S[i / 2]).x; };
             if (STATE_ONLY) {
                 float *z = p.seg + (bh * p.nseg + seg) * size + (int64_t)col * p.wab;
 #pragma unroll
                 for (int i = 0; i < KC; ++i)
-                    if (k0 + i < p.wab) z[k0 + i] = S[i];
+                    if (k0 + i < p.wab) z[k0 + i] = at(i);
             } else if (p.state_out && sp.last) {
                 float *z = p.state_out + bh * size;
 #pragma unroll
                 for (int i = 0; i < KC; ++i)
                     if (k0 + i < p.wab)
-                        z[p.out_t ? (int64_t)col * p.wab + k0 + i : (int64_t)(k0 + i) * p.wc + col] = S[i] * p.out_mul;
+                        z[p.out_t ? (int64_t)col * p.wab + k0 + i : (int64_t)(k0 + i) * p.wc + col] = at(i) * p.out_mul;
             }
         }
     } else if (warp < kScoreWarp) {
@@ -278,41 +319,72 @@ __global__ void __launch_bounds__(kThreads, 1) decay_walk_tc_kernel(const TcPara
             const int col = quad * 32 + lane;
             const uint32_t lanes = (uint32_t)(quad * 32) << 16;
             const bool on = col < p.wc;
-            OT *out = static_cast<OT *>(p.out) + b * p.os[0] + h * p.os[2] + col;
+            OT *out = static_cast<OT *>(p.out) + b * p.os[0] + h * p.os[2];
+            // 4-byte stores of two columns where every token's row allows them
+            const bool wide = ((reinterpret_cast<uintptr_t>(p.out) & 3) | ((p.os[0] | p.os[1] | p.os[2]) & 1)) == 0;
             for (int n = 0; n < steps; ++n) {
                 if (!wait_warp(&bar.odone, n & 1)) break;
                 tc::fence_after_sync();
-                float x[64];
+                const int64_t t0 = chunk_of(n) * kChunk;
+                const int valid = valid_of(chunk_of(n));
+                F2 x[32];
                 if (quad < 2 * VB) {
-                    float y[16];
-#pragma unroll
-                    for (int i = 0; i < 64; i += 16) tc::tmem_ld16(tmem + lanes + kColO2 + i, *reinterpret_cast<float(*)[16]>(x + i));
-                    const int64_t ch = chunk_of(n);
-                    const int valid = valid_of(ch);
-                    tc::tmem_wait_ld();
+                    // scale lam^. of 16 tokens per step, from the last to the first in the reverse walk
 #pragma unroll
                     for (int i = 0; i < 64; i += 16) {
-                        tc::tmem_ld16(tmem + lanes + kColO1 + i, y);
+                        float y[16], z[16];
+                        tc::tmem_ld16(tmem + lanes + kColO2 + i, y);
+                        tc::tmem_ld16(tmem + lanes + kColO1 + i, z);
                         tc::tmem_wait_ld();
 #pragma unroll
-                        for (int e = 0; e < 16; ++e) {
+                        for (int e = 0; e < 16; e += 2) {
                             const int r = i + e;
-                            const int w = p.reverse ? (valid - 1 - r < 0 ? 0 : valid - 1 - r) : r + 1;
-                            x[r] = p.scale * fmaf(pw[w], x[r], y[e]);
+                            F2 w;
+                            if (p.reverse)
+                                w = make2(spw[valid > r ? valid - 1 - r : 0], spw[valid > r + 1 ? valid - 2 - r : 0]);
+                            else
+                                w = make2(spw[r + 1], spw[r + 2]);
+                            x[r / 2] = fma2(w, make2(y[e], y[e + 1]), make2(z[e], z[e + 1]));
                         }
                     }
                 }
                 tc::fence_before_sync();
                 __syncwarp();
                 if (lane == 0) tc::mbar_arrive(&bar.ofree);
-                if (on) {
-                    const int64_t t0 = chunk_of(n) * kChunk;
-                    const int valid = valid_of(chunk_of(n));
-                    const int rows = (int)(p.time - t0 < kChunk ? p.time - t0 : kChunk);
-                    OT *o = out + t0 * p.os[1];
+                const int rows = (int)(p.time - t0 < kChunk ? p.time - t0 : kChunk);
+                if (valid < kChunk)  // padding gives zeros
 #pragma unroll
-                    for (int r = 0; r < 64; ++r)
-                        if (r < rows) o[r * p.os[1]] = Elem<OT>::from_float(r < valid ? x[r] : 0.f);
+                    for (int r = 0; r < 64; r += 2) {
+                        const float2 v = split2(x[r / 2]);
+                        x[r / 2] = make2(r < valid ? v.x : 0.f, r + 1 < valid ? v.y : 0.f);
+                    }
+                if constexpr (sizeof(OT) == 4) {
+                    OT *o = out + t0 * p.os[1] + col;
+                    if (on)
+#pragma unroll
+                        for (int r = 0; r < 64; ++r)
+                            if (r < rows) o[r * p.os[1]] = r & 1 ? split2(x[r / 2]).y : split2(x[r / 2]).x;
+                } else {
+                    // neighbouring lanes swap halves, so that a lane stores two columns of one token: the even
+                    // lane of the even tokens, the odd lane of the odd ones
+                    const int odd = lane & 1, pair = col & ~1;
+                    OT *o = out + (t0 + odd) * p.os[1] + pair;
+                    const bool both = wide && pair + 1 < p.wc;
+#pragma unroll
+                    for (int r = 0; r < 64; r += 2) {
+                        const uint32_t own = pack2(x[r / 2]), other = __shfl_xor_sync(0xffffffffu, own, 1);
+                        const uint32_t v = __byte_perm(odd ? other : own, odd ? own : other, odd ? 0x7632 : 0x5410);
+                        if (r + odd < rows) {
+                            OT *d = o + r * p.os[1];
+                            if (both) {
+                                *reinterpret_cast<uint32_t *>(d) = v;
+                            } else if (pair < p.wc) {
+                                const __nv_bfloat162 q = *reinterpret_cast<const __nv_bfloat162 *>(&v);
+                                d[0] = q.x;
+                                if (pair + 1 < p.wc) d[1] = q.y;
+                            }
+                        }
+                    }
                 }
             }
             // whole chunks past the row's length
@@ -321,7 +393,7 @@ __global__ void __launch_bounds__(kThreads, 1) decay_walk_tc_kernel(const TcPara
             if (z0 < s0) z0 = s0;
             if (z1 > s1) z1 = s1;
             if (on)
-                for (int64_t t = z0; t < z1; ++t) out[t * p.os[1]] = Elem<OT>::from_float(0.f);
+                for (int64_t t = z0; t < z1; ++t) out[t * p.os[1] + col] = Elem<OT>::from_float(0.f);
         }
     } else if (warp < kTmaWarp) {
         // -------------------------------------------------- decayed scores P (rows 0..63)
@@ -329,10 +401,23 @@ __global__ void __launch_bounds__(kThreads, 1) decay_walk_tc_kernel(const TcPara
             const int quad = warp & 3;  // 0 or 1
             const int row = quad * 32 + lane;
             const uint32_t lanes = (uint32_t)(quad * 32) << 16;
+            // the row's weights: the same for every chunk that is full
+            F2 w[32];
+            auto weights = [&](int valid) {  // scores of tokens past the row's length may be anything
+#pragma unroll
+                for (int j = 0; j < 64; j += 2) {
+                    const int d0 = p.reverse ? j - row : row - j, d1 = p.reverse ? d0 + 1 : d0 - 1;
+                    w[j / 2] = make2(d0 >= 0 && j < valid ? spw[d0 < 0 ? 0 : d0] : 0.f,
+                                     d1 >= 0 && j + 1 < valid ? spw[d1 < 0 ? 0 : d1] : 0.f);
+                }
+            };
+            int held = kChunk;
+            weights(held);
             for (int n = 0; n < steps; ++n) {
+                const int valid = valid_of(chunk_of(n));
+                if (valid != held) weights(held = valid);
                 if (!wait_warp(&bar.adone, n & 1)) break;
                 tc::fence_after_sync();
-                const int valid = valid_of(chunk_of(n));  // scores of later tokens may be anything
                 uint32_t r[32];
 #pragma unroll
                 for (int i = 0; i < 64; i += 16) {
@@ -340,13 +425,13 @@ __global__ void __launch_bounds__(kThreads, 1) decay_walk_tc_kernel(const TcPara
                     tc::tmem_ld16(tmem + lanes + kColA + i, x);
                     tc::tmem_wait_ld();
 #pragma unroll
-                    for (int e = 0; e < 16; ++e) {
-                        const int d = p.reverse ? i + e - row : row - (i + e);
-                        const float w = pw[d < 0 ? 0 : d];
-                        x[e] = d >= 0 && i + e < valid ? x[e] * w : 0.f;
+                    for (int e = 0; e < 16; e += 2) {
+                        const F2 f = w[(i + e) / 2];
+                        const float2 ff = split2(f);
+                        // a masked score may be NaN: select, do not multiply
+                        const float2 y = split2(mul2(f, make2(x[e], x[e + 1])));
+                        r[(i + e) / 2] = pack_bf16(ff.x != 0.f ? y.x : 0.f, ff.y != 0.f ? y.y : 0.f);
                     }
-#pragma unroll
-                    for (int e = 0; e < 8; ++e) r[i / 2 + e] = pack_bf16(x[2 * e], x[2 * e + 1]);
                 }
                 if (n > 0 && !wait_warp(&bar.odone, (n - 1) & 1)) break;
 #pragma unroll
@@ -394,14 +479,19 @@ __global__ void __launch_bounds__(kThreads, 1) decay_walk_tc_kernel(const TcPara
             constexpr uint32_t idQK = tc::idesc_bf16(128, 64);
             constexpr uint32_t idO1 = tc::idesc_bf16(128, 64) | tc::kIdescMnA;
             constexpr uint32_t idO2 = tc::idesc_bf16(128, 64);
-            constexpr uint32_t idT = tc::idesc_bf16(128, DK) | tc::kIdescMnB;
-            const uint32_t base = tc::smem_u32(smem), pbase = tc::smem_u32(sP);
-            auto scores = [&](int n) {  // rows 64..127 of the product are whatever follows the tile
-                const uint32_t qa = base + (n % stages) * kStage, kb = qa + kOffB;
+            constexpr uint32_t idT = tc::idesc_bf16(128, DK) | tc::kIdescMnA | tc::kIdescMnB;
+            // descriptors of the buffers' starts; an offset adds its bytes / 16 to the low word
+            const uint32_t base = tc::smem_u32(smem);
+            const uint64_t dP = tc::smem_desc_sw128(tc::smem_u32(sP));
+            const uint64_t dV = tc::smem_desc_sw128_mn(tc::smem_u32(sV), kBox);
+            // rows 64..127 of the scores, and value columns past c's boxes, are whatever follows the tile
+            auto scores = [&](int n) {
+                const uint64_t qa = tc::smem_desc_sw128(base + (n % stages) * kStage), kb = qa + kOffB / 16;
 #pragma unroll
-                for (int k = 0; k < DK / 16; ++k)
-                    tc::mma_bf16(tmem + kColA, tc::smem_desc_sw128(qa + (k / 4) * kBox + (k % 4) * 32),
-                                 tc::smem_desc_sw128(kb + (k / 4) * kBox + (k % 4) * 32), idQK, k > 0);
+                for (int k = 0; k < DK / 16; ++k) {
+                    const uint32_t off = ((k / 4) * kBox + (k % 4) * 32) / 16;
+                    tc::mma_bf16(tmem + kColA, qa + off, kb + off, idQK, k > 0);
+                }
                 tc::mma_commit(&bar.adone);
             };
             bool ok = true;
@@ -412,36 +502,38 @@ __global__ void __launch_bounds__(kThreads, 1) decay_walk_tc_kernel(const TcPara
             }
             for (int n = 0; n < steps && ok; ++n) {
                 const int st = n % stages;
-                const uint32_t qa = base + st * kStage, kb = qa + kOffB, vc = qa + kOffC;
-                if (!(ok = wait(&bar.sready, n & 1))) break;
+                const uint64_t qa = tc::smem_desc_sw128(base + st * kStage);
+                const uint64_t kb = tc::smem_desc_sw128_mn(base + st * kStage + kOffB, kBox);
+                const uint64_t vc = tc::smem_desc_sw128_mn(base + st * kStage + kOffC, kBox);
+                if (!(ok = wait(&bar.vready, n & 1))) break;
                 tc::fence_after_sync();
 #pragma unroll
                 for (int t = 0; t < 3; ++t)
 #pragma unroll
                     for (int k = 0; k < 4; ++k)
-                        tc::mma_bf16_tmem_a(tmem + kColT, tmem + kColV + t * 32 + k * 8,
-                                            tc::smem_desc_sw128_mn(kb + k * 2048, kBox), idT, t + k > 0);
+                        tc::mma_bf16(tmem + kColT, dV + (t * VB * kBox + k * 2048) / 16, kb + k * 2048 / 16, idT, t + k > 0);
                 tc::mma_commit(&bar.tdone);
                 if (!STATE_ONLY) {
-                    if (!(ok = wait(&bar.pready, n & 1))) break;
+                    if (!(ok = wait(&bar.sready, n & 1))) break;
                     if (n > 0 && !(ok = wait(&bar.ofree, (n - 1) & 1))) break;
                     tc::fence_after_sync();
-                    if (n + 1 < steps) {
-                        if (!(ok = wait(&bar.full[(n + 1) % stages], ((n + 1) / stages) & 1))) break;
-                        scores(n + 1);
-                    }
 #pragma unroll
                     for (int k = 0; k < DK / 16; ++k)
-                        tc::mma_bf16_tmem_a(tmem + kColO2, tmem + kColS + k * 8,
-                                            tc::smem_desc_sw128(qa + (k / 4) * kBox + (k % 4) * 32), idO2, k > 0);
+                        tc::mma_bf16_tmem_a(tmem + kColO2, tmem + kColS + k * 8, qa + ((k / 4) * kBox + (k % 4) * 32) / 16,
+                                            idO2, k > 0);
+                    if (!(ok = wait(&bar.pready, n & 1))) break;
+                    tc::fence_after_sync();
 #pragma unroll
                     for (int k = 0; k < 4; ++k)
-                        tc::mma_bf16(tmem + kColO1, tc::smem_desc_sw128_mn(vc + k * 2048, kBox),
-                                     tc::smem_desc_sw128(pbase + k * 32), idO1, k > 0);
+                        tc::mma_bf16(tmem + kColO1, vc + k * 2048 / 16, dP + k * 32 / 16, idO1, k > 0);
                     tc::mma_commit(&bar.odone);
                 }
                 tc::mma_commit(&bar.empty[st]);
                 done = n + 1;
+                if (!STATE_ONLY && n + 1 < steps) {
+                    if (!(ok = wait(&bar.full[(n + 1) % stages], ((n + 1) / stages) & 1))) break;
+                    scores(n + 1);
+                }
             }
             // nor a product
             if (done) tc::mbar_wait(&bar.empty[(done - 1) % stages], ((done - 1) / stages) & 1, kWaitNs);
@@ -505,15 +597,17 @@ bool encode(EncodeTiled fn, CUtensorMap *m, const Operand &o, int64_t time, int6
               CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) == CUDA_SUCCESS;
 }
 
+// Beside the stages: P, V', and for VB = 1 a box that the products' unused value lanes read.
+template <int VB> constexpr int extra_boxes() { return 1 + 3 * VB + (VB == 1); }
 template <int DKB, int VB> constexpr int stages_of(bool state_only) {
     const int stage = (state_only ? DKB + VB : 2 * DKB + VB) * kBox;
-    int n = (kSmemMax - 1024 - 3072 - kBox) / stage;
+    int n = (kSmemMax - 1024 - 3072 - extra_boxes<VB>() * kBox) / stage;
     return n > kMaxStages ? kMaxStages : n;
 }
 
 template <int DKB, int VB, typename OT, bool STATE_ONLY> int launch(TcParams &tp, const Maps &maps, cudaStream_t st) {
     tp.stages = stages_of<DKB, VB>(STATE_ONLY);
-    const int smem = tp.stages * (STATE_ONLY ? DKB + VB : 2 * DKB + VB) * kBox + kBox + 1024;
+    const int smem = tp.stages * (STATE_ONLY ? DKB + VB : 2 * DKB + VB) * kBox + extra_boxes<VB>() * kBox + 1024;
     auto kernel = decay_walk_tc_kernel<DKB, VB, OT, STATE_ONLY>;
     constexpr int kMaxDevices = 64;
     static std::mutex mu;

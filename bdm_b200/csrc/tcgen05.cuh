@@ -31,6 +31,16 @@ __device__ __forceinline__ bool mbar_test(uint64_t *bar, unsigned parity) {
         : "memory");
     return ok != 0;
 }
+// The same, suspended for up to about `ns` nanoseconds while the phase is incomplete.
+__device__ __forceinline__ bool mbar_test_for(uint64_t *bar, unsigned parity, unsigned ns) {
+    uint32_t ok;
+    asm volatile(
+        "{\n .reg .pred p;\n mbarrier.try_wait.parity.shared::cta.b64 p, [%1], %2, %3;\n selp.u32 %0, 1, 0, p;\n}\n"
+        : "=r"(ok)
+        : "r"(smem_u32(bar)), "r"(parity), "r"(ns)
+        : "memory");
+    return ok != 0;
+}
 __device__ __forceinline__ unsigned long long global_ns() {
     unsigned long long t;
     asm volatile("mov.u64 %0, %globaltimer;\n" : "=l"(t));
