@@ -100,6 +100,16 @@ __device__ __forceinline__ void three_terms(F2 x, uint32_t &hi, uint32_t &mid, u
     lo = pack2(x);
 }
 
+__device__ __noinline__ bool wait_slow(uint64_t *m, unsigned parity, volatile int *dead) {
+    const long long t0 = clock64();
+    for (int i = 0; i < (1 << 28); ++i) {
+        if (tc::mbar_test_for(m, parity, 1000)) return true;
+        if ((i & 15) == 15 && (*dead || clock64() - t0 > kWaitCycles)) break;
+    }
+    *dead = 1;
+    return false;
+}
+
 // The state the segment starts from, key columns [k0, k0 + KC) of value column `col` (see start_state).
 template <int KC>
 __device__ __forceinline__ void start_states(const Params &p, const Span &s, int64_t bh, int seg, float g, int k0, int col,
@@ -132,7 +142,8 @@ template <int DKB, int VB, typename OT, bool STATE_ONLY>
 __global__ void __launch_bounds__(kThreads, 1) decay_walk_tc_kernel(const TcParams tp, const __grid_constant__ Maps maps) {
     extern __shared__ char raw[];
     __shared__ Bars bar;
-    __shared__ float pw[kChunk + 1], spw[kChunk + 2];  // lam^m, scale lam^m
+    __shared__ float pw[kChunk + 1], spw[kChunk + 1];  // lam^m, scale lam^m
+    __shared__ float ow[2 * kChunk];                   // scale lam^. of a full chunk's tokens reading the state
     __shared__ uint32_t tmem_slot;
     __shared__ volatile int dead;
     const Params &p = tp.p;
@@ -158,6 +169,10 @@ __global__ void __launch_bounds__(kThreads, 1) decay_walk_tc_kernel(const TcPara
         pw[threadIdx.x] = threadIdx.x ? expf(g * (float)threadIdx.x) : 1.f;
         spw[threadIdx.x] = p.scale * pw[threadIdx.x];
     }
+    if (threadIdx.x < 2 * kChunk) {  // a chunk with fewer tokens starts later in the reverse walk's table
+        const int e = p.reverse ? kChunk - 1 - (int)threadIdx.x : (int)threadIdx.x + 1;
+        ow[threadIdx.x] = e < 0 || e > kChunk ? 0.f : p.scale * (e ? expf(g * (float)e) : 1.f);
+    }
     if (threadIdx.x == 0) {
         dead = 0;
         for (int i = 0; i < stages; ++i) {
@@ -179,24 +194,14 @@ __global__ void __launch_bounds__(kThreads, 1) decay_walk_tc_kernel(const TcPara
     tc::fence_after_sync();
     const uint32_t tmem = tmem_slot;
 
-    // bounded wait; false once any wait of the CTA has given up
-    auto wait = [&](uint64_t *m, unsigned parity) -> bool {
-        if (tc::mbar_test(m, parity)) return true;
-        const long long t0 = clock64();
-        for (int i = 0; i < (1 << 28); ++i) {
-            if (tc::mbar_test_for(m, parity, 1000)) return true;
-            if ((i & 15) == 15 && (dead || clock64() - t0 > kWaitCycles)) break;
-        }
-        dead = 1;
-        return false;
-    };
-    // the same for a whole warp, with one answer for its lanes
+    // bounded waits, the second for a whole warp with one answer for its lanes; false once any has given up
+    auto wait = [&](uint64_t *m, unsigned parity) -> bool { return tc::mbar_test(m, parity) || wait_slow(m, parity, &dead); };
     auto wait_warp = [&](uint64_t *m, unsigned parity) -> bool { return __all_sync(0xffffffffu, wait(m, parity)); };
-    auto chunk_of = [&](int n) -> int64_t { return p.reverse ? sp.c1 - 1 - n : sp.c0 + n; };
-    auto valid_of = [&](int64_t ch) -> int {
-        const int64_t left = sp.n - ch * kChunk;
-        return (int)(left < kChunk ? left : kChunk);
-    };
+    // first token and valid tokens of the n-th chunk of the walk
+    const int tokens = (int)sp.n, time = (int)p.time;
+    const int first = (int)(p.reverse ? sp.c1 - 1 : sp.c0) * kChunk, stride = p.reverse ? -kChunk : kChunk;
+    auto start_of = [&](int n) -> int { return first + n * stride; };
+    auto valid_of = [&](int n) -> int { return min(tokens - start_of(n), kChunk); };
 
     if (warp < kStateWarps) {
         // ------------------------------------------------------- V' and the state
@@ -217,24 +222,18 @@ __global__ void __launch_bounds__(kThreads, 1) decay_walk_tc_kernel(const TcPara
         }
         bool ok = true;
         int before = 0;  // valid tokens of the previous chunk
+        int st = 0, phase = 0;  // stage of the chunk, parity of its barrier
         for (int n = 0; n <= steps && ok; ++n) {
-            const int st = n % stages;
-            const int64_t ch = chunk_of(n);
-            const int valid = n < steps ? valid_of(ch) : 0;
-            uint4 raw[2 * VB];  // the chunk's values, 8 columns of a token each
+            const int valid = n < steps ? valid_of(n) : 0;
             if (n < steps) {
-                ok = wait_warp(&bar.full[st], (n / stages) & 1);
+                ok = wait_warp(&bar.full[st], phase);
                 if (!ok) break;
-                if (valid < kChunk && ch * kChunk + valid < p.time) {
+                if (valid < kChunk && start_of(n) + valid < time) {
                     // tokens past the row's length may hold anything: zero them for the products over j
                     uint4 *kb = reinterpret_cast<uint4 *>(smem + st * kStage + kOffB);
                     for (int i = threadIdx.x; i < (DKB + VB) * kBox / 16; i += kStateWarps * 32)
                         if ((i % (kBox / 16)) / 8 >= valid) kb[i] = make_uint4(0, 0, 0, 0);
                 }
-                // rows past `valid` are zero by now: their own thread, this one, has zeroed them
-                const uint4 *vc = reinterpret_cast<const uint4 *>(smem + st * kStage + kOffC);
-#pragma unroll
-                for (int u = 0; u < 2 * VB; ++u) raw[u] = vc[threadIdx.x + u * 256];
             }
             if (n > 0) {
                 ok = wait_warp(&bar.tdone, (n - 1) & 1);
@@ -254,24 +253,31 @@ __global__ void __launch_bounds__(kThreads, 1) decay_walk_tc_kernel(const TcPara
             }
             before = valid;
             if (n == steps) break;
-            // V' has the layout of the tile: the same place in each term's buffer
+            // V' has the layout of the tile: the same place in each term's buffer.  Rows past `valid` are zero
+            // by now (the thread that reads one has zeroed it, or the copy has).
+            {
+                const uint4 *src = reinterpret_cast<const uint4 *>(smem + st * kStage + kOffC) + threadIdx.x;
+                uint4 *dst = reinterpret_cast<uint4 *>(sV) + threadIdx.x;
+                const int j0 = threadIdx.x / 8;
+#pragma unroll 1
+                for (int box = 0; box < VB; ++box, src += kBox / 16, dst += kBox / 16)
 #pragma unroll
-            for (int u = 0; u < 2 * VB; ++u) {
-                const int i = threadIdx.x + u * 256;
-                const int j = (i % 512) / 8;
-                const int e = p.reverse ? j + 1 : valid - 1 - j;
-                const float w = pw[e < 0 ? 0 : e];
-                const F2 ww = make2(w, w);
-                uint4 t0, t1, t2;
-                three_terms(mul2(ww, unpack2(raw[u].x)), t0.x, t1.x, t2.x);
-                three_terms(mul2(ww, unpack2(raw[u].y)), t0.y, t1.y, t2.y);
-                three_terms(mul2(ww, unpack2(raw[u].z)), t0.z, t1.z, t2.z);
-                three_terms(mul2(ww, unpack2(raw[u].w)), t0.w, t1.w, t2.w);
-                uint4 *dst = reinterpret_cast<uint4 *>(sV) + i;
-                dst[0] = t0;
-                dst[VB * kBox / 16] = t1;
-                dst[2 * VB * kBox / 16] = t2;
+                    for (int u = 0; u < 2; ++u) {
+                        const uint4 raw = src[u * 256];
+                        const int e = p.reverse ? j0 + u * 32 + 1 : valid - 1 - j0 - u * 32;
+                        const float w = pw[e < 0 ? 0 : e];
+                        const F2 ww = make2(w, w);
+                        uint4 t0, t1, t2;
+                        three_terms(mul2(ww, unpack2(raw.x)), t0.x, t1.x, t2.x);
+                        three_terms(mul2(ww, unpack2(raw.y)), t0.y, t1.y, t2.y);
+                        three_terms(mul2(ww, unpack2(raw.z)), t0.z, t1.z, t2.z);
+                        three_terms(mul2(ww, unpack2(raw.w)), t0.w, t1.w, t2.w);
+                        dst[u * 256] = t0;
+                        dst[u * 256 + VB * kBox / 16] = t1;
+                        dst[u * 256 + 2 * VB * kBox / 16] = t2;
+                    }
             }
+            if (++st == stages) st = 0, phase ^= 1;
             tc::fence_async_smem();
             tc::fence_before_sync();
             __syncwarp();
@@ -321,71 +327,58 @@ __global__ void __launch_bounds__(kThreads, 1) decay_walk_tc_kernel(const TcPara
             const bool on = col < p.wc;
             OT *out = static_cast<OT *>(p.out) + b * p.os[0] + h * p.os[2];
             // 4-byte stores of two columns where every token's row allows them
-            const bool wide = ((reinterpret_cast<uintptr_t>(p.out) & 3) | ((p.os[0] | p.os[1] | p.os[2]) & 1)) == 0;
+            const int odd = lane & 1, pair = col & ~1;
+            const bool both = pair + 1 < p.wc &&
+                              ((reinterpret_cast<uintptr_t>(p.out) & 3) | ((p.os[0] | p.os[1] | p.os[2]) & 1)) == 0;
             for (int n = 0; n < steps; ++n) {
                 if (!wait_warp(&bar.odone, n & 1)) break;
                 tc::fence_after_sync();
-                const int64_t t0 = chunk_of(n) * kChunk;
-                const int valid = valid_of(chunk_of(n));
-                F2 x[32];
-                if (quad < 2 * VB) {
-                    // scale lam^. of 16 tokens per step, from the last to the first in the reverse walk
+                const int t0 = start_of(n), valid = valid_of(n), rows = min(time - t0, kChunk);
+                const bool full = valid == kChunk && both;
+                // neighbouring lanes swap halves of a BF16 pair, so that a lane stores two columns of one token:
+                // the even lane of the even tokens, the odd lane of the odd ones
+                OT *o = out + (int64_t)(sizeof(OT) == 4 ? t0 : t0 + odd) * p.os[1] + (sizeof(OT) == 4 ? col : pair);
+                const float *w = ow + (p.reverse ? kChunk - valid : 0);
+#pragma unroll 1
+                for (int i = 0; i < 64; i += 16, w += 16) {
+                    if (quad >= 2 * VB) break;
+                    float y[16], z[16];
+                    tc::tmem_ld16(tmem + lanes + kColO2 + i, y);
+                    tc::tmem_ld16(tmem + lanes + kColO1 + i, z);
+                    tc::tmem_wait_ld();
 #pragma unroll
-                    for (int i = 0; i < 64; i += 16) {
-                        float y[16], z[16];
-                        tc::tmem_ld16(tmem + lanes + kColO2 + i, y);
-                        tc::tmem_ld16(tmem + lanes + kColO1 + i, z);
-                        tc::tmem_wait_ld();
+                    for (int e = 0; e < 16; ++e) z[e] = fmaf(w[e], y[e], z[e]);
+                    if constexpr (sizeof(OT) == 4) {
 #pragma unroll
-                        for (int e = 0; e < 16; e += 2) {
-                            const int r = i + e;
-                            F2 w;
-                            if (p.reverse)
-                                w = make2(spw[valid > r ? valid - 1 - r : 0], spw[valid > r + 1 ? valid - 2 - r : 0]);
-                            else
-                                w = make2(spw[r + 1], spw[r + 2]);
-                            x[r / 2] = fma2(w, make2(y[e], y[e + 1]), make2(z[e], z[e + 1]));
+                        for (int e = 0; e < 16; ++e, o += p.os[1])
+                            if (on && i + e < rows) *o = i + e < valid ? z[e] : 0.f;
+                    } else {
+                        uint32_t v[8];
+#pragma unroll
+                        for (int e = 0; e < 8; ++e) {
+                            const uint32_t own = pack_bf16(z[2 * e], z[2 * e + 1]);
+                            const uint32_t other = __shfl_xor_sync(0xffffffffu, own, 1);
+                            v[e] = __byte_perm(odd ? other : own, odd ? own : other, odd ? 0x7632 : 0x5410);
+                        }
+                        if (full) {
+#pragma unroll
+                            for (int e = 0; e < 8; ++e, o += 2 * p.os[1]) *reinterpret_cast<uint32_t *>(o) = v[e];
+                        } else {
+#pragma unroll
+                            for (int e = 0; e < 8; ++e, o += 2 * p.os[1]) {
+                                const int r = i + 2 * e + odd;
+                                if (r >= rows || pair >= p.wc) continue;
+                                if (r >= valid) v[e] = 0;  // padding gives zeros
+                                const __nv_bfloat162 q = *reinterpret_cast<const __nv_bfloat162 *>(&v[e]);
+                                o[0] = q.x;
+                                if (pair + 1 < p.wc) o[1] = q.y;
+                            }
                         }
                     }
                 }
                 tc::fence_before_sync();
                 __syncwarp();
                 if (lane == 0) tc::mbar_arrive(&bar.ofree);
-                const int rows = (int)(p.time - t0 < kChunk ? p.time - t0 : kChunk);
-                if (valid < kChunk)  // padding gives zeros
-#pragma unroll
-                    for (int r = 0; r < 64; r += 2) {
-                        const float2 v = split2(x[r / 2]);
-                        x[r / 2] = make2(r < valid ? v.x : 0.f, r + 1 < valid ? v.y : 0.f);
-                    }
-                if constexpr (sizeof(OT) == 4) {
-                    OT *o = out + t0 * p.os[1] + col;
-                    if (on)
-#pragma unroll
-                        for (int r = 0; r < 64; ++r)
-                            if (r < rows) o[r * p.os[1]] = r & 1 ? split2(x[r / 2]).y : split2(x[r / 2]).x;
-                } else {
-                    // neighbouring lanes swap halves, so that a lane stores two columns of one token: the even
-                    // lane of the even tokens, the odd lane of the odd ones
-                    const int odd = lane & 1, pair = col & ~1;
-                    OT *o = out + (t0 + odd) * p.os[1] + pair;
-                    const bool both = wide && pair + 1 < p.wc;
-#pragma unroll
-                    for (int r = 0; r < 64; r += 2) {
-                        const uint32_t own = pack2(x[r / 2]), other = __shfl_xor_sync(0xffffffffu, own, 1);
-                        const uint32_t v = __byte_perm(odd ? other : own, odd ? own : other, odd ? 0x7632 : 0x5410);
-                        if (r + odd < rows) {
-                            OT *d = o + r * p.os[1];
-                            if (both) {
-                                *reinterpret_cast<uint32_t *>(d) = v;
-                            } else if (pair < p.wc) {
-                                const __nv_bfloat162 q = *reinterpret_cast<const __nv_bfloat162 *>(&v);
-                                d[0] = q.x;
-                                if (pair + 1 < p.wc) d[1] = q.y;
-                            }
-                        }
-                    }
-                }
             }
             // whole chunks past the row's length
             int64_t z0 = sp.chunks * kChunk, z1 = p.time;
@@ -401,21 +394,14 @@ __global__ void __launch_bounds__(kThreads, 1) decay_walk_tc_kernel(const TcPara
             const int quad = warp & 3;  // 0 or 1
             const int row = quad * 32 + lane;
             const uint32_t lanes = (uint32_t)(quad * 32) << 16;
-            // the row's weights: the same for every chunk that is full
-            F2 w[32];
-            auto weights = [&](int valid) {  // scores of tokens past the row's length may be anything
+            F2 w[32];  // the row's weights
 #pragma unroll
-                for (int j = 0; j < 64; j += 2) {
-                    const int d0 = p.reverse ? j - row : row - j, d1 = p.reverse ? d0 + 1 : d0 - 1;
-                    w[j / 2] = make2(d0 >= 0 && j < valid ? spw[d0 < 0 ? 0 : d0] : 0.f,
-                                     d1 >= 0 && j + 1 < valid ? spw[d1 < 0 ? 0 : d1] : 0.f);
-                }
-            };
-            int held = kChunk;
-            weights(held);
+            for (int j = 0; j < 64; j += 2) {
+                const int d0 = p.reverse ? j - row : row - j, d1 = p.reverse ? d0 + 1 : d0 - 1;
+                w[j / 2] = make2(d0 >= 0 ? spw[d0 < 0 ? 0 : d0] : 0.f, d1 >= 0 ? spw[d1 < 0 ? 0 : d1] : 0.f);
+            }
             for (int n = 0; n < steps; ++n) {
-                const int valid = valid_of(chunk_of(n));
-                if (valid != held) weights(held = valid);
+                const int valid = valid_of(n);
                 if (!wait_warp(&bar.adone, n & 1)) break;
                 tc::fence_after_sync();
                 uint32_t r[32];
@@ -425,14 +411,12 @@ __global__ void __launch_bounds__(kThreads, 1) decay_walk_tc_kernel(const TcPara
                     tc::tmem_ld16(tmem + lanes + kColA + i, x);
                     tc::tmem_wait_ld();
 #pragma unroll
-                    for (int e = 0; e < 16; e += 2) {
-                        const F2 f = w[(i + e) / 2];
-                        const float2 ff = split2(f);
-                        // a masked score may be NaN: select, do not multiply
-                        const float2 y = split2(mul2(f, make2(x[e], x[e + 1])));
-                        r[(i + e) / 2] = pack_bf16(ff.x != 0.f ? y.x : 0.f, ff.y != 0.f ? y.y : 0.f);
-                    }
+                    for (int e = 0; e < 16; e += 2) r[(i + e) / 2] = pack2(mul2(w[(i + e) / 2], make2(x[e], x[e + 1])));
                 }
+                if (valid < kChunk)  // scores of tokens past the row's length may be anything
+#pragma unroll
+                    for (int j = 0; j < 64; j += 2)
+                        r[j / 2] &= (j < valid ? 0xffffu : 0u) | (j + 1 < valid ? 0xffff0000u : 0u);
                 if (n > 0 && !wait_warp(&bar.odone, (n - 1) & 1)) break;
 #pragma unroll
                 for (int c = 0; c < 8; ++c)
@@ -452,7 +436,7 @@ __global__ void __launch_bounds__(kThreads, 1) decay_walk_tc_kernel(const TcPara
                 const int st = n % stages;
                 if (n >= stages && !wait(&bar.empty[st], ((n / stages) - 1) & 1)) break;
                 char *dst = smem + st * kStage;
-                const int t0 = (int)(chunk_of(n) * kChunk);
+                const int t0 = start_of(n);
                 tc::mbar_arrive_expect_tx(&bar.full[st], kStage);
                 if (!STATE_ONLY)
 #pragma unroll
