@@ -7,16 +7,18 @@
 //   P    = scale A * lam^(i-j), masked      -> BF16 in shared memory, [i][j]
 //   O1^T = Vc^T P^T                [dv, i]  Vc read MN-major
 //   O2^T = S^T Qa^T                [dv, i]  S^T is a BF16 operand in tensor memory
-//   T^T  = V'^T Kb                 [dv, dk] V' = lam^. Vc as three BF16 terms in shared memory, both MN-major
+//   T^T  = V'^T Kb                 [dv, dk] V' = lam^. Vc as three BF16 terms in tensor memory, Kb MN-major
 //   out  = O1 + scale lam^. O2,    S <- lam^n S + T
 // The state itself stays in registers in FP32.  Roundings to BF16: P and the copy of S that is read (one
 // rounding each, as large as the output's own); V' is split into three terms (24 bits), so that T, and with
 // it the state over any number of chunks, is exact to FP32.
 //
 // Roles (16 warps): 0-7 carry the state (thread = value column, half of the key columns) and scale V',
-// 8-11 the outputs, 12-13 P, 14 TMA, 15 MMA.  The cycle of a chunk is T(n) -> state update and V'(n+1) ->
-// T(n+1); O2, O1 and the next A fill the tensor pipe in between.  Every wait is bounded; one that gives up
-// sets the status bit and lets the CTA drain.
+// 8-11 the outputs, 12-13 P, 14 TMA, 15 MMA.  V' is made and T issued in two halves of 32 tokens, so that the
+// scaling of one overlaps the product of the other; O2, O1 and the next A run while the state warps take T.
+// V' is in tensor memory because shared memory's bandwidth is what the products and copies share: as a
+// shared-memory operand it took 768 more of its cycles per chunk (and 4100 cycles per chunk instead of 2900).
+// Every wait is bounded; one that gives up sets the status bit and lets the CTA drain.
 #include "decay_walk.cuh"
 #include "tcgen05.cuh"
 
@@ -38,7 +40,7 @@ constexpr long long kWaitCycles = 4000000000ll;  // about 2 s
 constexpr unsigned long long kWaitNs = 2000000000ull;
 
 // tensor memory columns
-constexpr uint32_t kColA = 0, kColO1 = 64, kColO2 = 128, kColT = 192, kColS = 320;
+constexpr uint32_t kColA = 0, kColO1 = 64, kColO2 = 128, kColT = 192, kColS = 320, kColV = 384;
 
 struct Maps {
     CUtensorMap a, b, c;
@@ -51,7 +53,7 @@ struct TcParams {
 
 struct Bars {
     uint64_t full[kMaxStages], empty[kMaxStages];
-    uint64_t vready, sready, tdone, adone, pready, odone, ofree;
+    uint64_t vready[2], sready, thalf, tdone, adone, pready, odone, ofree;
 };
 
 __device__ __forceinline__ uint32_t pack_bf16(float lo, float hi) {
@@ -144,17 +146,17 @@ __global__ void __launch_bounds__(kThreads, 1) decay_walk_tc_kernel(const TcPara
     __shared__ Bars bar;
     __shared__ float pw[kChunk + 1], spw[kChunk + 1];  // lam^m, scale lam^m
     __shared__ float ow[2 * kChunk];                   // scale lam^. of a full chunk's tokens reading the state
+    __shared__ alignas(8) float vw[2 * kChunk];        // lam^. of a full chunk's tokens writing it
     __shared__ uint32_t tmem_slot;
     __shared__ volatile int dead;
     const Params &p = tp.p;
-    const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+    const int warp = __shfl_sync(0xffffffffu, threadIdx.x >> 5, 0), lane = threadIdx.x & 31;
     char *smem = reinterpret_cast<char *>((reinterpret_cast<uintptr_t>(raw) + 1023) & ~(uintptr_t)1023);
     constexpr int kStage = (STATE_ONLY ? DKB + VB : 2 * DKB + VB) * kBox;
     constexpr int kOffB = STATE_ONLY ? 0 : DKB * kBox, kOffC = kOffB + DKB * kBox;
     constexpr int DK = DKB * 64;
     const int stages = tp.stages;
     char *sP = smem + stages * kStage;
-    char *sV = sP + kBox;  // V', three terms
 
     int64_t id = blockIdx.x;
     const int seg = (int)(id % p.nseg);
@@ -169,9 +171,11 @@ __global__ void __launch_bounds__(kThreads, 1) decay_walk_tc_kernel(const TcPara
         pw[threadIdx.x] = threadIdx.x ? expf(g * (float)threadIdx.x) : 1.f;
         spw[threadIdx.x] = p.scale * pw[threadIdx.x];
     }
-    if (threadIdx.x < 2 * kChunk) {  // a chunk with fewer tokens starts later in the reverse walk's table
+    if (threadIdx.x < 2 * kChunk) {  // a chunk with fewer tokens starts later in the tables that count down
         const int e = p.reverse ? kChunk - 1 - (int)threadIdx.x : (int)threadIdx.x + 1;
         ow[threadIdx.x] = e < 0 || e > kChunk ? 0.f : p.scale * (e ? expf(g * (float)e) : 1.f);
+        const int f = p.reverse ? (int)threadIdx.x + 1 : kChunk - 1 - (int)threadIdx.x;
+        vw[threadIdx.x] = f < 0 || f > kChunk ? 0.f : (f ? expf(g * (float)f) : 1.f);
     }
     if (threadIdx.x == 0) {
         dead = 0;
@@ -179,7 +183,9 @@ __global__ void __launch_bounds__(kThreads, 1) decay_walk_tc_kernel(const TcPara
             tc::mbar_init(&bar.full[i], 1);
             tc::mbar_init(&bar.empty[i], 1);
         }
-        tc::mbar_init(&bar.vready, kStateWarps);
+        tc::mbar_init(&bar.vready[0], kStateWarps);
+        tc::mbar_init(&bar.vready[1], kStateWarps);
+        tc::mbar_init(&bar.thalf, 1);
         tc::mbar_init(&bar.sready, kStateWarps);
         tc::mbar_init(&bar.tdone, 1);
         tc::mbar_init(&bar.adone, 1);
@@ -223,8 +229,35 @@ __global__ void __launch_bounds__(kThreads, 1) decay_walk_tc_kernel(const TcPara
         bool ok = true;
         int before = 0;  // valid tokens of the previous chunk
         int st = 0, phase = 0;  // stage of the chunk, parity of its barrier
-        for (int n = 0; n <= steps && ok; ++n) {
+        for (int n = 0; n <= steps; ++n) {
             const int valid = n < steps ? valid_of(n) : 0;
+            // 16 tokens of V' from 32 hb + 16 half on: this lane's column, scaled, as three BF16 terms
+            auto scale16 = [&](int hb) {
+                const int j0 = hb * 32 + half * 16;
+                const char *src = smem + st * kStage + kOffC + (col >> 6) * kBox + (col & 7) * 2 + j0 * 128;
+                const int chunk = (col & 63) >> 3;
+                const float2 *w = reinterpret_cast<const float2 *>(vw + (p.reverse ? 0 : kChunk - valid) + j0);
+                uint32_t v[3][8];
+#pragma unroll
+                for (int u = 0; u < 8; ++u) {
+                    const uint32_t x0 = *reinterpret_cast<const unsigned short *>(src + 2 * u * 128 + ((chunk ^ (2 * u & 7)) << 4));
+                    const uint32_t x1 =
+                        *reinterpret_cast<const unsigned short *>(src + (2 * u + 1) * 128 + ((chunk ^ ((2 * u + 1) & 7)) << 4));
+                    const float2 ww = valid == kChunk || p.reverse
+                                          ? w[u]
+                                          : make_float2(reinterpret_cast<const float *>(w)[2 * u], reinterpret_cast<const float *>(w)[2 * u + 1]);
+                    three_terms(mul2(make2(ww.x, ww.y), make2(__uint_as_float(x0 << 16), __uint_as_float(x1 << 16))), v[0][u],
+                                v[1][u], v[2][u]);
+                }
+#pragma unroll
+                for (int t = 0; t < 3; ++t) tc::tmem_st8(tmem + lanes + kColV + hb * 48 + t * 16 + half * 8, v[t]);
+            };
+            auto arrive = [&](uint64_t *m) {
+                tc::tmem_wait_st();
+                tc::fence_before_sync();
+                __syncwarp();
+                if (lane == 0) tc::mbar_arrive(m);
+            };
             if (n < steps) {
                 ok = wait_warp(&bar.full[st], phase);
                 if (!ok) break;
@@ -233,7 +266,15 @@ __global__ void __launch_bounds__(kThreads, 1) decay_walk_tc_kernel(const TcPara
                     uint4 *kb = reinterpret_cast<uint4 *>(smem + st * kStage + kOffB);
                     for (int i = threadIdx.x; i < (DKB + VB) * kBox / 16; i += kStateWarps * 32)
                         if ((i % (kBox / 16)) / 8 >= valid) kb[i] = make_uint4(0, 0, 0, 0);
+                    tc::fence_async_smem();
+                    asm volatile("bar.sync 1, %0;\n" ::"n"(kStateWarps * 32) : "memory");
                 }
+                if (n > 0) {
+                    ok = wait_warp(&bar.thalf, (n - 1) & 1);
+                    if (!ok) break;
+                    tc::fence_after_sync();
+                }
+                if (mine) scale16(0);
             }
             if (n > 0) {
                 ok = wait_warp(&bar.tdone, (n - 1) & 1);
@@ -253,35 +294,10 @@ __global__ void __launch_bounds__(kThreads, 1) decay_walk_tc_kernel(const TcPara
             }
             before = valid;
             if (n == steps) break;
-            // V' has the layout of the tile: the same place in each term's buffer.  Rows past `valid` are zero
-            // by now (the thread that reads one has zeroed it, or the copy has).
-            {
-                const uint4 *src = reinterpret_cast<const uint4 *>(smem + st * kStage + kOffC) + threadIdx.x;
-                uint4 *dst = reinterpret_cast<uint4 *>(sV) + threadIdx.x;
-                const int j0 = threadIdx.x / 8;
-#pragma unroll 1
-                for (int box = 0; box < VB; ++box, src += kBox / 16, dst += kBox / 16)
-#pragma unroll
-                    for (int u = 0; u < 2; ++u) {
-                        const uint4 raw = src[u * 256];
-                        const int e = p.reverse ? j0 + u * 32 + 1 : valid - 1 - j0 - u * 32;
-                        const float w = pw[e < 0 ? 0 : e];
-                        const F2 ww = make2(w, w);
-                        uint4 t0, t1, t2;
-                        three_terms(mul2(ww, unpack2(raw.x)), t0.x, t1.x, t2.x);
-                        three_terms(mul2(ww, unpack2(raw.y)), t0.y, t1.y, t2.y);
-                        three_terms(mul2(ww, unpack2(raw.z)), t0.z, t1.z, t2.z);
-                        three_terms(mul2(ww, unpack2(raw.w)), t0.w, t1.w, t2.w);
-                        dst[u * 256] = t0;
-                        dst[u * 256 + VB * kBox / 16] = t1;
-                        dst[u * 256 + 2 * VB * kBox / 16] = t2;
-                    }
-            }
+            arrive(&bar.vready[0]);
+            if (mine) scale16(1);
+            arrive(&bar.vready[1]);
             if (++st == stages) st = 0, phase ^= 1;
-            tc::fence_async_smem();
-            tc::fence_before_sync();
-            __syncwarp();
-            if (lane == 0) tc::mbar_arrive(&bar.vready);
             if (!STATE_ONLY) {
                 if (n > 0) {
                     ok = wait_warp(&bar.odone, (n - 1) & 1);  // the last chunk's reads of S are over
@@ -296,10 +312,7 @@ __global__ void __launch_bounds__(kThreads, 1) decay_walk_tc_kernel(const TcPara
                         for (int e = 0; e < 16; ++e) r[e] = pack2(S[i / 2 + e]);
                         tc::tmem_st16(tmem + lanes + kColS + (k0 + i) / 2, r);
                     }
-                tc::tmem_wait_st();
-                tc::fence_before_sync();
-                __syncwarp();
-                if (lane == 0) tc::mbar_arrive(&bar.sready);
+                arrive(&bar.sready);
             }
         }
         if (ok && col < p.wc) {
@@ -459,15 +472,14 @@ __global__ void __launch_bounds__(kThreads, 1) decay_walk_tc_kernel(const TcPara
         }
     } else {
         // --------------------------------------------------------------- products
-        if (lane == 0) {
+        if (tc::elect_one()) {
             constexpr uint32_t idQK = tc::idesc_bf16(128, 64);
             constexpr uint32_t idO1 = tc::idesc_bf16(128, 64) | tc::kIdescMnA;
             constexpr uint32_t idO2 = tc::idesc_bf16(128, 64);
-            constexpr uint32_t idT = tc::idesc_bf16(128, DK) | tc::kIdescMnA | tc::kIdescMnB;
+            constexpr uint32_t idT = tc::idesc_bf16(128, DK) | tc::kIdescMnB;
             // descriptors of the buffers' starts; an offset adds its bytes / 16 to the low word
             const uint32_t base = tc::smem_u32(smem);
             const uint64_t dP = tc::smem_desc_sw128(tc::smem_u32(sP));
-            const uint64_t dV = tc::smem_desc_sw128_mn(tc::smem_u32(sV), kBox);
             // rows 64..127 of the scores, and value columns past c's boxes, are whatever follows the tile
             auto scores = [&](int n) {
                 const uint64_t qa = tc::smem_desc_sw128(base + (n % stages) * kStage), kb = qa + kOffB / 16;
@@ -489,14 +501,19 @@ __global__ void __launch_bounds__(kThreads, 1) decay_walk_tc_kernel(const TcPara
                 const uint64_t qa = tc::smem_desc_sw128(base + st * kStage);
                 const uint64_t kb = tc::smem_desc_sw128_mn(base + st * kStage + kOffB, kBox);
                 const uint64_t vc = tc::smem_desc_sw128_mn(base + st * kStage + kOffC, kBox);
-                if (!(ok = wait(&bar.vready, n & 1))) break;
-                tc::fence_after_sync();
 #pragma unroll
-                for (int t = 0; t < 3; ++t)
+                for (int hb = 0; hb < 2; ++hb) {
+                    if (!(ok = wait(&bar.vready[hb], n & 1))) break;
+                    tc::fence_after_sync();
 #pragma unroll
-                    for (int k = 0; k < 4; ++k)
-                        tc::mma_bf16(tmem + kColT, dV + (t * VB * kBox + k * 2048) / 16, kb + k * 2048 / 16, idT, t + k > 0);
-                tc::mma_commit(&bar.tdone);
+                    for (int t = 0; t < 3; ++t)
+#pragma unroll
+                        for (int k = 0; k < 2; ++k)
+                            tc::mma_bf16_tmem_a(tmem + kColT, tmem + kColV + hb * 48 + t * 16 + k * 8,
+                                                kb + (2 * hb + k) * 2048 / 16, idT, hb + t + k > 0);
+                    tc::mma_commit(hb ? &bar.tdone : &bar.thalf);
+                }
+                if (!ok) break;
                 if (!STATE_ONLY) {
                     if (!(ok = wait(&bar.sready, n & 1))) break;
                     if (n > 0 && !(ok = wait(&bar.ofree, (n - 1) & 1))) break;
@@ -581,17 +598,15 @@ bool encode(EncodeTiled fn, CUtensorMap *m, const Operand &o, int64_t time, int6
               CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) == CUDA_SUCCESS;
 }
 
-// Beside the stages: P, V', and for VB = 1 a box that the products' unused value lanes read.
-template <int VB> constexpr int extra_boxes() { return 1 + 3 * VB + (VB == 1); }
 template <int DKB, int VB> constexpr int stages_of(bool state_only) {
     const int stage = (state_only ? DKB + VB : 2 * DKB + VB) * kBox;
-    int n = (kSmemMax - 1024 - 3072 - extra_boxes<VB>() * kBox) / stage;
+    int n = (kSmemMax - 1024 - 3072 - kBox) / stage;
     return n > kMaxStages ? kMaxStages : n;
 }
 
 template <int DKB, int VB, typename OT, bool STATE_ONLY> int launch(TcParams &tp, const Maps &maps, cudaStream_t st) {
     tp.stages = stages_of<DKB, VB>(STATE_ONLY);
-    const int smem = tp.stages * (STATE_ONLY ? DKB + VB : 2 * DKB + VB) * kBox + extra_boxes<VB>() * kBox + 1024;
+    const int smem = tp.stages * (STATE_ONLY ? DKB + VB : 2 * DKB + VB) * kBox + kBox + 1024;
     auto kernel = decay_walk_tc_kernel<DKB, VB, OT, STATE_ONLY>;
     constexpr int kMaxDevices = 64;
     static std::mutex mu;
