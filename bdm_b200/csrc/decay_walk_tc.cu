@@ -43,7 +43,7 @@ constexpr unsigned long long kWaitNs = 2000000000ull;
 constexpr uint32_t kColA = 0, kColO1 = 64, kColO2 = 128, kColT = 192, kColS = 320, kColV = 384;
 
 struct Maps {
-    CUtensorMap a, b, c;
+    CUtensorMap a, b, c, out;
 };
 struct TcParams {
     Params p;
@@ -53,7 +53,7 @@ struct TcParams {
 
 struct Bars {
     uint64_t full[kMaxStages], empty[kMaxStages];
-    uint64_t vready[2], sready, thalf, tdone, adone, pready, odone, ofree;
+    uint64_t vready[2], sready, thalf, tdone, adone, pready, odone, ofree, zeroed, ofull, oempty;
 };
 
 __device__ __forceinline__ uint32_t pack_bf16(float lo, float hi) {
@@ -146,7 +146,7 @@ __global__ void __launch_bounds__(kThreads, 1) decay_walk_tc_kernel(const TcPara
     __shared__ Bars bar;
     __shared__ float pw[kChunk + 1], spw[kChunk + 1];  // lam^m, scale lam^m
     __shared__ float ow[2 * kChunk];                   // scale lam^. of a full chunk's tokens reading the state
-    __shared__ alignas(8) float vw[2 * kChunk];        // lam^. of a full chunk's tokens writing it
+    __shared__ float vw[2 * kChunk];                   // lam^. of a full chunk's tokens writing it
     __shared__ uint32_t tmem_slot;
     __shared__ volatile int dead;
     const Params &p = tp.p;
@@ -192,6 +192,9 @@ __global__ void __launch_bounds__(kThreads, 1) decay_walk_tc_kernel(const TcPara
         tc::mbar_init(&bar.pready, 2);
         tc::mbar_init(&bar.odone, 1);
         tc::mbar_init(&bar.ofree, 4);
+        tc::mbar_init(&bar.zeroed, kStateWarps);
+        tc::mbar_init(&bar.ofull, 4);
+        tc::mbar_init(&bar.oempty, 1);
         tc::mbar_fence_init();
     }
     if (warp == kMmaWarp) tc::tmem_alloc(&tmem_slot, 512);
@@ -227,92 +230,99 @@ __global__ void __launch_bounds__(kThreads, 1) decay_walk_tc_kernel(const TcPara
             for (int i = 0; i < KC / 2; ++i) S[i] = make2(x[2 * i], x[2 * i + 1]);
         }
         bool ok = true;
-        int before = 0;  // valid tokens of the previous chunk
+        int valid = 0, before = 0;  // valid tokens of the chunk and of the one before
         int st = 0, phase = 0;  // stage of the chunk, parity of its barrier
-        for (int n = 0; n <= steps; ++n) {
-            const int valid = n < steps ? valid_of(n) : 0;
-            // 16 tokens of V' from 32 hb + 16 half on: this lane's column, scaled, as three BF16 terms
-            auto scale16 = [&](int hb) {
-                const int j0 = hb * 32 + half * 16;
-                const char *src = smem + st * kStage + kOffC + (col >> 6) * kBox + (col & 7) * 2 + j0 * 128;
-                const int chunk = (col & 63) >> 3;
-                const float2 *w = reinterpret_cast<const float2 *>(vw + (p.reverse ? 0 : kChunk - valid) + j0);
-                uint32_t v[3][8];
-#pragma unroll
-                for (int u = 0; u < 8; ++u) {
-                    const uint32_t x0 = *reinterpret_cast<const unsigned short *>(src + 2 * u * 128 + ((chunk ^ (2 * u & 7)) << 4));
-                    const uint32_t x1 =
-                        *reinterpret_cast<const unsigned short *>(src + (2 * u + 1) * 128 + ((chunk ^ ((2 * u + 1) & 7)) << 4));
-                    const float2 ww = valid == kChunk || p.reverse
-                                          ? w[u]
-                                          : make_float2(reinterpret_cast<const float *>(w)[2 * u], reinterpret_cast<const float *>(w)[2 * u + 1]);
-                    three_terms(mul2(make2(ww.x, ww.y), make2(__uint_as_float(x0 << 16), __uint_as_float(x1 << 16))), v[0][u],
-                                v[1][u], v[2][u]);
-                }
-#pragma unroll
-                for (int t = 0; t < 3; ++t) tc::tmem_st8(tmem + lanes + kColV + hb * 48 + t * 16 + half * 8, v[t]);
-            };
-            auto arrive = [&](uint64_t *m) {
-                tc::tmem_wait_st();
-                tc::fence_before_sync();
-                __syncwarp();
-                if (lane == 0) tc::mbar_arrive(m);
-            };
-            if (n < steps) {
+        // this lane's row of the matrices it loads: two of 8 tokens by two of 8 columns
+        const int mrow = ((lane >> 4) * 8 + (lane & 7)) * 128, mcol = (lane >> 3) & 1;
+        auto arrive = [&](uint64_t *m) {
+            tc::tmem_wait_st();
+            tc::fence_before_sync();
+            __syncwarp();
+            if (lane == 0) tc::mbar_arrive(m);
+        };
+        // Half steps (32 tokens) of a chunk; one copy of the scaling code, for the instruction cache's sake.
+        for (int hs = 0; hs <= 2 * steps; ++hs) {
+            const int n = hs >> 1, hb = hs & 1;
+            if (hb == 0 && n < steps) {
+                valid = valid_of(n);
                 ok = wait_warp(&bar.full[st], phase);
                 if (!ok) break;
                 if (valid < kChunk && start_of(n) + valid < time) {
                     // tokens past the row's length may hold anything: zero them for the products over j
                     uint4 *kb = reinterpret_cast<uint4 *>(smem + st * kStage + kOffB);
+#pragma unroll 1
                     for (int i = threadIdx.x; i < (DKB + VB) * kBox / 16; i += kStateWarps * 32)
                         if ((i % (kBox / 16)) / 8 >= valid) kb[i] = make_uint4(0, 0, 0, 0);
                     tc::fence_async_smem();
-                    asm volatile("bar.sync 1, %0;\n" ::"n"(kStateWarps * 32) : "memory");
+                    __syncwarp();
+                    if (lane == 0) tc::mbar_arrive(&bar.zeroed);  // once at most: a row has one such chunk
+                    ok = wait_warp(&bar.zeroed, 0);
+                    if (!ok) break;
                 }
                 if (n > 0) {
                     ok = wait_warp(&bar.thalf, (n - 1) & 1);
                     if (!ok) break;
                     tc::fence_after_sync();
                 }
-                if (mine) scale16(0);
             }
-            if (n > 0) {
-                ok = wait_warp(&bar.tdone, (n - 1) & 1);
-                if (!ok) break;
-                tc::fence_after_sync();
-                if (mine) {
-                    const F2 carry = make2(pw[before], pw[before]);
+            if (mine && n < steps) {
+                // 16 tokens of V' from 32 hb + 16 half on, this quadrant's columns: transposed on the way in, scaled,
+                // and split into BF16 terms as the fragments that tensor memory takes
+                const int j0 = hb * 32 + half * 16;
+                const char *src = smem + st * kStage + kOffC + (quad >> 1) * kBox + j0 * 128 + mrow;
+                const float *w = vw + (p.reverse ? 0 : kChunk - valid) + j0 + 2 * (lane & 3);
+                const F2 w0 = make2(w[0], w[1]), w1 = make2(w[8], w[9]);
+#pragma unroll 1
+                for (int d = 0; d < 2; ++d) {
+                    uint32_t r[4], t[3][4];
+                    tc::ldmatrix_x4_trans(src + ((((quad & 1) * 4 + d * 2 + mcol) ^ (lane & 7)) << 4), r);
 #pragma unroll
-                    for (int i = 0; i < KC; i += 16) {
-                        float t[16];
-                        tc::tmem_ld16(tmem + lanes + kColT + k0 + i, t);
-                        tc::tmem_wait_ld();
+                    for (int m = 0; m < 4; ++m) three_terms(mul2(m < 2 ? w0 : w1, unpack2(r[m])), t[0][m], t[1][m], t[2][m]);
 #pragma unroll
-                        for (int e = 0; e < 8; ++e) S[i / 2 + e] = fma2(carry, S[i / 2 + e], make2(t[2 * e], t[2 * e + 1]));
-                    }
+                    for (int u = 0; u < 3; ++u)
+                        tc::tmem_st_16x128b_x2(tmem + lanes + (d << 20) + kColV + hb * 48 + u * 16 + half * 8, t[u][0], t[u][1],
+                                               t[u][2], t[u][3]);
                 }
             }
-            before = valid;
-            if (n == steps) break;
-            arrive(&bar.vready[0]);
-            if (mine) scale16(1);
-            arrive(&bar.vready[1]);
-            if (++st == stages) st = 0, phase ^= 1;
-            if (!STATE_ONLY) {
+            if (hb == 0) {
                 if (n > 0) {
-                    ok = wait_warp(&bar.odone, (n - 1) & 1);  // the last chunk's reads of S are over
+                    ok = wait_warp(&bar.tdone, (n - 1) & 1);
                     if (!ok) break;
                     tc::fence_after_sync();
-                }
-                if (mine)
+                    if (mine) {
+                        const F2 carry = make2(pw[before], pw[before]);
 #pragma unroll
-                    for (int i = 0; i < KC; i += 32) {
-                        uint32_t r[16];
+                        for (int i = 0; i < KC; i += 16) {
+                            float t[16];
+                            tc::tmem_ld16(tmem + lanes + kColT + k0 + i, t);
+                            tc::tmem_wait_ld();
 #pragma unroll
-                        for (int e = 0; e < 16; ++e) r[e] = pack2(S[i / 2 + e]);
-                        tc::tmem_st16(tmem + lanes + kColS + (k0 + i) / 2, r);
+                            for (int e = 0; e < 8; ++e) S[i / 2 + e] = fma2(carry, S[i / 2 + e], make2(t[2 * e], t[2 * e + 1]));
+                        }
                     }
-                arrive(&bar.sready);
+                }
+                before = valid;
+                if (n == steps) break;
+                arrive(&bar.vready[0]);
+            } else {
+                arrive(&bar.vready[1]);
+                if (++st == stages) st = 0, phase ^= 1;
+                if (!STATE_ONLY) {
+                    if (n > 0) {
+                        ok = wait_warp(&bar.odone, (n - 1) & 1);  // the last chunk's reads of S are over
+                        if (!ok) break;
+                        tc::fence_after_sync();
+                    }
+                    if (mine)
+#pragma unroll
+                        for (int i = 0; i < KC; i += 32) {
+                            uint32_t r[16];
+#pragma unroll
+                            for (int e = 0; e < 16; ++e) r[e] = pack2(S[i / 2 + e]);
+                            tc::tmem_st16(tmem + lanes + kColS + (k0 + i) / 2, r);
+                        }
+                    arrive(&bar.sready);
+                }
             }
         }
         if (ok && col < p.wc) {
@@ -339,60 +349,84 @@ __global__ void __launch_bounds__(kThreads, 1) decay_walk_tc_kernel(const TcPara
             const uint32_t lanes = (uint32_t)(quad * 32) << 16;
             const bool on = col < p.wc;
             OT *out = static_cast<OT *>(p.out) + b * p.os[0] + h * p.os[2];
-            // 4-byte stores of two columns where every token's row allows them
-            const int odd = lane & 1, pair = col & ~1;
-            const bool both = pair + 1 < p.wc &&
-                              ((reinterpret_cast<uintptr_t>(p.out) & 3) | ((p.os[0] | p.os[1] | p.os[2]) & 1)) == 0;
+            constexpr bool kTma = sizeof(OT) == 2;  // BF16 outputs leave by TMA, FP32 ones (partial sums) by plain stores
+            const int mtok = ((lane >> 4) * 8 + (lane & 7)) * 128, mcol = (lane >> 3) & 1;
             for (int n = 0; n < steps; ++n) {
+                const int t0 = start_of(n), valid = valid_of(n);
+                char *stage = sP + (1 + (n & 1) * VB) * kBox;  // BF16 outputs on their way, [token][column]: the map's boxes
+                if (kTma && n > 1) {
+                    if (warp == kOutWarp && lane == 0) {
+                        tc::tma_store_wait_read<1>();
+                        tc::mbar_arrive(&bar.oempty);
+                    }
+                    if (!wait_warp(&bar.oempty, n & 1)) break;
+                }
                 if (!wait_warp(&bar.odone, n & 1)) break;
                 tc::fence_after_sync();
-                const int t0 = start_of(n), valid = valid_of(n), rows = min(time - t0, kChunk);
-                const bool full = valid == kChunk && both;
-                // neighbouring lanes swap halves of a BF16 pair, so that a lane stores two columns of one token:
-                // the even lane of the even tokens, the odd lane of the odd ones
-                OT *o = out + (int64_t)(sizeof(OT) == 4 ? t0 : t0 + odd) * p.os[1] + (sizeof(OT) == 4 ? col : pair);
-                const float *w = ow + (p.reverse ? kChunk - valid : 0);
+                if (quad < 2 * VB) {
+                    const float *w0 = ow + (p.reverse ? kChunk - valid : 0) + 2 * (lane & 3);
+                    // 16 columns by 32 tokens at a time.  Fragments: this lane has tokens 8 b + 2 (lane % 4) + {0, 1} of
+                    // column 16 d + lane / 4 (+ 8).
 #pragma unroll 1
-                for (int i = 0; i < 64; i += 16, w += 16) {
-                    if (quad >= 2 * VB) break;
-                    float y[16], z[16];
-                    tc::tmem_ld16(tmem + lanes + kColO2 + i, y);
-                    tc::tmem_ld16(tmem + lanes + kColO1 + i, z);
-                    tc::tmem_wait_ld();
+                    for (int q = 0; q < 4; ++q) {
+                        const int d = q >> 1, i = q & 1;
+                        float y[16], z[16];
+                        const uint32_t at = tmem + lanes + (d << 20) + i * 32;
+                        tc::tmem_ld_16x256b_x4(at + kColO2, y);
+                        tc::tmem_ld_16x256b_x4(at + kColO1, z);
+                        const float *w = w0 + i * 32;
+                        F2 wt[4];
 #pragma unroll
-                    for (int e = 0; e < 16; ++e) z[e] = fmaf(w[e], y[e], z[e]);
-                    if constexpr (sizeof(OT) == 4) {
+                        for (int e = 0; e < 4; ++e) wt[e] = make2(w[8 * e], w[8 * e + 1]);
+                        tc::tmem_wait_ld();
+                        F2 x[8];
 #pragma unroll
-                        for (int e = 0; e < 16; ++e, o += p.os[1])
-                            if (on && i + e < rows) *o = i + e < valid ? z[e] : 0.f;
-                    } else {
-                        uint32_t v[8];
+                        for (int e = 0; e < 8; ++e)
+                            x[e] = fma2(wt[e / 2], make2(y[2 * e], y[2 * e + 1]), make2(z[2 * e], z[2 * e + 1]));
+                        const int r0 = i * 32 + 2 * (lane & 3);
+                        if constexpr (kTma) {
+                            uint32_t v[8];
 #pragma unroll
-                        for (int e = 0; e < 8; ++e) {
-                            const uint32_t own = pack_bf16(z[2 * e], z[2 * e + 1]);
-                            const uint32_t other = __shfl_xor_sync(0xffffffffu, own, 1);
-                            v[e] = __byte_perm(odd ? other : own, odd ? own : other, odd ? 0x7632 : 0x5410);
-                        }
-                        if (full) {
+                            for (int e = 0; e < 8; ++e) v[e] = pack2(x[e]);
+                            if (valid < kChunk)  // padding gives zeros
 #pragma unroll
-                            for (int e = 0; e < 8; ++e, o += 2 * p.os[1]) *reinterpret_cast<uint32_t *>(o) = v[e];
+                                for (int e = 0; e < 8; ++e) {
+                                    const int r = r0 + e / 2 * 8;
+                                    v[e] &= (r < valid ? 0xffffu : 0u) | (r + 1 < valid ? 0xffff0000u : 0u);
+                                }
+                            char *dst = stage + (quad >> 1) * kBox + i * 32 * 128 + mtok +
+                                        ((((quad & 1) * 4 + d * 2 + mcol) ^ (lane & 7)) << 4);
+                            tc::stmatrix_x4_trans(dst, v[0], v[1], v[2], v[3]);
+                            tc::stmatrix_x4_trans(dst + 16 * 128, v[4], v[5], v[6], v[7]);
                         } else {
 #pragma unroll
-                            for (int e = 0; e < 8; ++e, o += 2 * p.os[1]) {
-                                const int r = i + 2 * e + odd;
-                                if (r >= rows || pair >= p.wc) continue;
-                                if (r >= valid) v[e] = 0;  // padding gives zeros
-                                const __nv_bfloat162 q = *reinterpret_cast<const __nv_bfloat162 *>(&v[e]);
-                                o[0] = q.x;
-                                if (pair + 1 < p.wc) o[1] = q.y;
+                            for (int e = 0; e < 8; ++e) {
+                                const int r = r0 + e / 2 * 8, c = quad * 32 + d * 16 + (e & 1) * 8 + (lane >> 2);
+                                const float2 v = split2(x[e]);
+                                OT *o = out + (int64_t)(t0 + r) * p.os[1] + c;
+                                if (c < p.wc && t0 + r < time) o[0] = r < valid ? v.x : 0.f;
+                                if (c < p.wc && t0 + r + 1 < time) o[p.os[1]] = r + 1 < valid ? v.y : 0.f;
                             }
                         }
                     }
                 }
                 tc::fence_before_sync();
+                if (kTma) tc::fence_async_smem();
                 __syncwarp();
-                if (lane == 0) tc::mbar_arrive(&bar.ofree);
+                if (lane == 0) {
+                    tc::mbar_arrive(&bar.ofree);
+                    if (kTma) tc::mbar_arrive(&bar.ofull);
+                }
+                if (kTma && warp == kOutWarp) {
+                    if (!wait_warp(&bar.ofull, n & 1)) break;
+                    if (lane == 0) {
+#pragma unroll
+                        for (int i = 0; i < VB; ++i) tc::tma_store_4d(&maps.out, stage + i * kBox, i * 64, t0, h, (int)b);
+                        tc::tma_store_commit();
+                    }
+                }
             }
+            if (kTma && warp == kOutWarp && lane == 0) tc::tma_store_wait();
             // whole chunks past the row's length
             int64_t z0 = sp.chunks * kChunk, z1 = p.time;
             const int64_t s0 = (int64_t)seg * p.cps * kChunk, s1 = s0 + (int64_t)p.cps * kChunk;
@@ -600,13 +634,13 @@ bool encode(EncodeTiled fn, CUtensorMap *m, const Operand &o, int64_t time, int6
 
 template <int DKB, int VB> constexpr int stages_of(bool state_only) {
     const int stage = (state_only ? DKB + VB : 2 * DKB + VB) * kBox;
-    int n = (kSmemMax - 1024 - 3072 - kBox) / stage;
+    int n = (kSmemMax - 1024 - 3072 - (1 + 2 * VB) * kBox) / stage;
     return n > kMaxStages ? kMaxStages : n;
 }
 
 template <int DKB, int VB, typename OT, bool STATE_ONLY> int launch(TcParams &tp, const Maps &maps, cudaStream_t st) {
     tp.stages = stages_of<DKB, VB>(STATE_ONLY);
-    const int smem = tp.stages * (STATE_ONLY ? DKB + VB : 2 * DKB + VB) * kBox + kBox + 1024;
+    const int smem = tp.stages * (STATE_ONLY ? DKB + VB : 2 * DKB + VB) * kBox + (1 + 2 * VB) * kBox + 1024;
     auto kernel = decay_walk_tc_kernel<DKB, VB, OT, STATE_ONLY>;
     constexpr int kMaxDevices = 64;
     static std::mutex mu;
@@ -642,6 +676,10 @@ bool decay_walk_tc_takes(const bdm_decay_walk_args &w) {
                             {w.c, w.c_stride, w.width_c, w.c_heads}};
     for (const Operand &o : ops)
         if (!fits_tma(o, w.time, w.batch)) return false;
+    if (w.out_dtype == BDM_BF16) {
+        if (!fits_tma({w.out, w.out_stride, w.width_c, w.heads}, w.time, w.batch)) return false;
+        if ((w.batch > 1 && !w.out_stride[0]) || (w.heads > 1 && !w.out_stride[2])) return false;
+    }
     return encode_tiled() != nullptr;
 }
 
@@ -671,6 +709,11 @@ int decay_walk_tc_launch(const bdm_decay_walk_args &w, const Params &p, bool sta
     CUtensorMap *m[3] = {&maps.a, &maps.b, &maps.c};
     for (int i = 0; i < 3; ++i)
         if (!encode(fn, m[i], ops[i], w.time, w.batch, tp.amul[i], tp.bmul[i])) return BDM_ERR_UNSUPPORTED;
+    if (w.out_dtype == BDM_BF16) {
+        int amul, bmul;
+        if (!encode(fn, &maps.out, {w.out, w.out_stride, w.width_c, w.heads}, w.time, w.batch, amul, bmul))
+            return BDM_ERR_UNSUPPORTED;
+    }
     const bool f32 = w.out_dtype == BDM_F32;
     if (p.wab > 64) {
         if (p.wc > 64) return launch_types<2, 2>(tp, maps, f32, state_only, st);
