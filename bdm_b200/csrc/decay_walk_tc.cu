@@ -48,12 +48,11 @@ struct Maps {
 struct TcParams {
     Params p;
     int amul[3], bmul[3];  // 0 where the operand's batch (head) is shared by all: a, b, c
-    int stages;
 };
 
 struct Bars {
     uint64_t full[kMaxStages], empty[kMaxStages];
-    uint64_t vready[2], sready, thalf, tdone, adone, pready, odone, ofree, zeroed, ofull, oempty;
+    uint64_t vready[2], tpart[2], sready, adone, pready, odone, ofree, zeroed, ofull, oempty;
 };
 
 __device__ __forceinline__ uint32_t pack_bf16(float lo, float hi) {
@@ -139,6 +138,13 @@ __device__ __forceinline__ void start_states(const Params &p, const Span &s, int
     }
 }
 
+// Stages of the load pipeline: what shared memory holds beside P and two buffers of outputs.
+template <int DKB, int VB, bool STATE_ONLY> constexpr int stages_of() {
+    const int stage = (STATE_ONLY ? DKB + VB : 2 * DKB + VB) * kBox;
+    const int n = (kSmemMax - 1024 - 3072 - (1 + 2 * VB) * kBox) / stage;
+    return n > kMaxStages ? kMaxStages : n;
+}
+
 // DKB, VB: 64-column boxes of a / b and of c.
 template <int DKB, int VB, typename OT, bool STATE_ONLY>
 __global__ void __launch_bounds__(kThreads, 1) decay_walk_tc_kernel(const TcParams tp, const __grid_constant__ Maps maps) {
@@ -155,7 +161,7 @@ __global__ void __launch_bounds__(kThreads, 1) decay_walk_tc_kernel(const TcPara
     constexpr int kStage = (STATE_ONLY ? DKB + VB : 2 * DKB + VB) * kBox;
     constexpr int kOffB = STATE_ONLY ? 0 : DKB * kBox, kOffC = kOffB + DKB * kBox;
     constexpr int DK = DKB * 64;
-    const int stages = tp.stages;
+    constexpr int stages = stages_of<DKB, VB, STATE_ONLY>();
     char *sP = smem + stages * kStage;
 
     int64_t id = blockIdx.x;
@@ -185,9 +191,9 @@ __global__ void __launch_bounds__(kThreads, 1) decay_walk_tc_kernel(const TcPara
         }
         tc::mbar_init(&bar.vready[0], kStateWarps);
         tc::mbar_init(&bar.vready[1], kStateWarps);
-        tc::mbar_init(&bar.thalf, 1);
+        tc::mbar_init(&bar.tpart[0], 1);
         tc::mbar_init(&bar.sready, kStateWarps);
-        tc::mbar_init(&bar.tdone, 1);
+        tc::mbar_init(&bar.tpart[1], 1);
         tc::mbar_init(&bar.adone, 1);
         tc::mbar_init(&bar.pready, 2);
         tc::mbar_init(&bar.odone, 1);
@@ -260,7 +266,7 @@ __global__ void __launch_bounds__(kThreads, 1) decay_walk_tc_kernel(const TcPara
                     if (!ok) break;
                 }
                 if (n > 0) {
-                    ok = wait_warp(&bar.thalf, (n - 1) & 1);
+                    ok = wait_warp(&bar.tpart[0], (n - 1) & 1);
                     if (!ok) break;
                     tc::fence_after_sync();
                 }
@@ -286,7 +292,7 @@ __global__ void __launch_bounds__(kThreads, 1) decay_walk_tc_kernel(const TcPara
             }
             if (hb == 0) {
                 if (n > 0) {
-                    ok = wait_warp(&bar.tdone, (n - 1) & 1);
+                    ok = wait_warp(&bar.tpart[1], (n - 1) & 1);
                     if (!ok) break;
                     tc::fence_after_sync();
                     if (mine) {
@@ -477,11 +483,11 @@ __global__ void __launch_bounds__(kThreads, 1) decay_walk_tc_kernel(const TcPara
         }
     } else if (warp == kTmaWarp) {
         // ------------------------------------------------------------------ loads
-        if (lane == 0) {
+        if (tc::elect_one()) {
             int issued = 0;
+            int st = 0, phase = 0;
             for (int n = 0; n < steps; ++n) {
-                const int st = n % stages;
-                if (n >= stages && !wait(&bar.empty[st], ((n / stages) - 1) & 1)) break;
+                if (n >= stages && !wait(&bar.empty[st], phase ^ 1)) break;
                 char *dst = smem + st * kStage;
                 const int t0 = start_of(n);
                 tc::mbar_arrive_expect_tx(&bar.full[st], kStage);
@@ -499,6 +505,7 @@ __global__ void __launch_bounds__(kThreads, 1) decay_walk_tc_kernel(const TcPara
                     tc::tma_load_4d(dst + kOffC + i * kBox, &maps.c, i * 64, t0, (h / p.cg) * tp.bmul[2],
                                     (int)b * tp.amul[2], &bar.full[st]);
                 issued = n + 1;
+                if (++st == stages) st = 0, phase ^= 1;
             }
             // no copy may be in flight when the CTA ends, whatever happened to its consumers
             for (int n = issued > stages ? issued - stages : 0; n < issued; ++n)
@@ -515,59 +522,59 @@ __global__ void __launch_bounds__(kThreads, 1) decay_walk_tc_kernel(const TcPara
             const uint32_t base = tc::smem_u32(smem);
             const uint64_t dP = tc::smem_desc_sw128(tc::smem_u32(sP));
             // rows 64..127 of the scores, and value columns past c's boxes, are whatever follows the tile
-            auto scores = [&](int n) {
-                const uint64_t qa = tc::smem_desc_sw128(base + (n % stages) * kStage), kb = qa + kOffB / 16;
+            auto scores = [&](int st) {
+                uint64_t qa = tc::smem_desc_sw128(base + st * kStage), kb = qa + kOffB / 16;
+#pragma unroll 1
+                for (int i = 0; i < DKB; ++i, qa += kBox / 16, kb += kBox / 16)
 #pragma unroll
-                for (int k = 0; k < DK / 16; ++k) {
-                    const uint32_t off = ((k / 4) * kBox + (k % 4) * 32) / 16;
-                    tc::mma_bf16(tmem + kColA, qa + off, kb + off, idQK, k > 0);
-                }
+                    for (int k = 0; k < 4; ++k) tc::mma_bf16(tmem + kColA, qa + k * 2, kb + k * 2, idQK, i + k > 0);
                 tc::mma_commit(&bar.adone);
             };
             bool ok = true;
-            int done = 0;
+            int done = 0, st = 0, phase = 0;
             if (!STATE_ONLY && steps > 0) {
                 ok = wait(&bar.full[0], 0);
                 if (ok) scores(0);
             }
             for (int n = 0; n < steps && ok; ++n) {
-                const int st = n % stages;
-                const uint64_t qa = tc::smem_desc_sw128(base + st * kStage);
-                const uint64_t kb = tc::smem_desc_sw128_mn(base + st * kStage + kOffB, kBox);
-                const uint64_t vc = tc::smem_desc_sw128_mn(base + st * kStage + kOffC, kBox);
-#pragma unroll
-                for (int hb = 0; hb < 2; ++hb) {
+                const uint32_t tile = base + st * kStage;
+                uint64_t kb = tc::smem_desc_sw128_mn(tile + kOffB, kBox);
+                uint32_t va = tmem + kColV;
+#pragma unroll 1
+                for (int hb = 0; hb < 2; ++hb, kb += 2 * 2048 / 16, va += 48) {
                     if (!(ok = wait(&bar.vready[hb], n & 1))) break;
                     tc::fence_after_sync();
 #pragma unroll
                     for (int t = 0; t < 3; ++t)
 #pragma unroll
                         for (int k = 0; k < 2; ++k)
-                            tc::mma_bf16_tmem_a(tmem + kColT, tmem + kColV + hb * 48 + t * 16 + k * 8,
-                                                kb + (2 * hb + k) * 2048 / 16, idT, hb + t + k > 0);
-                    tc::mma_commit(hb ? &bar.tdone : &bar.thalf);
+                            tc::mma_bf16_tmem_a(tmem + kColT, va + t * 16 + k * 8, kb + k * 2048 / 16, idT, hb + t + k > 0);
+                    tc::mma_commit(&bar.tpart[hb]);
                 }
                 if (!ok) break;
                 if (!STATE_ONLY) {
                     if (!(ok = wait(&bar.sready, n & 1))) break;
                     if (n > 0 && !(ok = wait(&bar.ofree, (n - 1) & 1))) break;
                     tc::fence_after_sync();
+                    uint64_t qa = tc::smem_desc_sw128(tile);
+                    uint32_t sa = tmem + kColS;
+#pragma unroll 1
+                    for (int i = 0; i < DKB; ++i, qa += kBox / 16, sa += 32)
 #pragma unroll
-                    for (int k = 0; k < DK / 16; ++k)
-                        tc::mma_bf16_tmem_a(tmem + kColO2, tmem + kColS + k * 8, qa + ((k / 4) * kBox + (k % 4) * 32) / 16,
-                                            idO2, k > 0);
+                        for (int k = 0; k < 4; ++k) tc::mma_bf16_tmem_a(tmem + kColO2, sa + k * 8, qa + k * 2, idO2, i + k > 0);
                     if (!(ok = wait(&bar.pready, n & 1))) break;
                     tc::fence_after_sync();
+                    const uint64_t vc = tc::smem_desc_sw128_mn(tile + kOffC, kBox);
 #pragma unroll
-                    for (int k = 0; k < 4; ++k)
-                        tc::mma_bf16(tmem + kColO1, vc + k * 2048 / 16, dP + k * 32 / 16, idO1, k > 0);
+                    for (int k = 0; k < 4; ++k) tc::mma_bf16(tmem + kColO1, vc + k * 2048 / 16, dP + k * 2, idO1, k > 0);
                     tc::mma_commit(&bar.odone);
                 }
                 tc::mma_commit(&bar.empty[st]);
                 done = n + 1;
+                if (++st == stages) st = 0, phase ^= 1;
                 if (!STATE_ONLY && n + 1 < steps) {
-                    if (!(ok = wait(&bar.full[(n + 1) % stages], ((n + 1) / stages) & 1))) break;
-                    scores(n + 1);
+                    if (!(ok = wait(&bar.full[st], phase))) break;
+                    scores(st);
                 }
             }
             // nor a product
@@ -632,15 +639,8 @@ bool encode(EncodeTiled fn, CUtensorMap *m, const Operand &o, int64_t time, int6
               CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) == CUDA_SUCCESS;
 }
 
-template <int DKB, int VB> constexpr int stages_of(bool state_only) {
-    const int stage = (state_only ? DKB + VB : 2 * DKB + VB) * kBox;
-    int n = (kSmemMax - 1024 - 3072 - (1 + 2 * VB) * kBox) / stage;
-    return n > kMaxStages ? kMaxStages : n;
-}
-
 template <int DKB, int VB, typename OT, bool STATE_ONLY> int launch(TcParams &tp, const Maps &maps, cudaStream_t st) {
-    tp.stages = stages_of<DKB, VB>(STATE_ONLY);
-    const int smem = tp.stages * (STATE_ONLY ? DKB + VB : 2 * DKB + VB) * kBox + (1 + 2 * VB) * kBox + 1024;
+    const int smem = stages_of<DKB, VB, STATE_ONLY>() * (STATE_ONLY ? DKB + VB : 2 * DKB + VB) * kBox + (1 + 2 * VB) * kBox + 1024;
     auto kernel = decay_walk_tc_kernel<DKB, VB, OT, STATE_ONLY>;
     constexpr int kMaxDevices = 64;
     static std::mutex mu;
