@@ -101,10 +101,10 @@ SIGNATURES = {
     'bdm_norm_gate_f32': (_int, [_vp, _i64, _i64, _vp, _i64, _vp, _vp, _flt, _int, _int, _vp, _vp]),
     'bdm_decode_step': (_int, [_vp, _vp, _vp, _vp, _vp, _vp, _vp, _vp, _vp, _vp, _i64, _i64, _int, _int, _int, _int,
                                _int, _int, _int, _flt, _vp, _int, _vp, _vp, _i64, _vp, _vp, _flt, _int, _vp, _vp]),
-    'bdm_decay_walk_workspace_bytes': (_i64, [ctypes.POINTER(DecayWalkArgs)]),
-    'bdm_decay_walk': (_int, [ctypes.POINTER(DecayWalkArgs), _vp, _i64, _vp]),
+    'bdm_decay_walk_workspace_bytes': (_i64, [_vp]),
+    'bdm_decay_walk': (_int, [_vp, _vp, _i64, _vp]),
     'bdm_decay_group_sum': (_int, [_vp, _i64, _int, _int, _int, _int, _vp, _vp]),
-    'bdm_decay_step': (_int, [ctypes.POINTER(DecayStepArgs), _vp]),
+    'bdm_decay_step': (_int, [_vp, _vp]),
     'bdm_beam_select_workspace_bytes': (_i64, [_i64, _int, _i64]),
     'bdm_beam_select': (_int, [_vp, _i64, _i64, _int, _i64, _int, _vp, _vp, _i64, _int, _vp, _vp, _vp, _vp, _vp, _i64,
                                _vp]),

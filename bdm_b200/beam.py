@@ -14,7 +14,7 @@ from typing import NamedTuple
 import torch
 
 from . import _lib, ops
-from .decay import _on
+from .decay import _on, _raw_stream
 
 MAX_BEAMS = 32
 
@@ -69,12 +69,12 @@ def beam_select(logits, scores, *, finished=None, eos_token=None, stable_slots=F
         out_scores = torch.empty((batch, beams), dtype=torch.float32, device=dev)
         index = torch.empty((2, batch, beams), dtype=torch.int64, device=dev)
         done = torch.empty((batch, beams), dtype=torch.bool, device=dev)
-        parents, tokens = index[0], index[1]
+        parents, tokens = index.unbind(0)
         ld = rows.stride(0) if batch * beams > 1 else vocab
         _lib.check(lib.bdm_beam_select(rows.data_ptr(), ld, batch, beams, vocab, code, scores.data_ptr(),
                                        ops._ptr(finished), -1 if eos_token is None else int(eos_token),
                                        int(stable_slots), out_scores.data_ptr(), parents.data_ptr(), tokens.data_ptr(),
-                                       done.data_ptr(), ws.data_ptr(), nbytes, ops._stream(dev)), 'bdm_beam_select')
+                                       done.data_ptr(), ws.data_ptr(), nbytes, _raw_stream(dev)), 'bdm_beam_select')
     return BeamStep(out_scores, parents, tokens, done)
 
 
@@ -119,7 +119,7 @@ def reorder_states(states, parents):
     with _on(dev):
         _lib.check(_lib.load().bdm_reorder_rows((ctypes.c_void_p * n)(*bases), (ctypes.c_int64 * n)(*strides),
                                                 (ctypes.c_int64 * n)(*sizes), n, parents.data_ptr(), batch, beams,
-                                                ops._scan_status_of(dev).word.data_ptr(), ops._stream(dev)),
+                                                ops._scan_status_of(dev).mapped_ptr + 4, _raw_stream(dev)),
                    'bdm_reorder_rows')
     return states
 

@@ -432,7 +432,7 @@ __global__ void __launch_bounds__(kThreads)
             if (s >= 0 && s < beams)
                 src[i] = (int)s;
             else if (status && threadIdx.x == 0)
-                atomicOr(status, 0x8);  // the row keeps its state
+                *(volatile int *)status = 0x8;  // the row keeps its state
             any |= src[i] != i;
         }
     }

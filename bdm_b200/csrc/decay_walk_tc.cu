@@ -584,7 +584,7 @@ __global__ void __launch_bounds__(kThreads, 1) decay_walk_tc_kernel(const TcPara
     __syncwarp();
     tc::fence_before_sync();
     __syncthreads();
-    if (threadIdx.x == 0 && dead && p.status) atomicOr(p.status, 0x4);
+    if (threadIdx.x == 0 && dead && p.status) *(volatile int *)p.status = 0x4;
     if (warp == kMmaWarp) {
         tc::fence_after_sync();
         tc::tmem_dealloc(tmem, 512);

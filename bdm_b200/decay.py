@@ -11,8 +11,8 @@ model can interleave the two (``HybridLanguageModel``).  There is no reference c
 """
 from __future__ import annotations
 
-import ctypes
 import math
+import struct
 from contextlib import nullcontext
 
 import torch
@@ -22,9 +22,16 @@ from torch.nn import functional as F
 from . import _lib, ops
 
 
+_HERE = nullcontext()
+
+
 def _on(device):
     """The launches below go to the device of their tensors."""
-    return nullcontext() if device.index == torch.cuda.current_device() else torch.cuda.device(device)
+    return _HERE if device.index == torch._C._cuda_getDevice() else torch.cuda.device(device)
+
+
+def _raw_stream(device) -> int:
+    return torch._C._cuda_getCurrentRawStream(device.index)
 
 
 def _rows(x):
@@ -32,28 +39,35 @@ def _rows(x):
     return x if x.stride(-1) == 1 or x.shape[-1] == 1 else x.contiguous()
 
 
-_I3 = ctypes.c_int64 * 3
-_I2 = ctypes.c_int64 * 2
+# bdm_decay_walk_args and bdm_decay_step_args (include/bdm_b200.h), packed in one go: filling a ctypes
+# structure field by field costs several times as much
+_WALK = struct.Struct('9P12q2q11i3f')
+_STEP = struct.Struct('6P6qq5if')
 
 
-def _walk(a, b, c, log_decay, lengths, *, heads, scale, reverse=False, out_dtype=None, state_in=None, state_in_mul=1.0,
-          state_in_transposed=False, state_out=None, state_out_mul=1.0, state_out_transposed=False):
+def _walk(a, b, c, log_decay, lengths, st, *, heads, scale, reverse=0, out_dtype=None, state_in=None, state_in_mul=1.0,
+          state_in_transposed=0, state_out=None, state_out_mul=1.0):
     """One bdm_decay_walk over [B, T, heads of the operand, width] tensors; returns out [B, T, heads, width of c]."""
-    batch, time = a.shape[:2]
-    out = torch.empty((batch, time, heads, c.shape[-1]), dtype=out_dtype or a.dtype, device=a.device)
-    w = _lib.DecayWalkArgs(
-        a.data_ptr(), b.data_ptr(), c.data_ptr(), out.data_ptr(), log_decay.data_ptr(), ops._ptr(lengths),
-        ops._ptr(state_in), ops._ptr(state_out), ops._scan_status_of(a.device).word.data_ptr(),
-        _I3(*a.stride()[:3]), _I3(*b.stride()[:3]), _I3(*c.stride()[:3]), _I3(*out.stride()[:3]), batch, time, heads,
-        a.shape[2], b.shape[2], c.shape[2], a.shape[3], c.shape[3], ops.dtype_code(a.dtype),
-        ops.dtype_code(out.dtype), int(reverse), int(state_in_transposed), int(state_out_transposed), scale,
-        state_in_mul, state_out_mul)
+    batch, time, a_heads, wab = a.shape
+    c_heads, wc = c.shape[2:]
+    dt = a.dtype
+    out = torch.empty((batch, time, heads, wc), dtype=out_dtype or dt, device=a.device)
+    w = _WALK.pack(a.data_ptr(), b.data_ptr(), c.data_ptr(), out.data_ptr(), log_decay.data_ptr(),
+                   0 if lengths is None else lengths.data_ptr(), 0 if state_in is None else state_in.data_ptr(),
+                   0 if state_out is None else state_out.data_ptr(), st.mapped_ptr,
+                   *a.stride()[:3], *b.stride()[:3], *c.stride()[:3], time * heads * wc, heads * wc, wc,
+                   batch, time, heads, a_heads, b.shape[2], c_heads, wab, wc, ops._DT[dt], ops._DT[out.dtype],
+                   reverse, state_in_transposed, 0, scale, state_in_mul, state_out_mul)
     lib = _lib.load()
-    nbytes = lib.bdm_decay_walk_workspace_bytes(ctypes.byref(w))
-    if nbytes < 0:
+    nbytes = lib.bdm_decay_walk_workspace_bytes(w)
+    ws = None
+    if nbytes > 0:
+        ws = torch.empty(nbytes, dtype=torch.uint8, device=a.device)
+    elif nbytes < 0:
         raise ValueError('invalid decay-attention geometry')
-    ws = torch.empty(nbytes, dtype=torch.uint8, device=a.device) if nbytes else None
-    _lib.check(lib.bdm_decay_walk(ctypes.byref(w), ops._ptr(ws), nbytes, ops._stream(a.device)), 'bdm_decay_walk')
+    status = lib.bdm_decay_walk(w, ws.data_ptr() if nbytes else None, nbytes, _raw_stream(a.device))
+    if status:
+        _lib.check(status, 'bdm_decay_walk')
     return out
 
 
@@ -62,23 +76,27 @@ def _group_sum(part, kv_heads, dtype):
     batch, time, heads, width = part.shape
     out = torch.empty((batch, time, kv_heads, width), dtype=dtype, device=part.device)
     _lib.check(_lib.load().bdm_decay_group_sum(part.data_ptr(), batch * time, kv_heads, heads // kv_heads, width,
-                                               ops.dtype_code(dtype), out.data_ptr(), ops._stream(part.device)),
+                                               ops._DT[dtype], out.data_ptr(), _raw_stream(part.device)),
                'bdm_decay_group_sum')
     return out
+
+
+def _forward(q, k, v, log_decay, initial_state, lengths, scale):
+    heads = q.shape[2]
+    state = torch.empty((q.shape[0], heads, q.shape[3], v.shape[3]), dtype=torch.float32, device=q.device)
+    with _on(q.device):
+        out = _walk(q, k, v, log_decay, lengths, ops._scan_status_of(q.device), heads=heads, scale=scale,
+                    state_in=initial_state, state_out=state)
+    return out, state
 
 
 class _DecayAttention(torch.autograd.Function):
     @staticmethod
     def forward(ctx, q, k, v, log_decay, initial_state, lengths, scale):
-        q, k, v = _rows(q), _rows(k), _rows(v)
-        heads = q.shape[2]
-        state = torch.empty((q.shape[0], heads, q.shape[3], v.shape[3]), dtype=torch.float32, device=q.device)
-        with _on(q.device):
-            out = _walk(q, k, v, log_decay, lengths, heads=heads, scale=scale, state_in=initial_state, state_out=state)
         ctx.save_for_backward(q, k, v, log_decay, initial_state, lengths)
         ctx.scale = scale
         ctx.set_materialize_grads(False)
-        return out, state
+        return _forward(q, k, v, log_decay, initial_state, lengths, scale)
 
     @staticmethod
     @torch.autograd.function.once_differentiable
@@ -93,37 +111,41 @@ class _DecayAttention(torch.autograd.Function):
         dq = dk = dv = ds0 = None
         shared = kv_heads != heads
         walk = dict(heads=heads, scale=scale)
-        back = dict(walk, reverse=True, state_in=dstate, state_in_mul=1.0 / scale,
+        back = dict(walk, reverse=1, state_in=dstate, state_in_mul=1.0 / scale,
                     out_dtype=torch.float32 if shared else dt)
         with _on(q.device):
-            ops.check_scan_status(q.device)
+            st = ops._scan_status_of(q.device)
+            ops.check_mapped_status(st)
             if need[0]:
-                dq = _walk(do, v, k, log_decay, lengths, state_in=s0, state_in_transposed=True, **walk)
+                dq = _walk(do, v, k, log_decay, lengths, st, state_in=s0, state_in_transposed=1, **walk)
             if need[1]:
-                dk = _walk(v, do, q, log_decay, lengths, state_in_transposed=True, **back)
+                dk = _walk(v, do, q, log_decay, lengths, st, state_in_transposed=1, **back)
                 dk = _group_sum(dk, kv_heads, dt) if shared else dk
             if need[2] or need[4]:
                 ds0 = torch.empty((q.shape[0], heads, q.shape[3], v.shape[3]), dtype=torch.float32,
                                   device=q.device) if need[4] else None
-                dv = _walk(k, q, do, log_decay, lengths, state_out=ds0, state_out_mul=scale, **back)
+                dv = _walk(k, q, do, log_decay, lengths, st, state_out=ds0, state_out_mul=scale, **back)
                 dv = _group_sum(dv, kv_heads, dt) if shared else dv
         return dq, dk, dv if need[2] else None, None, ds0, None, None
 
 
 def _check_heads(q, k, v, log_decay, scale):
-    ops._cuda(q, k, v, log_decay)
-    if q.dtype != k.dtype or q.dtype != v.dtype:
+    dev, dt = q.device, q.dtype
+    if not (q.is_cuda and k.is_cuda and v.is_cuda and log_decay.is_cuda):
+        ops._cuda(q, k, v, log_decay)
+    if k.dtype != dt or v.dtype != dt:
         raise ValueError('q, k and v must share one dtype')
-    ops.dtype_code(q.dtype)
-    if any(t.device != q.device for t in (k, v, log_decay)):
+    ops.dtype_code(dt)
+    if k.device != dev or v.device != dev or log_decay.device != dev:
         raise ValueError('q, k, v and log_decay must be on one device')
-    heads, kv_heads, dk = q.shape[-2], k.shape[-2], q.shape[-1]
-    if k.shape[-1] != dk or v.shape[-2] != kv_heads or k.shape[:-2] != q.shape[:-2] or v.shape[:-2] != q.shape[:-2]:
+    qs, ks, vs = q.shape, k.shape, v.shape
+    heads, kv_heads, dk = qs[-2], ks[-2], qs[-1]
+    if ks[-1] != dk or vs[-2] != kv_heads or ks[:-2] != qs[:-2] or vs[:-2] != qs[:-2]:
         raise ValueError('k must be [..., kv_heads, key width of q] and v [..., kv_heads, value width], '
                          'with the leading sizes of q')
-    if min(heads, kv_heads, dk, v.shape[-1]) < 1 or heads % kv_heads:
+    if heads < 1 or kv_heads < 1 or dk < 1 or vs[-1] < 1 or heads % kv_heads:
         raise ValueError('the heads of q must be a multiple of the heads of k and v')
-    if log_decay.dtype != torch.float32 or tuple(log_decay.shape) != (heads,) or not log_decay.is_contiguous():
+    if log_decay.dtype != torch.float32 or log_decay.shape != (heads,) or not log_decay.is_contiguous():
         raise ValueError(f'log_decay must be a contiguous float32 [{heads}] tensor')
     if log_decay.requires_grad and torch.is_grad_enabled():
         raise ValueError('log_decay is a constant: it gets no gradient')
@@ -161,8 +183,13 @@ def decay_attention(q, k, v, log_decay, *, scale=None, initial_state=None, lengt
         raise ValueError(f'lengths must be a contiguous int64 [{batch}] tensor on {q.device}')
     if q.shape[3] > 128 or v.shape[3] > 128:
         raise NotImplementedError('decay_attention supports head widths up to 128')
-    ops.check_scan_status(q.device)
-    out, state = _DecayAttention.apply(q, k, v, log_decay, initial_state, lengths, scale)
+    ops.check_mapped_status(ops._scan_status_of(q.device))
+    q, k, v = _rows(q), _rows(k), _rows(v)
+    run = _forward
+    if torch.is_grad_enabled() and (q.requires_grad or k.requires_grad or v.requires_grad
+                                    or (initial_state is not None and initial_state.requires_grad)):
+        run = _DecayAttention.apply
+    out, state = run(q, k, v, log_decay, initial_state, lengths, scale)
     return (out, state) if return_state else out
 
 
@@ -184,11 +211,13 @@ def decay_attention_step(q, k, v, log_decay, state, *, scale=None):
         raise NotImplementedError('decay_attention_step supports key widths up to 1024')
     q, k, v = _rows(q), _rows(k), _rows(v)
     out = torch.empty((batch, heads, dv), dtype=q.dtype, device=q.device)
-    a = _lib.DecayStepArgs(q.data_ptr(), k.data_ptr(), v.data_ptr(), log_decay.data_ptr(), state.data_ptr(),
-                           out.data_ptr(), _I2(*q.stride()[:2]), _I2(*k.stride()[:2]), _I2(*v.stride()[:2]), batch,
-                           heads, k.shape[1], dk, dv, ops.dtype_code(q.dtype), scale)
+    a = _STEP.pack(q.data_ptr(), k.data_ptr(), v.data_ptr(), log_decay.data_ptr(), state.data_ptr(), out.data_ptr(),
+                   *q.stride()[:2], *k.stride()[:2], *v.stride()[:2], batch, heads, k.shape[1], dk, dv,
+                   ops._DT[q.dtype], scale)
     with _on(q.device):
-        _lib.check(_lib.load().bdm_decay_step(ctypes.byref(a), ops._stream(q.device)), 'bdm_decay_step')
+        status = _lib.load().bdm_decay_step(a, _raw_stream(q.device))
+    if status:
+        _lib.check(status, 'bdm_decay_step')
     return out
 
 

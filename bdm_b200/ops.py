@@ -25,6 +25,8 @@ Training backward:
 """
 from __future__ import annotations
 
+import ctypes
+
 import torch
 
 from . import _lib
@@ -73,8 +75,15 @@ class _ScanStatus:
         with torch.inference_mode(False):
             self.word = torch.zeros(1, dtype=torch.int32, device=device)
             self.host = torch.zeros(1, dtype=torch.int32, pin_memory=True)
+            # words that kernels set directly (pinned, mapped): reading them costs the host nothing
+            self.mapped = torch.zeros(2, dtype=torch.int32, pin_memory=True)
+        self.mapped_ptr = self.mapped.data_ptr()
+        self._words = (ctypes.c_int32 * 2).from_address(self.mapped_ptr)
         self.event = None
         self.last = 0
+
+    def mapped_bits(self) -> int:
+        return self._words[0] | self._words[1]
 
 
 _SCAN_STATUS: dict = {}
@@ -99,12 +108,12 @@ def scan_status(device=None, *, wait: bool = False) -> int:
     """
     st = _scan_status_of(device)
     if torch.cuda.is_current_stream_capturing():
-        return st.last
+        return st.last | st.mapped_bits()
     stream = torch.cuda.current_stream(st.word.device)
     if wait:
         stream.synchronize()
         st.last = int(st.word.item())
-        return st.last
+        return st.last | st.mapped_bits()
     if st.event is not None and st.event.query():
         st.last = int(st.host.item())
         st.event = None
@@ -112,7 +121,7 @@ def scan_status(device=None, *, wait: bool = False) -> int:
         st.host.copy_(st.word, non_blocking=True)
         st.event = torch.cuda.Event()
         st.event.record(stream)
-    return st.last
+    return st.last | st.mapped_bits()
 
 
 def check_scan_status(device=None, *, wait: bool = False) -> None:
@@ -121,14 +130,28 @@ def check_scan_status(device=None, *, wait: bool = False) -> None:
         return
     bits = scan_status(device, wait=wait)
     if bits:
-        raise _lib.BDMError(f'bank kernels: device status {bits:#x} (a bounded wait inside a kernel gave up: 0x1 '
-                            f'recurrence, 0x2 combine + output projection; outputs since then are unspecified; '
-                            f'reset with ops.reset_scan_status)')
+        _raise_status(bits)
+
+
+def _raise_status(bits):
+    raise _lib.BDMError(f'bank kernels: device status {bits:#x} (a bounded wait inside a kernel gave up: 0x1 '
+                        f'recurrence, 0x2 combine + output projection, 0x4 decay attention; 0x8: a parent of a '
+                        f'reordering was out of range; outputs since then are unspecified; '
+                        f'reset with ops.reset_scan_status)')
+
+
+def check_mapped_status(st: _ScanStatus) -> None:
+    """Raises BDMError if a kernel has set one of the mapped words: no call into the driver, at most the
+    launches still running late."""
+    bits = st.mapped_bits()
+    if bits:
+        _raise_status(bits)
 
 
 def reset_scan_status(device=None) -> None:
     st = _scan_status_of(device)
     st.word.zero_()
+    st.mapped.zero_()
     if st.event is not None:
         st.event.synchronize()
         st.event = None

@@ -477,7 +477,8 @@ BDM_API int bdm_decode_token_step(const void *proj, int64_t batch, int64_t ld, i
  * Strides are in elements, in the order batch, token, head; columns are contiguous.  Head h uses head
  * h / (heads / x_heads) of operand x.  States are FP32 [batch, heads, width_ab, width_c], or with
  * *_transposed [batch, heads, width_c, width_ab].  Products, sums and states are FP32.
- * width_ab, width_c <= 128.  status (optional int): 0x4 is ORed in if a bounded wait gave up.
+ * width_ab, width_c <= 128.  status (optional, an int the device can write, mapped host
+ * memory included): set to 0x4 if a bounded wait gave up; the outputs are then unspecified.
  */
 typedef struct bdm_decay_walk_args {
     const void *a, *b, *c;
@@ -539,7 +540,7 @@ BDM_API int bdm_beam_select(const void *logits, int64_t ld, int64_t batch, int b
 /*
  * In place, for every tensor: row (g, i) <- row (g, parents[g, i]) of its groups * beams rows of row_bytes
  * bytes, row_strides bytes apart.  bases, row_strides and row_bytes are host arrays of `count` entries.  A
- * parent out of range keeps the row and ORs 0x8 into status (optional).  beams <= 32.
+ * parent out of range keeps the row and sets status (optional, as above) to 0x8.  beams <= 32.
  */
 BDM_API int bdm_reorder_rows(void *const *bases, const int64_t *row_strides, const int64_t *row_bytes, int count,
                              const int64_t *parents, int64_t groups, int beams, int *status, void *stream);
