@@ -101,10 +101,12 @@ def reorder_states(states, parents):
             raise RuntimeError('reorder_states requires no_grad or inference_mode for states that need gradients')
         if s.numel() == 0:
             continue
-        if not s[0].is_contiguous():
-            raise ValueError('the rows of a state must be contiguous')
-        size = s[0].numel() * s.element_size()
-        stride = s.stride(0) * s.element_size() if s.shape[0] > 1 else size
+        size = s.numel() // (batch * beams) * s.element_size()
+        stride = size
+        if not s.is_contiguous():
+            if not s[0].is_contiguous():
+                raise ValueError('the rows of a state must be contiguous')
+            stride = s.stride(0) * s.element_size() if s.shape[0] > 1 else size
         if stride < size:
             raise ValueError('the rows of a state must not overlap')
         bases.append(s.data_ptr())

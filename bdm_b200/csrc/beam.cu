@@ -63,59 +63,16 @@ __device__ u64 block_max(u64 m, TopShared &sh) {
     return m;
 }
 
-// The K largest of all threads' keys key(0) .. key(E-1) (0 = none), in descending order in sh.best (0 where
-// there are fewer).  Keys are distinct.  The K-th largest of one warp's 32 thread maxima bounds the K-th
-// largest of the CTA's keys from below; the keys above the largest such bound (a few times K) go to a list
-// and are ranked there.  When the list overflows (a few threads hold most of the largest keys), K rounds of
-// a CTA-wide maximum take its place.
-template <int E, typename F> __device__ void block_topk(int K, TopShared &sh, F key) {
-    const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
-    u64 mx = 0;
-#pragma unroll
-    for (int e = 0; e < E; ++e) {
-        const u64 x = key(e);
-        mx = x > mx ? x : mx;
-    }
-    const u64 sorted = warp_sort_desc(mx);
-    const u64 kth = __shfl_sync(0xffffffffu, sorted, K - 1);
-    if (lane == 0) sh.warp[warp] = kth;
-    if (tid == 0) sh.count = 0;
-    if (tid < K) sh.best[tid] = 0;
-    __syncthreads();
-    u64 bound = 1;
-#pragma unroll
-    for (int w = 0; w < kWarps; ++w) bound = sh.warp[w] > bound ? sh.warp[w] : bound;
-    if (mx >= bound)
-#pragma unroll
-        for (int e = 0; e < E; ++e) {
-            const u64 x = key(e);
-            if (x >= bound) {
-                const int at = atomicAdd(&sh.count, 1);
-                if (at < kList) sh.list[at] = x;
-            }
-        }
-    __syncthreads();
-    const int n = sh.count;
-    if (n <= kList) {
-        for (int i = tid; i < n; i += kThreads) {
-            const u64 x = sh.list[i];
-            int rank = 0;
-            for (int j = 0; j < n && rank < K; ++j) rank += sh.list[j] > x;
-            if (rank < K) sh.best[rank] = x;
-        }
-        __syncthreads();
-        return;
-    }
+// The K largest keys by K rounds of a CTA-wide maximum, in sh.best; each(use) calls use(key) for the thread's.
+template <typename F> __device__ __forceinline__ void block_maxima(int K, TopShared &sh, F each) {
     u64 last = ~0ull;
     for (int r = 0; r < K; ++r) {
         u64 m = 0;
-#pragma unroll
-        for (int e = 0; e < E; ++e) {
-            const u64 x = key(e);
+        each([&](u64 x) {
             if (x < last && x > m) m = x;
-        }
+        });
         last = block_max(m, sh);
-        if (tid == 0) sh.best[r] = last;
+        if (threadIdx.x == 0) sh.best[r] = last;
         if (last == 0) break;
     }
     __syncthreads();
@@ -150,13 +107,27 @@ template <> __device__ __forceinline__ void unpack<bf16>(const uint4 &r, float *
     }
 }
 
-// E logits per thread.  VECTOR: rows start on 16-byte boundaries.
+__device__ __forceinline__ float exp2_ftz(float x) {
+    float y;
+    asm("ex2.approx.ftz.f32 %0, %1;\n" : "=f"(y) : "f"(x));
+    return y;
+}
+
+// One pass over the logits, E per thread in registers: the maximum, then the sum, then the few
+// candidates: the K-th largest of one warp's lane maxima bounds the K-th largest of the slice from below, and the
+// logits at or above the largest such bound (a few times K) go to a list and are ranked there; when the list
+// overflows, K rounds of a CTA-wide maximum take its place.  Bound by HBM where the batch fills the
+// GPU; what it costs beside the load is about 7 instructions per logit (exp as one multiplication and
+// ex2.approx, off by 2^-22 and by |x - max| 2^-24 for terms that are exp(x - max) small).
+// VECTOR: rows start on 16-byte boundaries.
 template <typename T, int E, bool VECTOR>
 __global__ void __launch_bounds__(kThreads)
     beam_slice_kernel(const T *__restrict__ logits, int64_t ld, int vocab, int K, int splits, Slice *__restrict__ stat,
                       u64 *__restrict__ lists) {
     __shared__ TopShared sh;
-    __shared__ float redf[kWarps];
+    __shared__ float redm[kWarps], redk[kWarps], reds[kWarps];
+    asm volatile("griddepcontrol.launch_dependents;\n" ::: "memory");
+    const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
     const int64_t row = blockIdx.x / splits;
     const int split = (int)(blockIdx.x % splits);
     const int base = split * (E * kThreads);
@@ -164,49 +135,102 @@ __global__ void __launch_bounds__(kThreads)
     constexpr int V = VECTOR ? Vec<T>::n : 1;
     float x[E];
     auto index = [&](int e) { return base + (e / V * kThreads + (int)threadIdx.x) * V + e % V; };
+    if (VECTOR && base + E * kThreads <= vocab) {
+        uint4 r[E / V];
 #pragma unroll
-    for (int e = 0; e < E; e += V) {
-        const int i = index(e);
-        if (VECTOR && i + V <= vocab) {
-            unpack<T>(*reinterpret_cast<const uint4 *>(src + i), x + e);
-        } else {
+        for (int e = 0; e < E / V; ++e) r[e] = *reinterpret_cast<const uint4 *>(src + index(e * V));
 #pragma unroll
-            for (int u = 0; u < V; ++u) x[e + u] = i + u < vocab ? Elem<T>::to_float(src[i + u]) : -INFINITY;
+        for (int e = 0; e < E / V; ++e) unpack<T>(r[e], x + e * V);
+    } else {
+#pragma unroll
+        for (int e = 0; e < E; e += V) {
+            const int i = index(e);
+            if (VECTOR && i + V <= vocab) {
+                unpack<T>(*reinterpret_cast<const uint4 *>(src + i), x + e);
+            } else {
+#pragma unroll
+                for (int u = 0; u < V; ++u) x[e + u] = i + u < vocab ? Elem<T>::to_float(src[i + u]) : -INFINITY;
+            }
         }
     }
-    // maximum; NaN and +inf make the whole row's log-probabilities NaN
-    float m = -INFINITY;
-    bool bad = false;
+    float mine = -INFINITY;
 #pragma unroll
-    for (int e = 0; e < E; ++e) {
-        m = fmaxf(m, x[e]);
-        bad |= !(x[e] < INFINITY);
+    for (int e = 0; e < E; ++e) mine = fmaxf(mine, x[e]);
+    // the warp's largest, and the K-th largest of its lanes' (equal ones leave together: the bound is lower
+    // then, which is no harm)
+    uint32_t left = mine == mine ? ordered(mine) : 0u, top = __reduce_max_sync(0xffffffffu, left), kth = top;
+    for (int k = 1; k < K; ++k) {
+        if (left == kth) left = 0;
+        kth = __reduce_max_sync(0xffffffffu, left);
     }
-#pragma unroll
-    for (int o = 16; o > 0; o >>= 1) m = fmaxf(m, __shfl_xor_sync(0xffffffffu, m, o));
-    if ((threadIdx.x & 31) == 0) redf[threadIdx.x >> 5] = m;
-    bad = __syncthreads_or(bad);
-#pragma unroll
-    for (int w = 0; w < kWarps; ++w) m = fmaxf(m, redf[w]);
-    float s = 0.f;
-    if (m > -INFINITY && !bad)
-#pragma unroll
-        for (int e = 0; e < E; ++e) s += expf(x[e] - m);
-    s = warp_sum(s);
+    if (lane == 0) {
+        redm[warp] = unordered(top ? top : ordered(-INFINITY));
+        redk[warp] = unordered(kth ? kth : ordered(-INFINITY));
+    }
+    if (threadIdx.x == 0) sh.count = 0;
+    if (threadIdx.x < K) sh.best[threadIdx.x] = 0;
     __syncthreads();
-    if ((threadIdx.x & 31) == 0) redf[threadIdx.x >> 5] = s;
+    float m = redm[0], bound = redk[0];
+#pragma unroll
+    for (int w = 1; w < kWarps; ++w) {
+        m = fmaxf(m, redm[w]);
+        bound = fmaxf(bound, redk[w]);
+    }
+    // NaN and +inf make the sum NaN, and with it the whole row's log-probabilities
+    float s0 = 0.f, s1 = 0.f;
+    if (m > -INFINITY) {
+#pragma unroll
+        for (int e = 0; e < E; e += 2) {
+            s0 += exp2_ftz((x[e] - m) * 1.4426950408889634f);
+            s1 += exp2_ftz((x[e + 1] - m) * 1.4426950408889634f);
+        }
+    } else {  // all -inf, or NaN
+#pragma unroll
+        for (int e = 0; e < E; ++e) s0 += x[e] == -INFINITY ? 0.f : NAN;
+    }
+    const float s = warp_sum(s0 + s1);
+    if (lane == 0) reds[warp] = s;
+    if (mine >= bound) {
+        uint32_t hot = 0;
+#pragma unroll
+        for (int e = 0; e < E; ++e) hot |= x[e] >= bound ? 1u << e : 0u;
+        while (hot) {  // rare: the logit is read again, as registers have no index
+            const int e = __ffs(hot) - 1, i = index(e);
+            hot &= hot - 1;
+            if (i >= vocab) continue;
+            const int at = atomicAdd(&sh.count, 1);
+            if (at < kList) sh.list[at] = make_key(Elem<T>::to_float(src[i]), (uint32_t)i);
+        }
+    }
     __syncthreads();
     if (threadIdx.x == 0) {
-        s = 0.f;
-        for (int w = 0; w < kWarps; ++w) s += redf[w];
-        stat[row * splits + split] = Slice{bad ? NAN : m, s};
+        float t = 0.f;
+#pragma unroll
+        for (int w = 0; w < kWarps; ++w) t += reds[w];
+        stat[row * splits + split] = Slice{t == t ? m : NAN, t};
     }
-    if (bad) return;  // the row has no candidate of its own: its list is not read
-    block_topk<E>(K, sh, [&](int e) {
-        const int i = index(e);
-        return i < vocab ? make_key(x[e], (uint32_t)i) : 0ull;
+    const int n = sh.count;
+    u64 *dst = lists + (row * splits + split) * K;
+    if (n <= kList) {
+        for (int i = threadIdx.x; i < n; i += kThreads) {
+            const u64 k = sh.list[i];
+            int rank = 0;
+            for (int j = 0; j < n && rank < K; ++j) rank += sh.list[j] > k;
+            if (rank < K) dst[rank] = k;
+        }
+        for (int i = n + threadIdx.x; i < K; i += kThreads) dst[i] = 0;
+        return;
+    }
+    // a few threads hold most of the largest logits: repeated maxima, over the logits read again
+    const int end = base + E * kThreads < vocab ? base + E * kThreads : vocab;
+    block_maxima(K, sh, [&](auto &&use) {
+#pragma unroll 1
+        for (int i = base + threadIdx.x; i < end; i += kThreads) {
+            const float y = Elem<T>::to_float(src[i]);
+            if (y == y) use(make_key(y, (uint32_t)i));
+        }
     });
-    if (threadIdx.x < K) lists[(row * splits + split) * K + threadIdx.x] = sh.best[threadIdx.x];
+    if (threadIdx.x < K) dst[threadIdx.x] = sh.best[threadIdx.x];
 }
 
 // ------------------------------------------------------------------- merging
@@ -242,114 +266,121 @@ __global__ void __launch_bounds__(kThreads)
                       uint8_t *__restrict__ out_finished) {
     __shared__ TopShared sh;
     __shared__ Row rows[kMaxBeams];
+    __shared__ u64 lead[kMaxBeams][kMaxBeams];  // each row's K best candidates, in order
     __shared__ u64 kept[kMaxBeams];
-    __shared__ int reach[kMaxBeams];
+    asm volatile("griddepcontrol.wait;\n" ::: "memory");  // the slices, as this launch may have begun before they ended
     const int64_t b = blockIdx.x;
-    const int K = beams, tid = threadIdx.x;
-    if (tid < beams) {
-        const int64_t row = b * beams + tid;
+    const int K = beams, tid = threadIdx.x, lane = tid & 31, per = splits * K;
+    const unsigned all = 0xffffffffu;
+    for (int w = tid >> 5; w < beams; w += kWarps) {  // a warp for each row
+        const int64_t row = b * beams + w;
+        const u64 *list = lists + row * per;
+        u64 x = lane < per ? list[lane] : 0ull;  // on its way while the sums are joined
         Row r;
         r.score = scores[row];
+        const bool done = finished && finished[row];
         float m = -INFINITY, s = 0.f;
         bool bad = false;
-        for (int i = 0; i < splits; ++i) {
+        for (int i = lane; i < splits; i += 32) {
             const Slice t = stat[row * splits + i];
             bad |= t.max != t.max;
-            m = fmaxf(m, t.max);
+            const float n = fmaxf(m, t.max);
+            if (t.max > -INFINITY) s = s * (m > -INFINITY ? expf(m - n) : 0.f) + t.sum * expf(t.max - n);
+            m = n;
         }
-        for (int i = 0; i < splits; ++i) {
-            const Slice t = stat[row * splits + i];
-            if (t.max > -INFINITY) s += t.sum * expf(t.max - m);
-        }
-        r.max = m;
+        bad = __any_sync(all, bad);
+        float top = m;
+#pragma unroll
+        for (int o = 16; o > 0; o >>= 1) top = fmaxf(top, __shfl_xor_sync(all, top, o));
+        s = warp_sum(m > -INFINITY ? s * expf(m - top) : 0.f);
+        r.max = top;
         r.logsum = logf(s);
-        r.kind = bad || m == -INFINITY || r.score != r.score || r.score == -INFINITY;
-        if (finished && finished[row]) r.kind = 2;
-        rows[tid] = r;
-        kept[tid] = 0;
+        r.kind = bad || top == -INFINITY || r.score != r.score || r.score == -INFINITY;
+        if (done) r.kind = 2;
+        const uint32_t flat = (uint32_t)w * (uint32_t)vocab;
+        u64 best;
+        if (r.kind == 0) {
+            auto cand = [&](u64 y) { return y ? make_key(candidate(r, key_value(y)), flat + key_index(y)) : 0ull; };
+            best = warp_sort_desc(cand(x));
+            for (int i0 = 32; i0 < per; i0 += 32) {
+                x = i0 + lane < per ? list[i0 + lane] : 0ull;
+                const u64 y = __shfl_sync(all, warp_sort_desc(cand(x)), 31 - lane);
+                best = warp_sort_desc(best > y ? best : y);
+            }
+        } else if (r.kind == 1) {  // every candidate is -inf: the lowest tokens
+            best = lane < vocab ? make_key(-INFINITY, flat + lane) : 0ull;
+        } else {  // finished: the end token keeps the score, then the lowest other tokens
+            const int t = lane - 1 < (int)eos ? lane - 1 : lane;
+            best = lane == 0 ? make_key(r.score == r.score ? r.score : -INFINITY, flat + (uint32_t)eos)
+                             : (t < vocab ? make_key(-INFINITY, flat + t) : 0ull);
+            best = warp_sort_desc(best);  // a score of -inf ties with them
+        }
+        if (lane < K) lead[w][lane] = best;
+        if (lane == 0) rows[w] = r;
+    }
+    if (tid < K) kept[tid] = 0;
+    __syncthreads();
+    // a candidate's rank: the larger ones of every row, counted until it falls out
+    for (int i = tid; i < beams * K; i += kThreads) {
+        const int w = i / K, j = i % K;
+        const u64 x = lead[w][j];
+        int rank = x ? j : K;
+        for (int v = 0; v < beams && rank < K; ++v)
+            if (v != w)
+                for (int q = 0; q < K && rank < K && lead[v][q] > x; ++q) ++rank;
+        if (rank < K) kept[rank] = x;
     }
     __syncthreads();
-    // rows 0 .. beams-1, per row splits * K listed keys (K made-up ones for kinds 1 and 2)
-    const int per = splits * K, total = beams * per;
-    constexpr int E = 8;
-    u64 limit[E];
-    auto entry = [&](int i) -> u64 {
-        const int w = i / per, j = i % per;
-        const Row r = rows[w];
-        const uint32_t flat = (uint32_t)w * (uint32_t)vocab;
-        if (r.kind == 0) {
-            const u64 x = lists[(b * beams + w) * per + j];
-            return x ? make_key(candidate(r, key_value(x)), flat + key_index(x)) : 0ull;
-        }
-        if (j >= K) return 0ull;
-        if (r.kind == 1) return j < vocab ? make_key(-INFINITY, flat + j) : 0ull;
-        // finished: the end token keeps the score, then the lowest other tokens
-        if (j == 0) return make_key(r.score == r.score ? r.score : -INFINITY, flat + (uint32_t)eos);
-        const int t = j - 1 < (int)eos ? j - 1 : j;
-        return t < vocab ? make_key(-INFINITY, flat + t) : 0ull;
-    };
-    auto select = [&]() {
-        if (tid < beams) kept[tid] = 0;
-        for (int i0 = 0; i0 < total; i0 += kThreads * (E - 1)) {
-#pragma unroll
-            for (int e = 0; e < E - 1; ++e) {
-                const int i = i0 + e * kThreads + tid;
-                limit[e] = i < total ? entry(i) : 0ull;
-            }
-            __syncthreads();
-            limit[E - 1] = tid < K ? kept[tid] : 0ull;
-            block_topk<E>(K, sh, [&](int e) { return limit[e]; });
-            if (tid < K) kept[tid] = sh.best[tid];
-            __syncthreads();
-        }
-    };
-    select();
     // Rounding may give unlisted logits (below the row's list) the value of a listed one and a lower index.
-    // That can matter only where the type's next value below the list's last logit already rounds to the same
-    // candidate, and that candidate reaches the selection: such a row is read again, by candidate.
-    // (the row then has K listed candidates at or above the last kept value)
-    if (tid < beams) reach[tid] = 0;
-    __syncthreads();
+    // That can matter only where the row's last listed candidate reaches the selection and the type's next
+    // value below its logit already rounds to the same candidate: such a row is read again, by candidate.
     const uint32_t kth = (uint32_t)(kept[K - 1] >> 32);
-    for (int i = tid; i < total; i += kThreads)
-        if (rows[i / per].kind == 0 && (uint32_t)(entry(i) >> 32) >= kth) atomicAdd(&reach[i / per], 1);
-    __syncthreads();
-    for (int w = 0; w < beams; ++w) {
-        const Row r = rows[w];
-        if (reach[w] < K || vocab <= K) continue;
-        u64 lowest = ~0ull;  // the row's K-th largest logit
-        for (int k = 0; k < K; ++k) {
-            u64 m = 0;
-            for (int j = tid; j < per; j += kThreads) {
-                const u64 x = lists[(b * beams + w) * per + j];
-                if (x < lowest && x > m) m = x;
+    const bool reach = tid < beams && vocab > K && rows[tid].kind == 0 && (uint32_t)(lead[tid][K - 1] >> 32) >= kth;
+    if (__syncthreads_or(reach)) {
+        for (int w = 0; w < beams; ++w) {
+            const Row r = rows[w];
+            if (r.kind != 0 || vocab <= K || (uint32_t)(lead[w][K - 1] >> 32) < kth) continue;
+            u64 lowest = ~0ull;  // the row's K-th largest logit
+            for (int k = 0; k < K; ++k) {
+                u64 m = 0;
+                for (int j = tid; j < per; j += kThreads) {
+                    const u64 x = lists[(b * beams + w) * per + j];
+                    if (x < lowest && x > m) m = x;
+                }
+                lowest = block_max(m, sh);
             }
-            lowest = block_max(m, sh);
-        }
-        const float x = key_value(lowest);
-        if (!(x > -INFINITY)) continue;
-        const float c = candidate(r, x);
-        if (candidate(r, next_below<T>(x)) != c) continue;
-        // the row's K best by candidate, merged with the other rows' candidates kept so far
-        const uint32_t flat = (uint32_t)w * (uint32_t)vocab;
-        u64 last = ~0ull;
-        u64 mine = 0;  // thread k < K: the row's k-th
-        for (int k = 0; k < K; ++k) {
-            u64 m = 0;
-            for (int i = tid; i < vocab; i += kThreads) {
-                const u64 y = make_key(candidate(r, Elem<T>::to_float(logits[(b * beams + w) * ld + i])),
-                                       flat + i);
-                if (y < last && y > m) m = y;
+            const float x = key_value(lowest);
+            if (!(x > -INFINITY) || candidate(r, next_below<T>(x)) != candidate(r, x)) continue;
+            // the row's K best by candidate, merged with the other rows' candidates kept so far
+            const uint32_t flat = (uint32_t)w * (uint32_t)vocab;
+            u64 last = ~0ull;
+            u64 mine = 0;  // thread k < K: the row's k-th
+            for (int k = 0; k < K; ++k) {
+                u64 m = 0;
+                for (int i = tid; i < vocab; i += kThreads) {
+                    const u64 y = make_key(candidate(r, Elem<T>::to_float(logits[(b * beams + w) * ld + i])), flat + i);
+                    if (y < last && y > m) m = y;
+                }
+                last = block_max(m, sh);
+                if (tid == k) mine = last;
             }
-            last = block_max(m, sh);
-            if (tid == k) mine = last;
+            u64 other = tid < K ? kept[tid] : 0ull;
+            if (other && key_index(other) / (uint32_t)vocab == (uint32_t)w) other = 0;  // its own are in `mine`
+            __syncthreads();
+            // 2 K distinct keys at most, in the first threads
+            if (tid < K) {
+                sh.list[tid] = mine;
+                sh.list[K + tid] = other;
+                kept[tid] = 0;
+            }
+            __syncthreads();
+            if (tid < 2 * K && sh.list[tid]) {
+                int rank = 0;
+                for (int j = 0; j < 2 * K; ++j) rank += sh.list[j] > sh.list[tid];
+                if (rank < K) kept[rank] = sh.list[tid];
+            }
+            __syncthreads();
         }
-        u64 other = tid < K ? kept[tid] : 0ull;
-        if (other && key_index(other) / (uint32_t)vocab == (uint32_t)w) other = 0;  // its own are in `mine`
-        __syncthreads();
-        block_topk<2>(K, sh, [&](int e) { return e ? mine : other; });
-        if (tid < K) kept[tid] = sh.best[tid];
-        __syncthreads();
     }
     if (tid < 32) {
         const bool on = tid < K;
@@ -360,7 +391,6 @@ __global__ void __launch_bounds__(kThreads)
         int slot = tid;
         if (stable) {
             // the first child of a parent takes its slot, the others the free slots in turn
-            const unsigned all = 0xffffffffu;
             const unsigned same = __match_any_sync(all, parent);
             const bool first = (same & ((1u << tid) - 1)) == 0;
             unsigned taken = on ? 1u << parent : 0u;
@@ -474,9 +504,9 @@ int reorder_launch(Tensors t, const int64_t *row_bytes, const int64_t *parents, 
         reorder_rows_kernel<U, 4><<<(unsigned)tiles, kThreads, 0, st>>>(t, parents, beams, groups, status);
     else if (beams <= 8)
         reorder_rows_kernel<U, 8><<<(unsigned)tiles, kThreads, 0, st>>>(t, parents, beams, groups, status);
-    else if (beams <= 16)
+    else if (beams <= 16 || sizeof(U) == 16)  // 16-byte columns of 32 rows would not fit the registers
         reorder_rows_kernel<U, 16><<<(unsigned)tiles, kThreads, 0, st>>>(t, parents, beams, groups, status);
-    else
+    else if constexpr (sizeof(U) < 16)
         reorder_rows_kernel<U, 32><<<(unsigned)tiles, kThreads, 0, st>>>(t, parents, beams, groups, status);
     return launch_status();
 }
@@ -525,9 +555,20 @@ extern "C" int bdm_beam_select(const void *logits, int64_t ld, int64_t batch, in
                 beam_slice_kernel<T, 8, false><<<grid, kThreads, 0, st>>>(x, ld, (int)vocab, beams, p.splits, stat, lists);
         }
         if (int rc = launch_status()) return rc;
-        beam_merge_kernel<T><<<(unsigned)batch, kThreads, 0, st>>>(x, ld, scores, finished, eos_token, beams, (int)vocab,
-                                                                  p.splits, stable_slots, stat, lists, out_scores,
-                                                                  out_parents, out_tokens, out_finished);
+        // a programmatic dependent launch: its start overlaps the slices' end
+        cudaLaunchConfig_t cfg{};
+        cfg.gridDim = dim3((unsigned)batch);
+        cfg.blockDim = dim3(kThreads);
+        cfg.stream = st;
+        cudaLaunchAttribute attr{};
+        attr.id = cudaLaunchAttributeProgrammaticStreamSerialization;
+        attr.val.programmaticStreamSerializationAllowed = 1;
+        cfg.attrs = &attr;
+        cfg.numAttrs = 1;
+        if (int rc = cuda_status(cudaLaunchKernelEx(&cfg, beam_merge_kernel<T>, x, ld, scores, finished, eos_token, beams,
+                                                    (int)vocab, p.splits, stable_slots, (const Slice *)stat,
+                                                    (const u64 *)lists, out_scores, out_parents, out_tokens, out_finished)))
+            return rc;
     });
     return launch_status();
 }
@@ -542,12 +583,13 @@ extern "C" int bdm_reorder_rows(void *const *bases, const int64_t *row_strides, 
     for (int i = 0; i < count; ++i)
         if (row_bytes[i] < 0 || row_strides[i] < row_bytes[i] || (row_bytes[i] && !bases[i])) return BDM_ERR_INVALID;
     cudaStream_t st = as_stream(stream);
-    for (int width : {16, 4, 1}) {  // the widest access each tensor's rows allow
+    for (int width : {16, 8, 4, 1}) {  // the widest access each tensor's rows allow, 8 bytes at most past 16 beams
         Tensors t{};
         int64_t bytes[kMaxTensors];
         auto flush = [&]() {
             const int rc = t.count == 0 ? BDM_OK
                            : width == 16 ? reorder_launch<uint4>(t, bytes, parents, groups, beams, status, st)
+                           : width == 8  ? reorder_launch<uint2>(t, bytes, parents, groups, beams, status, st)
                            : width == 4  ? reorder_launch<uint32_t>(t, bytes, parents, groups, beams, status, st)
                                          : reorder_launch<uint8_t>(t, bytes, parents, groups, beams, status, st);
             t.count = 0;
@@ -555,7 +597,7 @@ extern "C" int bdm_reorder_rows(void *const *bases, const int64_t *row_strides, 
         };
         for (int i = 0; i < count; ++i) {
             const uint64_t bits = reinterpret_cast<uintptr_t>(bases[i]) | (uint64_t)row_strides[i] | (uint64_t)row_bytes[i];
-            const int fits = bits % 16 == 0 ? 16 : (bits % 4 == 0 ? 4 : 1);
+            const int fits = bits % 16 == 0 && beams <= 16 ? 16 : (bits % 8 == 0 ? 8 : (bits % 4 == 0 ? 4 : 1));
             if (fits != width || row_bytes[i] == 0) continue;
             t.base[t.count] = bases[i];
             t.stride[t.count] = row_strides[i];
