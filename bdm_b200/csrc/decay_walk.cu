@@ -273,7 +273,12 @@ int64_t simt_segments(int64_t ctas, int64_t chunks, int sms) {
     return s < 1 ? 1 : s;
 }
 
-int plan(const bdm_decay_walk_args &w, Params &p, bool &tc, int sms) {
+struct Split {
+    bool tc;        // the tensor-core walk takes it
+    int sub, scps;  // its state launch's sub-segments and their chunks
+};
+
+int plan(const bdm_decay_walk_args &w, Params &p, Split &split, int sms) {
     p.a = w.a, p.b = w.b, p.c = w.c, p.out = w.out;
     for (int i = 0; i < 3; ++i) {
         p.as[i] = w.a_stride[i];
@@ -293,11 +298,14 @@ int plan(const bdm_decay_walk_args &w, Params &p, bool &tc, int sms) {
     p.status = w.status;
     p.seg = nullptr;
     const int64_t chunks = ceil_div(w.time, kChunk) > 0 ? ceil_div(w.time, kChunk) : 1;
-    tc = decay_walk_tc_takes(w);
-    const int64_t nseg = tc ? decay_walk_tc_segments(w.batch * w.heads, chunks, sms)
-                            : simt_segments(w.batch * w.heads * ceil_div(w.width_c, kCols), chunks, sms);
-    p.cps = (int)ceil_div(chunks, nseg);
-    p.nseg = (int)ceil_div(chunks, p.cps);
+    split = Split{decay_walk_tc_takes(w), 1, 1};
+    if (split.tc) {
+        decay_walk_tc_split(w.batch * w.heads, chunks, sms, p.nseg, p.cps, split.sub, split.scps);
+    } else {
+        const int64_t nseg = simt_segments(w.batch * w.heads * ceil_div(w.width_c, kCols), chunks, sms);
+        p.cps = (int)ceil_div(chunks, nseg);
+        p.nseg = (int)ceil_div(chunks, p.cps);
+    }
     return BDM_OK;
 }
 
@@ -313,7 +321,8 @@ int check_args(const bdm_decay_walk_args &w) {
     return BDM_OK;
 }
 
-int64_t seg_bytes(const Params &p) {
+int64_t seg_bytes(const Params &p, const Split &split) {
+    if (split.tc) return decay_walk_tc_bytes(p, split.sub);
     return p.nseg > 1 ? p.batch * p.heads * p.nseg * (int64_t)p.wab * p.wc * 4 : 0;
 }
 
@@ -327,9 +336,9 @@ extern "C" int64_t bdm_decay_walk_workspace_bytes(const bdm_decay_walk_args *w) 
     int sms = 0;
     if (device_setup(sms)) return -1;
     Params p{};
-    bool tc = false;
-    if (plan(*w, p, tc, sms)) return -1;
-    return seg_bytes(p);
+    Split split{};
+    if (plan(*w, p, split, sms)) return -1;
+    return seg_bytes(p, split);
 }
 
 extern "C" int bdm_decay_walk(const bdm_decay_walk_args *w, void *workspace, int64_t workspace_bytes, void *stream) {
@@ -341,17 +350,16 @@ extern "C" int bdm_decay_walk(const bdm_decay_walk_args *w, void *workspace, int
     int sms = 0;
     if (int rc = device_setup(sms)) return rc;
     Params p{};
-    bool tc = false;
-    if (int rc = plan(*w, p, tc, sms)) return rc;
-    const int64_t need = seg_bytes(p);
+    Split split{};
+    if (int rc = plan(*w, p, split, sms)) return rc;
+    const int64_t need = seg_bytes(p, split);
     if (need > workspace_bytes || (need && !workspace)) return BDM_ERR_WORKSPACE;
     p.seg = static_cast<float *>(workspace);
     cudaStream_t st = as_stream(stream);
+    if (split.tc) return decay_walk_tc_launch(*w, p, split.sub, split.scps, workspace, st);
     for (int pass = p.nseg > 1 ? 0 : 1; pass < 2; ++pass) {
         int rc;
-        if (tc)
-            rc = decay_walk_tc_launch(*w, p, pass == 0, st);
-        else if (w->dtype == BDM_F32)
+        if (w->dtype == BDM_F32)
             rc = simt_launch<float, float>(p, pass == 0, st);
         else if (w->out_dtype == BDM_F32)
             rc = simt_launch<bf16, float>(p, pass == 0, st);

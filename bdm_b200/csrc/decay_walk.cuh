@@ -105,7 +105,8 @@ __device__ __forceinline__ float start_state(const Params &p, const Span &s, int
 
 // The tensor-core walk (decay_walk_tc.cu): BF16 operands that TMA can address.
 bool decay_walk_tc_takes(const bdm_decay_walk_args &w);
-int64_t decay_walk_tc_segments(int64_t rows, int64_t chunks, int sms);
-int decay_walk_tc_launch(const bdm_decay_walk_args &w, const walk::Params &p, bool state_only, cudaStream_t st);
+void decay_walk_tc_split(int64_t rows, int64_t chunks, int sms, int &nseg, int &cps, int &sub, int &scps);
+int64_t decay_walk_tc_bytes(const walk::Params &p, int sub);
+int decay_walk_tc_launch(const bdm_decay_walk_args &w, walk::Params p, int sub, int scps, void *workspace, cudaStream_t st);
 
 }  // namespace bdm
