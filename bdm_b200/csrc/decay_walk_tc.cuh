@@ -14,14 +14,14 @@
 // returned: T, and with it the state over any number of chunks, is then exact to FP32.  Where none is, two
 // terms (an error of 2^-17 beside the outputs' 2^-9) are enough.
 //
-// Roles (20 warps): 0-7 carry the state (a quadrant's value columns, half of the key columns), 8-11 scale V',
-// 12-15 the outputs, 16-17 P, 18 TMA, 19 MMA.  V' is made and T issued in two halves of 32 tokens, so that the
+// Roles (22 warps of 24): 0-7 carry the state (a quadrant's value columns, half of the key columns), 8-11 scale V',
+// 12-15 the outputs, 16-19 P, 20 MMA, 21 TMA.  V' is made and T issued in two halves of 32 tokens, so that the
 // scaling of one overlaps the product of the other.  V' is in tensor memory because shared memory's bandwidth
 // is what the products and copies share: as a shared-memory operand it took 768 more of its cycles per chunk.
 // The roles' loops are kept short on purpose: five roles' unrolled code does not fit the instruction cache
 // (measured: 100 us unrolled, 78 us rolled, for the same work).
-// Value widths up to 64 use M = 64 products, whose 64 rows are 16 lanes of each quadrant, so that all four
-// schedulers share the work; wider ones use all 128 lanes.
+// The scores, and value widths up to 64, use M = 64 products, whose 64 rows are 16 lanes of each quadrant, so
+// that all four schedulers share the work; wider values use all 128 lanes.
 // Every wait is bounded; one that gives up sets the status word and lets the CTA drain.
 #pragma once
 
@@ -35,9 +35,13 @@
 namespace bdm {
 namespace walk {
 
-constexpr int kTcThreads = 640;
+constexpr int kTcThreads = 768;
+// Registers: 6 groups of 4 warps, 80 per thread at launch (480 in all), dealt out as 2 x 112 (state) + 72 (V') + 80
+// (outputs) + 64 (P) + 40 (loads and products).
+constexpr int kStateRegs = 112, kScaleRegs = 72, kOutRegs = 80, kScoreRegs = 64, kMmaRegs = 40;
+static_assert(2 * kStateRegs + kScaleRegs + kOutRegs + kScoreRegs + kMmaRegs <= 6 * 80, "register shares");
 constexpr int kBox = 64 * 128;  // bytes of a TMA box: 64 tokens x 64 BF16 columns
-constexpr int kStateWarps = 8, kScaleWarp = 8, kOutWarp = 12, kScoreWarp = 16, kTmaWarp = 18, kMmaWarp = 19;
+constexpr int kStateWarps = 8, kScaleWarp = 8, kOutWarp = 12, kScoreWarp = 16, kMmaWarp = 20, kTmaWarp = 21;
 constexpr int kMaxStages = 8;
 constexpr int kSmemMax = 227 * 1024;
 constexpr long long kWaitCycles = 4000000000ll;  // about 2 s
@@ -56,9 +60,11 @@ struct TcParams {
     float *z;              // its states, [batch*heads, (nseg - 1) * sub, wc, wab]
 };
 
+// A parity tells a phase from the next only, so no waiter may fall two phases behind: each barrier's next phase
+// needs something that its waiter gives after the wait (P's two buffers have one barrier each for that reason).
 struct Bars {
     uint64_t full[kMaxStages], empty[kMaxStages];
-    uint64_t vready[2], tpart[2], tfree, sready, adone, pready, odone, ofree, zeroed, ofull, oempty;
+    uint64_t vready[2], tpart[2], pfree[2], tlast, tfree, sready, adone, pready, odone, ofree, zeroed, ofull, oempty;
 };
 
 __device__ __forceinline__ uint32_t pack_bf16(float lo, float hi) {
@@ -109,7 +115,7 @@ template <int N> __device__ __forceinline__ void terms(F2 x, uint32_t &hi, uint3
     }
 }
 
-static __device__ __noinline__ bool wait_slow(uint64_t *m, unsigned parity, volatile int *dead) {
+__device__ __forceinline__ bool wait_slow(uint64_t *m, unsigned parity, volatile int *dead) {
     const long long t0 = clock64();
     for (int i = 0; i < (1 << 28); ++i) {
         if (tc::mbar_test_for(m, parity, 1000)) return true;
@@ -120,10 +126,10 @@ static __device__ __noinline__ bool wait_slow(uint64_t *m, unsigned parity, vola
 }
 
 
-// Stages of the load pipeline: what shared memory holds beside P and two buffers of outputs.
+// Stages of the load pipeline: what shared memory holds beside two buffers of P and of outputs.
 template <int DKB, int VB, bool STATE_ONLY> constexpr int stages_of() {
     const int stage = (STATE_ONLY ? DKB + VB : 2 * DKB + VB) * kBox;
-    const int n = (kSmemMax - 1024 - 3072 - (1 + 2 * VB) * kBox) / stage;
+    const int n = (kSmemMax - 1024 - 3072 - 2 * (1 + VB) * kBox) / stage;
     return n > kMaxStages ? kMaxStages : n;
 }
 
@@ -186,11 +192,13 @@ __global__ void __launch_bounds__(kTcThreads, 1) decay_walk_tc_kernel(const TcPa
         for (int i = 0; i < 2; ++i) {
             tc::mbar_init(&bar.vready[i], 4);
             tc::mbar_init(&bar.tpart[i], 1);
+            tc::mbar_init(&bar.pfree[i], 1);
         }
+        tc::mbar_init(&bar.tlast, 1);
         tc::mbar_init(&bar.tfree, kStateWarps);
         tc::mbar_init(&bar.sready, kStateWarps);
         tc::mbar_init(&bar.adone, 1);
-        tc::mbar_init(&bar.pready, 2);
+        tc::mbar_init(&bar.pready, 4);
         tc::mbar_init(&bar.odone, 1);
         tc::mbar_init(&bar.ofree, 4);
         tc::mbar_init(&bar.zeroed, 4);
@@ -224,6 +232,7 @@ __global__ void __launch_bounds__(kTcThreads, 1) decay_walk_tc_kernel(const TcPa
     constexpr int kQuadCols = 16 * kHalves;  // value columns of a quadrant
 
     if (warp < kStateWarps) {
+        tc::regs_up<kStateRegs>();
         // ------------------------------------------------------------------ state
         // Fragments: S[d][4 b + 2 r + e] is key column k0 + 8 b + 2 (lane % 4) + e of value column
         // quad * kQuadCols + 16 d + 8 r + lane / 4.
@@ -266,9 +275,9 @@ __global__ void __launch_bounds__(kTcThreads, 1) decay_walk_tc_kernel(const TcPa
         bool ok = true;
         for (int n = 0; n <= steps; ++n) {
             if (n > 0) {
-                ok = wait_warp(&bar.tpart[1], (n - 1) & 1);
-                if (!ok) break;
                 if (STATE_ONLY && n < steps) continue;  // T gathers all chunks in tensor memory
+                ok = STATE_ONLY ? wait_warp(&bar.tlast, 0) : wait_warp(&bar.tpart[1], (n - 1) & 1);
+                if (!ok) break;
                 tc::fence_after_sync();
                 const float f = STATE_ONLY ? 0.f : pw[valid_of(n - 1)];
                 const F2 carry = make2(f, f);
@@ -315,6 +324,7 @@ __global__ void __launch_bounds__(kTcThreads, 1) decay_walk_tc_kernel(const TcPa
                 }
         }
     } else if (warp < kOutWarp) {
+        tc::regs_down<kScaleRegs>();
         // --------------------------------------------------------------------- V'
         // this lane's row of the matrices it loads: two of 8 tokens by two of 8 columns
         const int mrow = ((lane >> 4) * 8 + (lane & 7)) * 128, mcol = (lane >> 3) & 1;
@@ -357,7 +367,7 @@ __global__ void __launch_bounds__(kTcThreads, 1) decay_walk_tc_kernel(const TcPa
             const float *w = vw + (p.reverse ? 0 : kChunk - valid) + hb * 32 + 2 * (lane & 3);
             const char *src = smem + st * kStage + kOffC + (VB == 2 ? (quad >> 1) * kBox : 0) + hb * 32 * 128 + mrow;
             const int c0 = VB == 2 ? (quad & 1) * 4 : quad * 2;
-#pragma unroll 1
+#pragma unroll (VB == 1 ? 2 : 1)
             for (int q = 0; q < 2; ++q, src += 16 * 128, w += 16) {
                 const F2 w0 = make2(w[0] * far, w[1] * far), w1 = make2(w[8] * far, w[9] * far);
                 uint32_t r[kHalves][4];
@@ -389,7 +399,7 @@ __global__ void __launch_bounds__(kTcThreads, 1) decay_walk_tc_kernel(const TcPa
             const int c0 = VB == 2 ? (quad & 1) * 4 : quad * 2;
             for (int n = 0; n < steps; ++n) {
                 const int t0 = start_of(n), valid = valid_of(n);
-                char *stage = sP + (1 + (n & 1) * VB) * kBox;  // BF16 outputs on their way, [token][column]: the map's boxes
+                char *stage = sP + (2 + (n & 1) * VB) * kBox;  // BF16 outputs on their way, [token][column]: the map's boxes
                 if (kTma && n > 1) {
                     if (warp == kOutWarp && lane == 0) {
                         tc::tma_store_wait_read<1>();
@@ -470,79 +480,59 @@ __global__ void __launch_bounds__(kTcThreads, 1) decay_walk_tc_kernel(const TcPa
             if (col < p.wc)
                 for (int64_t t = z0; t < z1; ++t) out[t * p.os[1] + col] = Elem<OT>::from_float(0.f);
         }
-    } else if (warp < kTmaWarp) {
-        // ------------------------------------------------ decayed scores P (rows 0..63)
+    } else if (warp < kMmaWarp) {
+        tc::regs_down<kScoreRegs>();
+        // ------------------------------------------------------------ decayed scores P
         if constexpr (!STATE_ONLY) {
-            const int row = quad * 32 + lane;
-            const float *w0 = wt + kChunk + (p.reverse ? -row : row);
+            // fragments: rows quad * 16 + lane / 4 (+ 8), columns 8 b + 2 (lane % 4) + {0, 1}
+            const int row = quad * 16 + (lane >> 2), col = 2 * (lane & 3), step = p.reverse ? 1 : -1;
+            const float *w0 = wt + kChunk + (p.reverse ? col - row : row - col);
+            const int srow = quad * 16 + (lane & 15), scol = lane >> 4;  // stmatrix: this lane's row and block of 8 columns
             for (int n = 0; n < steps; ++n) {
                 const int valid = valid_of(n);
                 if (!wait_warp(&bar.adone, n & 1)) break;
                 tc::fence_after_sync();
-                if (n > 0 && !wait_warp(&bar.odone, (n - 1) & 1)) break;  // the last chunk's reads of P are over
-                const float *w = w0;
-                const int step = p.reverse ? 1 : -1;
+                if (n > 1 && !wait_warp(&bar.pfree[n & 1], ((n >> 1) - 1) & 1)) break;  // this buffer's last reads are over
+                char *dst = sP + (n & 1) * kBox + srow * 128;
 #pragma unroll 1
-                for (int i = 0; i < 64; i += 16) {
+                for (int i = 0; i < 64; i += 32) {
                     float x[16];
-                    tc::tmem_ld16(tmem + lanes + kColA + i, x);
+                    tc::tmem_ld_16x256b_x4(tmem + lanes + kColA + i, x);
+                    F2 w[8];
+#pragma unroll
+                    for (int e = 0; e < 8; ++e) {
+                        const float *f = w0 + step * (i + e / 2 * 8 - (e & 1) * 8);  // row + 8 is 8 columns back
+                        w[e] = make2(f[0], f[step]);
+                    }
                     tc::tmem_wait_ld();
                     uint32_t r[8];
 #pragma unroll
-                    for (int e = 0; e < 8; ++e, w += 2 * step) r[e] = pack2(mul2(make2(w[0], w[step]), make2(x[2 * e], x[2 * e + 1])));
+                    for (int e = 0; e < 8; ++e) r[e] = pack2(mul2(w[e], make2(x[2 * e], x[2 * e + 1])));
                     if (valid < kChunk)  // scores of tokens past the row's length may be anything
 #pragma unroll
-                        for (int e = 0; e < 8; ++e)
-                            r[e] &= (i + 2 * e < valid ? 0xffffu : 0u) | (i + 2 * e + 1 < valid ? 0xffff0000u : 0u);
+                        for (int e = 0; e < 8; ++e) {
+                            const int j = i + e / 2 * 8 + col;
+                            r[e] &= (j < valid ? 0xffffu : 0u) | (j + 1 < valid ? 0xffff0000u : 0u);
+                        }
 #pragma unroll
-                    for (int c = 0; c < 2; ++c)
-                        *reinterpret_cast<uint4 *>(sP + row * 128 + (((i / 8 + c) ^ (row & 7)) << 4)) =
-                            make_uint4(r[4 * c], r[4 * c + 1], r[4 * c + 2], r[4 * c + 3]);
+                    for (int e = 0; e < 8; e += 4)
+                        tc::stmatrix_x4(dst + (((i / 8 + e / 2 + scol) ^ (srow & 7)) << 4), r[e], r[e + 1], r[e + 2], r[e + 3]);
                 }
                 tc::fence_async_smem();
                 arrive(&bar.pready);
             }
         }
-    } else if (warp == kTmaWarp) {
-        // ------------------------------------------------------------------ loads
-        if (tc::elect_one()) {
-            int issued = 0, st = 0, phase = 0;
-            for (int n = 0; n < steps; ++n) {
-                if (n >= stages && !wait(&bar.empty[st], phase ^ 1)) break;
-                char *dst = smem + st * kStage;
-                const int t0 = start_of(n);
-                tc::mbar_arrive_expect_tx(&bar.full[st], kStage);
-                if (!STATE_ONLY)
-#pragma unroll
-                    for (int i = 0; i < DKB; ++i)
-                        tc::tma_load_4d(dst + i * kBox, &maps.a, i * 64, t0, (h / p.ag) * tp.bmul[0], (int)b * tp.amul[0],
-                                        &bar.full[st]);
-#pragma unroll
-                for (int i = 0; i < DKB; ++i)
-                    tc::tma_load_4d(dst + kOffB + i * kBox, &maps.b, i * 64, t0, (h / p.bg) * tp.bmul[1],
-                                    (int)b * tp.amul[1], &bar.full[st]);
-#pragma unroll
-                for (int i = 0; i < VB; ++i)
-                    tc::tma_load_4d(dst + kOffC + i * kBox, &maps.c, i * 64, t0, (h / p.cg) * tp.bmul[2],
-                                    (int)b * tp.amul[2], &bar.full[st]);
-                issued = n + 1;
-                if (++st == stages) st = 0, phase ^= 1;
-            }
-            // no copy may be in flight when the CTA ends, whatever happened to its consumers
-            for (int n = issued > stages ? issued - stages : 0; n < issued; ++n)
-                tc::mbar_wait(&bar.full[n % stages], (n / stages) & 1, kWaitNs);
-        }
     } else {
         // --------------------------------------------------------------- products
-        if (tc::elect_one()) {
-            constexpr uint32_t idQK = tc::idesc_bf16(128, 64);
+        tc::regs_down<kMmaRegs>();
+        if (warp == kMmaWarp && tc::elect_one()) {
+            constexpr uint32_t idQK = tc::idesc_bf16(64, 64);
             constexpr uint32_t idO1 = tc::idesc_bf16(M, 64) | tc::kIdescMnA;
             constexpr uint32_t idO2 = tc::idesc_bf16(M, 64);
             constexpr uint32_t idT = tc::idesc_bf16(M, DK) | tc::kIdescMnB;
             // descriptors of the buffers' starts; an offset adds its bytes / 16 to the low word
             const uint32_t base = tc::smem_u32(smem);
             const uint64_t dP = tc::smem_desc_sw128(tc::smem_u32(sP));
-            // rows 64..127 of the scores are whatever follows the tile
             auto scores = [&](int st) {
                 uint64_t qa = tc::smem_desc_sw128(base + st * kStage), kb = qa + kOffB / 16;
 #pragma unroll 1
@@ -575,7 +565,15 @@ __global__ void __launch_bounds__(kTcThreads, 1) decay_walk_tc_kernel(const TcPa
                     tc::mma_commit(&bar.tpart[hb]);
                 }
                 if (!ok) break;
+                const int st1 = st + 1 == stages ? 0 : st + 1, phase1 = st + 1 == stages ? phase ^ 1 : phase;
                 if (!STATE_ONLY) {
+                    // P(n) is ready, so A is free: the next scores go first, P(n + 1) is what takes longest
+                    if (!(ok = wait(&bar.pready, n & 1))) break;
+                    tc::fence_after_sync();
+                    if (n + 1 < steps) {
+                        if (!(ok = wait(&bar.full[st1], phase1))) break;
+                        scores(st1);
+                    }
                     if (!(ok = wait(&bar.sready, n & 1))) break;
                     if (n > 0 && !(ok = wait(&bar.ofree, (n - 1) & 1))) break;
                     tc::fence_after_sync();
@@ -585,23 +583,42 @@ __global__ void __launch_bounds__(kTcThreads, 1) decay_walk_tc_kernel(const TcPa
                     for (int i = 0; i < DKB; ++i, qa += kBox / 16, sa += 32)
 #pragma unroll
                         for (int k = 0; k < 4; ++k) tc::mma_bf16_tmem_a(tmem + kColO2, sa + k * 8, qa + k * 2, idO2, i + k > 0);
-                    if (!(ok = wait(&bar.pready, n & 1))) break;
-                    tc::fence_after_sync();
-                    const uint64_t vc = tc::smem_desc_sw128_mn(tile + kOffC, kBox);
+                    const uint64_t vc = tc::smem_desc_sw128_mn(tile + kOffC, kBox), pn = dP + (n & 1) * kBox / 16;
 #pragma unroll
-                    for (int k = 0; k < 4; ++k) tc::mma_bf16(tmem + kColO1, vc + k * 2048 / 16, dP + k * 2, idO1, k > 0);
+                    for (int k = 0; k < 4; ++k) tc::mma_bf16(tmem + kColO1, vc + k * 2048 / 16, pn + k * 2, idO1, k > 0);
                     tc::mma_commit(&bar.odone);
+                    tc::mma_commit(&bar.pfree[n & 1]);
                 }
                 tc::mma_commit(&bar.empty[st]);
                 done = n + 1;
-                if (++st == stages) st = 0, phase ^= 1;
-                if (!STATE_ONLY && n + 1 < steps) {
-                    if (!(ok = wait(&bar.full[st], phase))) break;
-                    scores(st);
-                }
+                st = st1, phase = phase1;
             }
-            // nor a product
+            if (STATE_ONLY && ok) tc::mma_commit(&bar.tlast);
+            // no product may be in flight when the CTA ends, whatever happened to its consumers
             if (done) tc::mbar_wait(&bar.empty[(done - 1) % stages], ((done - 1) / stages) & 1, kWaitNs);
+        } else if (warp == kTmaWarp && tc::elect_one()) {
+            // --------------------------------------------------------------- loads
+            const int ha = (h / p.ag) * tp.bmul[0], hk = (h / p.bg) * tp.bmul[1], hc = (h / p.cg) * tp.bmul[2];
+            const int ba = (int)b * tp.amul[0], bb = (int)b * tp.amul[1], bc = (int)b * tp.amul[2];
+            int issued = 0, st = 0, phase = 0;
+            for (int n = 0; n < steps; ++n) {
+                if (n >= stages && !wait(&bar.empty[st], phase ^ 1)) break;
+                char *dst = smem + st * kStage;
+                const int t0 = start_of(n);
+                tc::mbar_arrive_expect_tx(&bar.full[st], kStage);
+#pragma unroll
+                for (int i = 0; i < DKB; ++i) {
+                    if (!STATE_ONLY) tc::tma_load_4d(dst + i * kBox, &maps.a, i * 64, t0, ha, ba, &bar.full[st]);
+                    tc::tma_load_4d(dst + kOffB + i * kBox, &maps.b, i * 64, t0, hk, bb, &bar.full[st]);
+                }
+#pragma unroll
+                for (int i = 0; i < VB; ++i) tc::tma_load_4d(dst + kOffC + i * kBox, &maps.c, i * 64, t0, hc, bc, &bar.full[st]);
+                issued = n + 1;
+                if (++st == stages) st = 0, phase ^= 1;
+            }
+            // nor a copy
+            for (int n = issued > stages ? issued - stages : 0; n < issued; ++n)
+                tc::mbar_wait(&bar.full[n % stages], (n / stages) & 1, kWaitNs);
         }
     }
     __syncwarp();
@@ -618,7 +635,7 @@ __global__ void __launch_bounds__(kTcThreads, 1) decay_walk_tc_kernel(const TcPa
 template <int DKB, int VB, int TERMS, typename OT, bool STATE_ONLY>
 int tc_launch(const TcParams &tp, const Maps &maps, bool dependent, cudaStream_t st) {
     constexpr int smem = stages_of<DKB, VB, STATE_ONLY>() * (STATE_ONLY ? DKB + VB : 2 * DKB + VB) * kBox +
-                         (1 + 2 * VB) * kBox + 1024;
+                         2 * (1 + VB) * kBox + 1024;
     auto kernel = decay_walk_tc_kernel<DKB, VB, TERMS, OT, STATE_ONLY>;
     constexpr int kMaxDevices = 64;
     static std::mutex mu;

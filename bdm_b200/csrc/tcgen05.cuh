@@ -25,6 +25,11 @@ __device__ __forceinline__ bool elect_one() {
     return p != 0;
 }
 
+// This warp group's registers per thread from here on.  The groups' shares must not exceed, in all, what the block
+// was launched with.
+template <int N> __device__ __forceinline__ void regs_up() { asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;\n" ::"n"(N)); }
+template <int N> __device__ __forceinline__ void regs_down() { asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;\n" ::"n"(N)); }
+
 // ------------------------------------------------------------------ mbarriers
 __device__ __forceinline__ void mbar_init(uint64_t *bar, unsigned count) {
     asm volatile("mbarrier.init.shared::cta.b64 [%0], %1;\n" ::"r"(smem_u32(bar)), "r"(count) : "memory");
@@ -193,8 +198,8 @@ __device__ __forceinline__ void tmem_st_16x128b_x2(uint32_t taddr, uint32_t r0, 
                  "r"(taddr)
                  : "memory");
 }
-// Four 8 x 8 matrices of 16-bit elements, transposed: lane l gives the address of row l % 8 of matrix l / 8 and
-// gets (holds) rows 2 (l % 4) + {0, 1} of column l / 4 of each.
+// Four 8 x 8 matrices of 16-bit elements: lane l gives the address of row l % 8 of matrix l / 8 and holds columns
+// 2 (l % 4) + {0, 1} of row l / 4 of each; transposed, rows 2 (l % 4) + {0, 1} of column l / 4.
 __device__ __forceinline__ void ldmatrix_x4_trans(const void *row, uint32_t (&r)[4]) {
     asm volatile("ldmatrix.sync.aligned.m8n8.x4.trans.shared.b16 {%0, %1, %2, %3}, [%4];\n"
                  : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3])
@@ -204,6 +209,11 @@ __device__ __forceinline__ void ldmatrix_x4_trans(const void *row, uint32_t (&r)
 __device__ __forceinline__ void stmatrix_x4_trans(void *row, uint32_t r0, uint32_t r1, uint32_t r2, uint32_t r3) {
     asm volatile("stmatrix.sync.aligned.m8n8.x4.trans.shared.b16 [%0], {%1, %2, %3, %4};\n" ::"r"(smem_u32(row)), "r"(r0),
                  "r"(r1), "r"(r2), "r"(r3)
+                 : "memory");
+}
+__device__ __forceinline__ void stmatrix_x4(void *row, uint32_t r0, uint32_t r1, uint32_t r2, uint32_t r3) {
+    asm volatile("stmatrix.sync.aligned.m8n8.x4.shared.b16 [%0], {%1, %2, %3, %4};\n" ::"r"(smem_u32(row)), "r"(r0), "r"(r1),
+                 "r"(r2), "r"(r3)
                  : "memory");
 }
 // 4-D tiled store of one box from shared memory (async proxy; clipped at the tensor's ends), its group's commit,
