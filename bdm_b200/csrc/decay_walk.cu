@@ -23,15 +23,26 @@ int simt_smem(int wab, bool state_only) {
     return f * 4;
 }
 
-// Rows [t0, t0 + 64) of one head into shared memory as FP32; invalid rows and columns are zero.
+// Rows [t0, t0 + 64) of one head into shared memory as FP32; invalid rows and columns are zero.  A warp takes
+// every 8th row, its lanes neighbouring columns; four rows' loads are in flight at a time.
 template <typename T>
 __device__ __forceinline__ void load_rows(float *dst, int pitch, const T *src, int64_t st, int64_t t0, int valid, int first,
                                           int width, int cols) {
-    for (int i = threadIdx.x; i < kChunk * cols; i += kThreads) {
-        const int r = i / cols, d = i % cols;
-        float x = 0.f;
-        if (r < valid && first + d < width) x = Elem<T>::to_float(src[(t0 + r) * st + first + d]);
-        dst[r * pitch + d] = x;
+    const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+    for (int d = lane; d < cols; d += 32) {
+        const bool in = first + d < width;
+        const T *p = src + t0 * st + first + d;
+#pragma unroll
+        for (int u0 = 0; u0 < kChunk / 8; u0 += 4) {
+            float x[4];
+#pragma unroll
+            for (int u = 0; u < 4; ++u) {
+                const int r = warp + (u0 + u) * 8;
+                x[u] = in && r < valid ? Elem<T>::to_float(p[r * st]) : 0.f;
+            }
+#pragma unroll
+            for (int u = 0; u < 4; ++u) dst[(warp + (u0 + u) * 8) * pitch + d] = x[u];
+        }
     }
 }
 
@@ -41,8 +52,10 @@ __global__ void __launch_bounds__(kThreads) decay_walk_kernel(const Params p) {
     extern __shared__ float sm[];
     const int slices = (p.wc + kCols - 1) / kCols;
     int64_t id = blockIdx.x;
-    const int seg = (int)(id % p.nseg);
-    id /= p.nseg;
+    const int segs = STATE_ONLY ? p.nseg - 1 : p.nseg;
+    const int zid = (int)(id % segs);
+    const int seg = STATE_ONLY ? zid + p.reverse : zid;  // the last segment walked needs no state of its own
+    id /= segs;
     const int slice = (int)(id % slices);
     const int64_t bh = id / slices;
     const int64_t b = bh / p.heads;
@@ -59,6 +72,8 @@ __global__ void __launch_bounds__(kThreads) decay_walk_kernel(const Params p) {
 
     const float g = head_log_decay(p, h);
     for (int i = threadIdx.x; i <= kChunk; i += kThreads) pw[i] = i ? expf(g * (float)i) : 1.f;
+    asm volatile("griddepcontrol.launch_dependents;\n" ::: "memory");
+    if (!STATE_ONLY && p.nseg > 1) asm volatile("griddepcontrol.wait;\n" ::: "memory");
 
     const Span sp = span_of(p, row_tokens(p, b), seg);
     const int tx = threadIdx.x % 16, ty = threadIdx.x / 16;
@@ -68,13 +83,25 @@ __global__ void __launch_bounds__(kThreads) decay_walk_kernel(const Params p) {
     OT *out = static_cast<OT *>(p.out) + b * p.os[0] + h * p.os[2];
 
     // state elements (ty + 16 r, n0 + 4 tx + e) in registers
+    const int64_t size = (int64_t)p.wab * p.wc;
+    const bool before = !STATE_ONLY && p.nseg > 1 && (p.reverse ? seg < p.nseg - 1 : seg > 0);
+    float given = 0.f;
+    if (!STATE_ONLY && p.state_in) {
+        const int64_t end = sp.c1 * kChunk < sp.n ? sp.c1 * kChunk : sp.n;
+        const int64_t far = p.reverse ? sp.n - end : sp.c0 * kChunk;
+        given = (far ? expf(g * (float)far) : 1.f) * p.in_mul;
+    }
     float S[8][4];
 #pragma unroll
     for (int r = 0; r < 8; ++r)
 #pragma unroll
         for (int e = 0; e < 4; ++e) {
             const int i = ty + 16 * r, j = n0 + 4 * tx + e;
-            S[r][e] = (!STATE_ONLY && i < p.wab && j < p.wc) ? start_state(p, sp, bh, seg, g, i, j) : 0.f;
+            S[r][e] = 0.f;
+            if (i >= p.wab || j >= p.wc) continue;
+            if (before) S[r][e] = p.seg[(bh * p.nseg + seg) * size + (int64_t)i * p.wc + j];
+            if (!STATE_ONLY && p.state_in)
+                S[r][e] = fmaf(given, p.state_in[bh * size + (p.in_t ? (int64_t)j * p.wab + i : (int64_t)i * p.wc + j)], S[r][e]);
         }
 
     for (int64_t step = 0; step < sp.c1 - sp.c0; ++step) {
@@ -167,7 +194,8 @@ __global__ void __launch_bounds__(kThreads) decay_walk_kernel(const Params p) {
                 }
             }
         }
-        // S = lam^valid S + sum_j lam^. b_j c_j
+        // S = lam^valid S + sum_j lam^. b_j c_j, where anyone asks for it
+        if (!STATE_ONLY && step + 1 == sp.c1 - sp.c0 && !(p.state_out && sp.last)) break;
         const float carry = pw[valid];
 #pragma unroll
         for (int r = 0; r < 8; ++r)
@@ -186,7 +214,6 @@ __global__ void __launch_bounds__(kThreads) decay_walk_kernel(const Params p) {
         }
     }
 
-    const int64_t size = (int64_t)p.wab * p.wc;
     if (STATE_ONLY || (p.state_out && sp.last)) {
 #pragma unroll
         for (int r = 0; r < 8; ++r)
@@ -195,7 +222,7 @@ __global__ void __launch_bounds__(kThreads) decay_walk_kernel(const Params p) {
                 const int i = ty + 16 * r, j = n0 + 4 * tx + e;
                 if (i >= p.wab || j >= p.wc) continue;
                 if (STATE_ONLY)
-                    p.seg[(bh * p.nseg + seg) * size + (int64_t)j * p.wab + i] = S[r][e];
+                    p.seg[(bh * segs + zid) * size + (int64_t)i * p.wc + j] = S[r][e];
                 else
                     p.state_out[bh * size + (p.out_t ? (int64_t)j * p.wab + i : (int64_t)i * p.wc + j)] =
                         S[r][e] * p.out_mul;
@@ -210,6 +237,38 @@ __global__ void __launch_bounds__(kThreads) decay_walk_kernel(const Params p) {
         const int cols = p.wc - n0 < kCols ? p.wc - n0 : kCols;
         for (int64_t i = threadIdx.x; i < (z1 - z0) * cols; i += kThreads)
             out[(z0 + i / cols) * p.os[1] + n0 + i % cols] = Elem<OT>::from_float(0.f);
+    }
+}
+
+// The state each segment starts from (without the given one): the sub-segments before it in walk order, each
+// lam^(tokens of one) further away than the next.  One thread per state element.
+__global__ void __launch_bounds__(256) decay_prefix_kernel(const Params p, const float *__restrict__ z, int sub, int scps) {
+    asm volatile("griddepcontrol.launch_dependents;\n" ::: "memory");
+    asm volatile("griddepcontrol.wait;\n" ::: "memory");
+    const int64_t size = (int64_t)p.wab * p.wc, blocks = (size + 255) / 256;
+    const int64_t bh = blockIdx.x / blocks, e = blockIdx.x % blocks * 256 + threadIdx.x;
+    if (e >= size) return;
+    const float step = expf(head_log_decay(p, (int)(bh % p.heads)) * (float)((int64_t)scps * kChunk));
+    const int count = (p.nseg - 1) * sub;
+    const int64_t dir = p.reverse ? -1 : 1;
+    const float *src = z + (bh * count + (p.reverse ? count - 1 : 0)) * size + e;
+    float *dst = p.seg + (bh * p.nseg + (p.reverse ? p.nseg - 2 : 1)) * size + e;
+    float acc = 0.f;
+    int u = 0;
+    for (int i = 0; i < count; i += 8) {
+        float x[8];
+#pragma unroll
+        for (int k = 0; k < 8; ++k) x[k] = i + k < count ? src[dir * (i + k) * size] : 0.f;
+#pragma unroll
+        for (int k = 0; k < 8; ++k) {
+            if (i + k >= count) break;
+            acc = fmaf(acc, step, x[k]);
+            if (++u == sub) {
+                *dst = acc;
+                dst += dir * size;
+                u = 0;
+            }
+        }
     }
 }
 
@@ -254,23 +313,41 @@ int device_setup(int &sms) {
     return BDM_OK;
 }
 
-template <typename T, typename OT> int simt_launch(const Params &p, bool state_only, cudaStream_t st) {
-    const int64_t blocks = p.batch * p.heads * ceil_div(p.wc, kCols) * p.nseg;
-    if (blocks > 0x7fffffff) return BDM_ERR_UNSUPPORTED;
-    const int smem = simt_smem(p.wab, state_only);
-    if (state_only)
-        decay_walk_kernel<T, T, true><<<(unsigned)blocks, kThreads, smem, st>>>(p);
-    else
-        decay_walk_kernel<T, OT, false><<<(unsigned)blocks, kThreads, smem, st>>>(p);
+// The state launch, the prefix launch and the walk; each start overlaps the end of the one before.
+template <typename T, typename OT> int simt_launch(Params p, void *workspace, cudaStream_t st) {
+    const int64_t rows = p.batch * p.heads, slices = ceil_div(p.wc, kCols), size = (int64_t)p.wab * p.wc;
+    if (rows * slices * p.nseg > 0x7fffffff) return BDM_ERR_UNSUPPORTED;
+    cudaLaunchConfig_t cfg{};
+    cfg.blockDim = dim3(kThreads);
+    cfg.stream = st;
+    cudaLaunchAttribute attr{};
+    attr.id = cudaLaunchAttributeProgrammaticStreamSerialization;
+    attr.val.programmaticStreamSerializationAllowed = 1;
+    cfg.attrs = &attr;
+    if (p.nseg > 1) {
+        p.seg = static_cast<float *>(workspace);
+        float *z = p.seg + rows * p.nseg * size;
+        Params q = p;
+        q.seg = z;
+        cfg.gridDim = dim3((unsigned)(rows * slices * (p.nseg - 1)));
+        cfg.dynamicSmemBytes = simt_smem(p.wab, true);
+        if (int rc = cuda_status(cudaLaunchKernelEx(&cfg, decay_walk_kernel<T, T, true>, (const Params)q))) return rc;
+        if (int rc = launch_status()) return rc;
+        if (int rc = decay_prefix_launch(p, z, 1, p.cps, st)) return rc;
+        cfg.numAttrs = 1;
+    }
+    cfg.gridDim = dim3((unsigned)(rows * slices * p.nseg));
+    cfg.dynamicSmemBytes = simt_smem(p.wab, false);
+    if (int rc = cuda_status(cudaLaunchKernelEx(&cfg, decay_walk_kernel<T, OT, false>, (const Params)p))) return rc;
     return launch_status();
 }
 
-// Segments of the time axis for the CUDA-core walk: enough CTAs for two per SM, at least 4 chunks each.
+// Segments of the time axis for the CUDA-core walk: three CTAs per SM, down to a chunk each.  A segment more
+// costs a second pass over its b and c and half of a chunk's arithmetic, so rows that fill the GPU stay whole.
 int64_t simt_segments(int64_t ctas, int64_t chunks, int sms) {
-    if (ctas >= sms || chunks < 8) return 1;
-    int64_t s = 2 * sms / ctas;
-    if (s > chunks / 4) s = chunks / 4;
-    return s < 1 ? 1 : s;
+    if (ctas >= 2 * sms) return 1;
+    const int64_t s = 3 * sms / ctas;
+    return s > chunks ? chunks : s;
 }
 
 struct Split {
@@ -322,11 +399,27 @@ int check_args(const bdm_decay_walk_args &w) {
 }
 
 int64_t seg_bytes(const Params &p, const Split &split) {
-    if (split.tc) return decay_walk_tc_bytes(p, split.sub);
-    return p.nseg > 1 ? p.batch * p.heads * p.nseg * (int64_t)p.wab * p.wc * 4 : 0;
+    return p.nseg > 1 ? p.batch * p.heads * ((int64_t)p.nseg + (int64_t)(p.nseg - 1) * split.sub) * p.wab * p.wc * 4 : 0;
 }
 
 }  // namespace
+
+int decay_prefix_launch(const walk::Params &p, const float *z, int sub, int scps, cudaStream_t st) {
+    const int64_t blocks = p.batch * p.heads * ceil_div((int64_t)p.wab * p.wc, 256);
+    if (blocks > 0x7fffffff) return BDM_ERR_UNSUPPORTED;
+    cudaLaunchConfig_t cfg{};
+    cfg.gridDim = dim3((unsigned)blocks);
+    cfg.blockDim = dim3(256);
+    cfg.stream = st;
+    cudaLaunchAttribute attr{};
+    attr.id = cudaLaunchAttributeProgrammaticStreamSerialization;
+    attr.val.programmaticStreamSerializationAllowed = 1;
+    cfg.attrs = &attr;
+    cfg.numAttrs = 1;
+    if (int rc = cuda_status(cudaLaunchKernelEx(&cfg, decay_prefix_kernel, p, z, sub, scps))) return rc;
+    return launch_status();
+}
+
 }  // namespace bdm
 
 extern "C" int64_t bdm_decay_walk_workspace_bytes(const bdm_decay_walk_args *w) {
@@ -354,20 +447,11 @@ extern "C" int bdm_decay_walk(const bdm_decay_walk_args *w, void *workspace, int
     if (int rc = plan(*w, p, split, sms)) return rc;
     const int64_t need = seg_bytes(p, split);
     if (need > workspace_bytes || (need && !workspace)) return BDM_ERR_WORKSPACE;
-    p.seg = static_cast<float *>(workspace);
     cudaStream_t st = as_stream(stream);
     if (split.tc) return decay_walk_tc_launch(*w, p, split.sub, split.scps, workspace, st);
-    for (int pass = p.nseg > 1 ? 0 : 1; pass < 2; ++pass) {
-        int rc;
-        if (w->dtype == BDM_F32)
-            rc = simt_launch<float, float>(p, pass == 0, st);
-        else if (w->out_dtype == BDM_F32)
-            rc = simt_launch<bf16, float>(p, pass == 0, st);
-        else
-            rc = simt_launch<bf16, bf16>(p, pass == 0, st);
-        if (rc) return rc;
-    }
-    return BDM_OK;
+    if (w->dtype == BDM_F32) return simt_launch<float, float>(p, workspace, st);
+    if (w->out_dtype == BDM_F32) return simt_launch<bf16, float>(p, workspace, st);
+    return simt_launch<bf16, bf16>(p, workspace, st);
 }
 
 extern "C" int bdm_decay_group_sum(const float *part, int64_t tokens, int groups, int group, int width, int dtype, void *out,

@@ -12,8 +12,8 @@
 // In a chunk of kChunk tokens starting at t0, row r = t - t0 of n' = min(kChunk, n - t0) valid ones, the
 // exponents are: inside t-s (or s-t); reading the carried state r+1 (n'-1-r); writing it n'-1-r (r+1);
 // carrying it n'.  The time axis is cut into segments of whole chunks when there are too few (row, head)
-// pairs for the SMs: a first launch leaves every segment's own state (X = 0) in the workspace, and the
-// main launch starts each segment from the given state and its predecessors'.
+// pairs for the SMs: a first launch leaves the segments' own states (X = 0) in the workspace, a second sums
+// what each segment starts from (in order: no atomics), and the main launch walks all segments side by side.
 #pragma once
 
 #include "common.cuh"
@@ -37,7 +37,7 @@ struct Params {
     float *state_out;
     float in_mul, out_mul;
     int in_t, out_t;  // state stored [wc, wab] instead of [wab, wc]
-    float *seg;       // segment states, [batch*heads, nseg, wc, wab]
+    float *seg;       // what each segment starts from, beside the given state: [batch*heads, nseg, wab * wc]
     int64_t batch, time;
     int heads, wab, wc, reverse;
     float scale;
@@ -75,38 +75,15 @@ __device__ __forceinline__ Span span_of(const Params &p, int64_t n, int seg) {
     return s;
 }
 
-// Element (i of wab, j of wc) of the state the segment starts from.
-__device__ __forceinline__ float start_state(const Params &p, const Span &s, int64_t bh, int seg, float g, int i, int j) {
-    const int64_t size = (int64_t)p.wab * p.wc;
-    float x = 0.f;
-    if (p.state_in) {
-        const int64_t end = s.c1 * kChunk < s.n ? s.c1 * kChunk : s.n;
-        const int64_t far = p.reverse ? s.n - end : s.c0 * kChunk;
-        const float v = p.state_in[bh * size + (p.in_t ? (int64_t)j * p.wab + i : (int64_t)i * p.wc + j)] * p.in_mul;
-        x = far ? v * expf(g * (float)far) : v;
-    }
-    if (p.nseg > 1) {
-        // predecessors in walk order, nearest last; all but the row's last segment are whole
-        const float *z = p.seg + (bh * p.nseg) * size + (int64_t)j * p.wab + i;
-        const float step = expf(g * (float)((int64_t)p.cps * kChunk));
-        float acc = 0.f;
-        if (!p.reverse) {
-            for (int q = 0; q < seg; ++q) acc = acc * step + z[q * size];
-        } else {
-            const int lastseg = (int)((s.chunks + p.cps - 1) / p.cps) - 1;
-            for (int q = lastseg; q > seg; --q) acc = acc * step + z[q * size];
-        }
-        x += acc;
-    }
-    return x;
-}
-
 }  // namespace walk
+
+// Sums the segments' start states from z, [batch*heads, (nseg - 1) * sub, wab * wc], the own states of the
+// sub-segments (scps chunks each, sub in a segment) of all segments but the last one walked.
+int decay_prefix_launch(const walk::Params &p, const float *z, int sub, int scps, cudaStream_t st);
 
 // The tensor-core walk (decay_walk_tc.cu): BF16 operands that TMA can address.
 bool decay_walk_tc_takes(const bdm_decay_walk_args &w);
 void decay_walk_tc_split(int64_t rows, int64_t chunks, int sms, int &nseg, int &cps, int &sub, int &scps);
-int64_t decay_walk_tc_bytes(const walk::Params &p, int sub);
 int decay_walk_tc_launch(const bdm_decay_walk_args &w, walk::Params p, int sub, int scps, void *workspace, cudaStream_t st);
 
 }  // namespace bdm

@@ -55,38 +55,6 @@ bool encode(EncodeTiled fn, CUtensorMap *m, const Operand &o, int64_t time, int6
 }
 
 
-// The state each segment starts from (without the given one): the sub-segments before it in walk order, each
-// lam^(tokens of one) further away than the next.  One thread per state element.
-__global__ void __launch_bounds__(256) decay_prefix_kernel(const Params p, const float *__restrict__ z, int sub, int scps) {
-    asm volatile("griddepcontrol.launch_dependents;\n" ::: "memory");
-    asm volatile("griddepcontrol.wait;\n" ::: "memory");
-    const int64_t size = (int64_t)p.wab * p.wc, blocks = (size + 255) / 256;
-    const int64_t bh = blockIdx.x / blocks, e = blockIdx.x % blocks * 256 + threadIdx.x;
-    if (e >= size) return;
-    const float step = expf(head_log_decay(p, (int)(bh % p.heads)) * (float)((int64_t)scps * kChunk));
-    const int count = (p.nseg - 1) * sub;
-    const int64_t dir = p.reverse ? -1 : 1;
-    const float *src = z + (bh * count + (p.reverse ? count - 1 : 0)) * size + e;
-    float *dst = p.seg + (bh * p.nseg + (p.reverse ? p.nseg - 2 : 1)) * size + e;
-    float acc = 0.f;
-    int u = 0;
-    for (int i = 0; i < count; i += 8) {
-        float x[8];
-#pragma unroll
-        for (int k = 0; k < 8; ++k) x[k] = i + k < count ? src[dir * (i + k) * size] : 0.f;
-#pragma unroll
-        for (int k = 0; k < 8; ++k) {
-            if (i + k >= count) break;
-            acc = fmaf(acc, step, x[k]);
-            if (++u == sub) {
-                *dst = acc;
-                dst += dir * size;
-                u = 0;
-            }
-        }
-    }
-}
-
 }  // namespace
 
 bool decay_walk_tc_takes(const bdm_decay_walk_args &w) {
@@ -98,6 +66,7 @@ bool decay_walk_tc_takes(const bdm_decay_walk_args &w) {
         if (!fits_tma(o, w.time, w.batch)) return false;
     if (w.out_dtype == BDM_BF16) {
         if (!fits_tma({w.out, w.out_stride, w.width_c, w.heads}, w.time, w.batch)) return false;
+        if (w.width_c % 8) return false;
         if ((w.batch > 1 && !w.out_stride[0]) || (w.heads > 1 && !w.out_stride[2])) return false;
     }
     return encode_tiled() != nullptr;
@@ -119,10 +88,6 @@ void decay_walk_tc_split(int64_t rows, int64_t chunks, int sms, int &nseg, int &
         const double t = ceil_div(rows * n, sms) * (c + 3.0) + ceil_div(rows * (n - 1) * u, sms) * (0.6 * sc + 3.0) + 6.0;
         if (t < cost) cost = t, nseg = (int)n, cps = (int)c, sub = (int)u, scps = (int)sc;
     }
-}
-
-int64_t decay_walk_tc_bytes(const Params &p, int sub) {
-    return p.nseg > 1 ? p.batch * p.heads * ((int64_t)p.nseg + (int64_t)(p.nseg - 1) * sub) * p.wab * p.wc * 4 : 0;
 }
 
 int decay_walk_tc_launch(const bdm_decay_walk_args &w, Params p, int sub, int scps, void *workspace, cudaStream_t st) {
@@ -150,19 +115,7 @@ int decay_walk_tc_launch(const bdm_decay_walk_args &w, Params p, int sub, int sc
     auto run = p.wab > 64 ? (p.wc > 64 ? tc_launch_22 : tc_launch_21) : (p.wc > 64 ? tc_launch_12 : tc_launch_11);
     if (p.nseg > 1) {
         if (int rc = run(tp, maps, kTcState, terms, false, st)) return rc;
-        const int64_t blocks = p.batch * p.heads * ceil_div((int64_t)p.wab * p.wc, 256);
-        if (blocks > 0x7fffffff) return BDM_ERR_UNSUPPORTED;
-        cudaLaunchConfig_t cfg{};
-        cfg.gridDim = dim3((unsigned)blocks);
-        cfg.blockDim = dim3(256);
-        cfg.stream = st;
-        cudaLaunchAttribute attr{};
-        attr.id = cudaLaunchAttributeProgrammaticStreamSerialization;
-        attr.val.programmaticStreamSerializationAllowed = 1;
-        cfg.attrs = &attr;
-        cfg.numAttrs = 1;
-        if (int rc = cuda_status(cudaLaunchKernelEx(&cfg, decay_prefix_kernel, p, (const float *)tp.z, sub, scps))) return rc;
-        if (int rc = launch_status()) return rc;
+        if (int rc = decay_prefix_launch(p, tp.z, sub, scps, st)) return rc;
     }
     return run(tp, maps, w.out_dtype == BDM_F32 ? kTcFloat : kTcBf16, terms, p.nseg > 1, st);
 }

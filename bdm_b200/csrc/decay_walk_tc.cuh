@@ -57,7 +57,7 @@ struct TcParams {
     Params p;
     int amul[3], bmul[3];  // 0 where the operand's batch (head) is shared by all: a, b, c
     int sub, scps;         // state launch: sub-segments of a segment, chunks of one
-    float *z;              // its states, [batch*heads, (nseg - 1) * sub, wc, wab]
+    float *z;              // its states, [batch*heads, (nseg - 1) * sub, wc * wab]
 };
 
 // A parity tells a phase from the next only, so no waiter may fall two phases behind: each barrier's next phase
@@ -471,14 +471,6 @@ __global__ void __launch_bounds__(kTcThreads, 1) decay_walk_tc_kernel(const TcPa
                 }
             }
             if (kTma && warp == kOutWarp && lane == 0) tc::tma_store_wait();
-            // whole chunks past the row's length
-            int64_t z0 = sp.chunks * kChunk, z1 = p.time;
-            const int64_t s0 = (int64_t)seg * p.cps * kChunk, s1 = s0 + (int64_t)p.cps * kChunk;
-            if (z0 < s0) z0 = s0;
-            if (z1 > s1) z1 = s1;
-            const int col = threadIdx.x - kOutWarp * 32;
-            if (col < p.wc)
-                for (int64_t t = z0; t < z1; ++t) out[t * p.os[1] + col] = Elem<OT>::from_float(0.f);
         }
     } else if (warp < kMmaWarp) {
         tc::regs_down<kScoreRegs>();
@@ -624,6 +616,24 @@ __global__ void __launch_bounds__(kTcThreads, 1) decay_walk_tc_kernel(const TcPa
     __syncwarp();
     tc::fence_before_sync();
     __syncthreads();
+    if constexpr (!STATE_ONLY) {
+        // whole chunks past the row's length
+        int64_t z0 = sp.chunks * kChunk, z1 = p.time;
+        const int64_t s0 = (int64_t)seg * p.cps * kChunk, s1 = s0 + (int64_t)p.cps * kChunk;
+        if (z0 < s0) z0 = s0;
+        if (z1 > s1) z1 = s1;
+        OT *out = static_cast<OT *>(p.out) + b * p.os[0] + h * p.os[2];
+        constexpr int kLane = sizeof(OT) == 2 ? 8 : 1;  // BF16 rows are whole 16-byte units (TMA writes them too)
+        const int units = p.wc / kLane, per = kTcThreads / units;
+        const int row = threadIdx.x / units, unit = threadIdx.x % units;
+        if (row < per)
+            for (int64_t t = z0 + row; t < z1; t += per) {
+                if constexpr (sizeof(OT) == 2)
+                    *reinterpret_cast<uint4 *>(out + t * p.os[1] + unit * 8) = make_uint4(0, 0, 0, 0);
+                else
+                    out[t * p.os[1] + unit] = 0.f;
+            }
+    }
     if (threadIdx.x == 0 && dead && p.status) *(volatile int *)p.status = 0x4;
     if (warp == kMmaWarp) {
         tc::fence_after_sync();
