@@ -111,6 +111,9 @@ int decay_walk_tc_launch(const bdm_decay_walk_args &w, Params p, int sub, int sc
     tp.sub = sub;
     tp.scps = scps;
     tp.z = p.seg + p.batch * p.heads * p.nseg * (int64_t)p.wab * p.wc;
+    // ragged rows in more than one wave (24 x 1333, 192 CTAs: 62 us in the order of the batch, 43 us sorted); a
+    // CTA's sort is a loop over the batch, so large batches, whose many waves level out by themselves, go without
+    tp.longest_first = p.lengths && p.batch > 1 && p.batch <= 256 && p.batch * p.heads * p.nseg > kNumSMs;
     const int terms = p.state_out ? 3 : 2;
     auto run = p.wab > 64 ? (p.wc > 64 ? tc_launch_22 : tc_launch_21) : (p.wc > 64 ? tc_launch_12 : tc_launch_11);
     if (p.nseg > 1) {

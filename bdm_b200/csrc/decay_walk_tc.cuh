@@ -57,6 +57,7 @@ struct TcParams {
     Params p;
     int amul[3], bmul[3];  // 0 where the operand's batch (head) is shared by all: a, b, c
     int sub, scps;         // state launch: sub-segments of a segment, chunks of one
+    int longest_first;     // rows are dealt out by length
     float *z;              // its states, [batch*heads, (nseg - 1) * sub, wc * wab]
 };
 
@@ -157,7 +158,23 @@ __global__ void __launch_bounds__(kTcThreads, 1) decay_walk_tc_kernel(const TcPa
     int64_t id = blockIdx.x;
     const int segs = STATE_ONLY ? (p.nseg - 1) * tp.sub : p.nseg;
     const int seg = (int)(id % segs);
-    const int64_t bh = id / segs;
+    int64_t bh = id / segs;
+    if (tp.longest_first) {
+        // rows in the order of their lengths, so that the last wave of CTAs is short ones
+        __shared__ int pick;
+        const int want = (int)(bh / p.heads), i = threadIdx.x;
+        if (i < p.batch) {
+            const int64_t mine = row_tokens(p, i);
+            int rank = 0;
+            for (int j = 0; j < p.batch; ++j) {
+                const int64_t other = row_tokens(p, j);
+                rank += other > mine || (other == mine && j < i);
+            }
+            if (rank == want) pick = i;
+        }
+        __syncthreads();
+        bh = (int64_t)pick * p.heads + bh % p.heads;
+    }
     const int64_t b = bh / p.heads;
     const int h = (int)(bh % p.heads);
     const float g = head_log_decay(p, h);
@@ -251,8 +268,9 @@ __global__ void __launch_bounds__(kTcThreads, 1) decay_walk_tc_kernel(const TcPa
             const int64_t end = sp.c1 * kChunk < sp.n ? sp.c1 * kChunk : sp.n;
             const int64_t far = p.reverse ? sp.n - end : sp.c0 * kChunk;
             const float w = p.state_in ? (far ? expf(g * (float)far) : 1.f) * p.in_mul : 0.f;
-            const float *x = p.state_in + bh * size;
-            if (before || p.state_in) {
+            const float *x = p.state_in ? p.state_in + bh * size : nullptr;
+            // every load at an address that exists, the ones outside selected away: no branch holds the next one up
+            auto gather = [&](const float *from, bool transposed, float mul) {
 #pragma unroll
                 for (int d = 0; d < kHalves; ++d)
 #pragma unroll
@@ -261,16 +279,16 @@ __global__ void __launch_bounds__(kTcThreads, 1) decay_walk_tc_kernel(const TcPa
                         float s[2];
 #pragma unroll
                         for (int e = 0; e < 2; ++e) {
-                            s[e] = 0.f;
-                            if (v < p.wc && k + e < p.wab) {
-                                if (before) s[e] = zs[(int64_t)v * p.wab + k + e];
-                                if (p.state_in)
-                                    s[e] = fmaf(w, x[p.in_t ? (int64_t)v * p.wab + k + e : (int64_t)(k + e) * p.wc + v], s[e]);
-                            }
+                            const bool in = v < p.wc && k + e < p.wab;
+                            const int at = transposed ? v * p.wab + k + e : (k + e) * p.wc + v;
+                            const float f = __ldg(from + (in ? at : 0));
+                            s[e] = in ? f : 0.f;
                         }
-                        S[d][i] = make2(s[0], s[1]);
+                        S[d][i] = fma2(make2(mul, mul), make2(s[0], s[1]), S[d][i]);
                     }
-            }
+            };
+            if (before) gather(zs, true, 1.f);
+            if (p.state_in) gather(x, p.in_t, w);
         }
         bool ok = true;
         for (int n = 0; n <= steps; ++n) {
