@@ -113,6 +113,74 @@ __device__ __forceinline__ float exp2_ftz(float x) {
     return y;
 }
 
+// The slice's maximum and a lower bound of its K-th largest logit: the largest, over the warps, of the K-th
+// largest of a warp's lane maxima (equal ones leave together: the bound is lower then, which is no harm).
+__device__ __forceinline__ void slice_bound(float mine, int K, float *redm, float *redk, float &m, float &bound,
+                                            TopShared &sh) {
+    const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+    uint32_t left = mine == mine ? ordered(mine) : 0u, top = __reduce_max_sync(0xffffffffu, left), kth = top;
+    for (int k = 1; k < K; ++k) {
+        if (left == kth) left = 0;
+        kth = __reduce_max_sync(0xffffffffu, left);
+    }
+    if (lane == 0) {
+        redm[warp] = unordered(top ? top : ordered(-INFINITY));
+        redk[warp] = unordered(kth ? kth : ordered(-INFINITY));
+    }
+    if (threadIdx.x == 0) sh.count = 0;
+    if (threadIdx.x < K) sh.best[threadIdx.x] = 0;
+    __syncthreads();
+    m = redm[0], bound = redk[0];
+#pragma unroll
+    for (int w = 1; w < kWarps; ++w) {
+        m = fmaxf(m, redm[w]);
+        bound = fmaxf(bound, redk[w]);
+    }
+}
+
+// Joins the warps' sums, collects the candidates that hot(use) names by index (a logit is read again: registers
+// have no index) and writes the K largest.
+template <typename T, typename F>
+__device__ __forceinline__ void finish_slice(float warp_total, float fix, float m, F hot, TopShared &sh, const T *src,
+                                             int base, int count, int vocab, int K, Slice *stat, u64 *dst) {
+    __shared__ float reds[kWarps];
+    if ((threadIdx.x & 31) == 0) reds[threadIdx.x >> 5] = warp_total;
+    hot([&](int i) {
+        if (i >= vocab) return;
+        const int at = atomicAdd(&sh.count, 1);
+        if (at < kList) sh.list[at] = make_key(Elem<T>::to_float(src[i]), (uint32_t)i);
+    });
+    __syncthreads();
+    if (threadIdx.x == 0) {
+        float t = 0.f;
+#pragma unroll
+        for (int w = 0; w < kWarps; ++w) t += reds[w];
+        t *= fix;
+        *stat = Slice{t == t ? m : NAN, t};
+    }
+    const int n = sh.count;
+    if (n <= kList) {
+        for (int i = threadIdx.x; i < n; i += kThreads) {
+            const u64 k = sh.list[i];
+            int rank = 0;
+            for (int j = 0; j < n && rank < K; ++j) rank += sh.list[j] > k;
+            if (rank < K) dst[rank] = k;
+        }
+        for (int i = n + threadIdx.x; i < K; i += kThreads) dst[i] = 0;
+        return;
+    }
+    // a few threads hold most of the largest logits: repeated maxima, over the logits read again
+    const int end = base + count < vocab ? base + count : vocab;
+    block_maxima(K, sh, [&](auto &&use) {
+#pragma unroll 1
+        for (int i = base + threadIdx.x; i < end; i += kThreads) {
+            const float y = Elem<T>::to_float(src[i]);
+            if (y == y) use(make_key(y, (uint32_t)i));
+        }
+    });
+    if (threadIdx.x < K) dst[threadIdx.x] = sh.best[threadIdx.x];
+}
+
 // One pass over the logits, E per thread in registers: the maximum, then the sum, then the few
 // candidates: the K-th largest of one warp's lane maxima bounds the K-th largest of the slice from below, and the
 // logits at or above the largest such bound (a few times K) go to a list and are ranked there; when the list
@@ -125,9 +193,8 @@ __global__ void __launch_bounds__(kThreads)
     beam_slice_kernel(const T *__restrict__ logits, int64_t ld, int vocab, int K, int splits, Slice *__restrict__ stat,
                       u64 *__restrict__ lists) {
     __shared__ TopShared sh;
-    __shared__ float redm[kWarps], redk[kWarps], reds[kWarps];
+    __shared__ float redm[kWarps], redk[kWarps];
     asm volatile("griddepcontrol.launch_dependents;\n" ::: "memory");
-    const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
     const int64_t row = blockIdx.x / splits;
     const int split = (int)(blockIdx.x % splits);
     const int base = split * (E * kThreads);
@@ -156,26 +223,8 @@ __global__ void __launch_bounds__(kThreads)
     float mine = -INFINITY;
 #pragma unroll
     for (int e = 0; e < E; ++e) mine = fmaxf(mine, x[e]);
-    // the warp's largest, and the K-th largest of its lanes' (equal ones leave together: the bound is lower
-    // then, which is no harm)
-    uint32_t left = mine == mine ? ordered(mine) : 0u, top = __reduce_max_sync(0xffffffffu, left), kth = top;
-    for (int k = 1; k < K; ++k) {
-        if (left == kth) left = 0;
-        kth = __reduce_max_sync(0xffffffffu, left);
-    }
-    if (lane == 0) {
-        redm[warp] = unordered(top ? top : ordered(-INFINITY));
-        redk[warp] = unordered(kth ? kth : ordered(-INFINITY));
-    }
-    if (threadIdx.x == 0) sh.count = 0;
-    if (threadIdx.x < K) sh.best[threadIdx.x] = 0;
-    __syncthreads();
-    float m = redm[0], bound = redk[0];
-#pragma unroll
-    for (int w = 1; w < kWarps; ++w) {
-        m = fmaxf(m, redm[w]);
-        bound = fmaxf(bound, redk[w]);
-    }
+    float m, bound;
+    slice_bound(mine, K, redm, redk, m, bound, sh);
     // NaN and +inf make the sum NaN, and with it the whole row's log-probabilities
     float s0 = 0.f, s1 = 0.f;
     if (m > -INFINITY) {
@@ -188,49 +237,88 @@ __global__ void __launch_bounds__(kThreads)
 #pragma unroll
         for (int e = 0; e < E; ++e) s0 += x[e] == -INFINITY ? 0.f : NAN;
     }
-    const float s = warp_sum(s0 + s1);
-    if (lane == 0) reds[warp] = s;
-    if (mine >= bound) {
+    finish_slice<T>(warp_sum(s0 + s1), 1.f, m, [&](auto &&use) {
+        if (mine < bound) return;
         uint32_t hot = 0;
 #pragma unroll
         for (int e = 0; e < E; ++e) hot |= x[e] >= bound ? 1u << e : 0u;
-        while (hot) {  // rare: the logit is read again, as registers have no index
-            const int e = __ffs(hot) - 1, i = index(e);
-            hot &= hot - 1;
-            if (i >= vocab) continue;
-            const int at = atomicAdd(&sh.count, 1);
-            if (at < kList) sh.list[at] = make_key(Elem<T>::to_float(src[i]), (uint32_t)i);
-        }
-    }
-    __syncthreads();
-    if (threadIdx.x == 0) {
-        float t = 0.f;
+        for (; hot; hot &= hot - 1) use(index(__ffs(hot) - 1));
+    }, sh, src, base, E * kThreads, vocab, K, stat + row * splits + split, lists + (row * splits + split) * K);
+}
+
+// The same for BF16 rows that start on 16-byte boundaries, which stay packed: the maximum and the comparisons
+// take two logits an instruction, and exp(x - max) is one packed multiply-add and ex2 (the rounding of
+// max * log2 e, which all terms share, is taken out of the sum at the end).
+template <int E>
+__global__ void __launch_bounds__(kThreads)
+    beam_slice_bf16_kernel(const bf16 *__restrict__ logits, int64_t ld, int vocab, int K, int splits,
+                           Slice *__restrict__ stat, u64 *__restrict__ lists) {
+    __shared__ TopShared sh;
+    __shared__ float redm[kWarps], redk[kWarps];
+    asm volatile("griddepcontrol.launch_dependents;\n" ::: "memory");
+    const int64_t row = blockIdx.x / splits;
+    const int split = (int)(blockIdx.x % splits);
+    const int base = split * (E * kThreads);
+    const bf16 *src = logits + row * ld;
+    uint32_t r[E / 2];
+    auto index = [&](int e) { return base + (e / 8 * kThreads + (int)threadIdx.x) * 8 + e % 8; };
 #pragma unroll
-        for (int w = 0; w < kWarps; ++w) t += reds[w];
-        stat[row * splits + split] = Slice{t == t ? m : NAN, t};
-    }
-    const int n = sh.count;
-    u64 *dst = lists + (row * splits + split) * K;
-    if (n <= kList) {
-        for (int i = threadIdx.x; i < n; i += kThreads) {
-            const u64 k = sh.list[i];
-            int rank = 0;
-            for (int j = 0; j < n && rank < K; ++j) rank += sh.list[j] > k;
-            if (rank < K) dst[rank] = k;
+    for (int v = 0; v < E / 8; ++v) {
+        const int i = index(8 * v);
+        uint4 q = make_uint4(0xff80ff80u, 0xff80ff80u, 0xff80ff80u, 0xff80ff80u);  // -inf
+        if (i + 8 <= vocab) {
+            q = *reinterpret_cast<const uint4 *>(src + i);
+        } else if (i < vocab) {
+            uint32_t w[4] = {q.x, q.y, q.z, q.w};
+#pragma unroll
+            for (int u = 0; u < 8; ++u)
+                if (i + u < vocab) {
+                    const uint32_t bits = (uint32_t)__bfloat16_as_ushort(src[i + u]) << (u & 1 ? 16 : 0);
+                    w[u / 2] = (w[u / 2] & (u & 1 ? 0xffffu : 0xffff0000u)) | bits;
+                }
+            q = make_uint4(w[0], w[1], w[2], w[3]);
         }
-        for (int i = n + threadIdx.x; i < K; i += kThreads) dst[i] = 0;
-        return;
+        r[4 * v] = q.x, r[4 * v + 1] = q.y, r[4 * v + 2] = q.z, r[4 * v + 3] = q.w;
     }
-    // a few threads hold most of the largest logits: repeated maxima, over the logits read again
-    const int end = base + E * kThreads < vocab ? base + E * kThreads : vocab;
-    block_maxima(K, sh, [&](auto &&use) {
-#pragma unroll 1
-        for (int i = base + threadIdx.x; i < end; i += kThreads) {
-            const float y = Elem<T>::to_float(src[i]);
-            if (y == y) use(make_key(y, (uint32_t)i));
+    auto two = [](uint32_t w) { return *reinterpret_cast<const __nv_bfloat162 *>(&w); };
+    __nv_bfloat162 top2 = two(r[0]);
+#pragma unroll
+    for (int i = 1; i < E / 2; ++i) top2 = __hmax2(top2, two(r[i]));
+    const float mine = fmaxf(__low2float(top2), __high2float(top2));
+    float m, bound;
+    slice_bound(mine, K, redm, redk, m, bound, sh);
+    float sum = 0.f, fix = 1.f;
+    if (m > -INFINITY && m < INFINITY) {
+        constexpr float kLog2e = 1.4426950408889634f;
+        const float c = m * kLog2e;
+        fix = exp2_ftz(-fmaf(m, kLog2e, -c));
+        float s0 = 0.f, s1 = 0.f;
+#pragma unroll
+        for (int i = 0; i < E / 2; ++i) {
+            s0 += exp2_ftz(fmaf(__uint_as_float(r[i] << 16), kLog2e, -c));
+            s1 += exp2_ftz(fmaf(__uint_as_float(r[i] & 0xffff0000u), kLog2e, -c));
         }
-    });
-    if (threadIdx.x < K) dst[threadIdx.x] = sh.best[threadIdx.x];
+        sum = s0 + s1;
+    } else if (m == -INFINITY) {  // all -inf, or NaN
+#pragma unroll
+        for (int i = 0; i < E / 2; ++i) sum += __hbeq2(two(r[i]), __bfloat162bfloat162(__float2bfloat16_rn(-INFINITY))) ? 0.f : NAN;
+    } else {
+        sum = NAN;
+    }
+    finish_slice<bf16>(warp_sum(sum), fix, m, [&](auto &&use) {
+        if (mine < bound) return;
+        const __nv_bfloat162 b2 = __bfloat162bfloat162(__float2bfloat16_rn(bound));  // a logit: exact
+#pragma unroll
+        for (int v = 0; v < E / 8; ++v) {
+            uint32_t hot = 0;
+#pragma unroll
+            for (int i = 0; i < 4; ++i) hot |= (__hge2_mask(two(r[4 * v + i]), b2) & 0x10001u) << i;  // bit i: low, 16 + i: high
+            for (; hot; hot &= hot - 1) {
+                const int e = __ffs(hot) - 1;
+                use(index(8 * v) + 2 * (e & 15) + (e >> 4));
+            }
+        }
+    }, sh, src, base, E * kThreads, vocab, K, stat + row * splits + split, lists + (row * splits + split) * K);
 }
 
 // ------------------------------------------------------------------- merging
@@ -418,16 +506,28 @@ __global__ void __launch_bounds__(kThreads)
     }
 }
 
-// Logits per thread of the slice kernel and the splits of a row.
+// Logits per thread of the slice kernel and the splits of a row: as many as the registers hold (a CTA's fixed
+// work is then least) where the rows alone fill the GPU, 8 (more CTAs per row) where they do not.
 struct BeamPlan {
     int e, splits;
 };
-BeamPlan beam_plan(int64_t rows, int64_t vocab) {
+BeamPlan beam_plan(int64_t rows, int64_t vocab, bool packed) {
     BeamPlan p;
-    // 32 logits per thread where the rows alone fill the GPU, fewer (more CTAs per row) where they do not
-    p.e = rows * ceil_div(vocab, 32 * kThreads) >= kNumSMs ? 32 : 8;
+    p.e = packed ? 64 : 32;
+    if (p.e == 64 && rows * ceil_div(vocab, 64 * kThreads) < 2 * kNumSMs) p.e = 32;
+    if (p.e == 32 && rows * ceil_div(vocab, 32 * kThreads) < kNumSMs) p.e = 8;
     p.splits = (int)ceil_div(vocab, p.e * kThreads);
     return p;
+}
+
+template <typename T> using SliceFn = void (*)(const T *, int64_t, int, int, int, Slice *, u64 *);
+SliceFn<float> slice_fn(const float *, bool vec, int e) {
+    if (vec) return e == 32 ? beam_slice_kernel<float, 32, true> : beam_slice_kernel<float, 8, true>;
+    return e == 32 ? beam_slice_kernel<float, 32, false> : beam_slice_kernel<float, 8, false>;
+}
+SliceFn<bf16> slice_fn(const bf16 *, bool vec, int e) {
+    if (vec) return e == 64 ? beam_slice_bf16_kernel<64> : (e == 32 ? beam_slice_bf16_kernel<32> : beam_slice_bf16_kernel<8>);
+    return e == 32 ? beam_slice_kernel<bf16, 32, false> : beam_slice_kernel<bf16, 8, false>;
 }
 
 // ------------------------------------------------------------------ reordering
@@ -517,7 +617,7 @@ int reorder_launch(Tensors t, const int64_t *row_bytes, const int64_t *parents, 
 extern "C" int64_t bdm_beam_select_workspace_bytes(int64_t batch, int beams, int64_t vocab) {
     using namespace bdm;
     if (batch < 0 || beams <= 0 || vocab <= 0 || beams > kMaxBeams || vocab * beams >= 0xffffffffll) return -1;
-    const BeamPlan p = beam_plan(batch * beams, vocab);
+    const BeamPlan p = beam_plan(batch * beams, vocab, false);  // never fewer splits than the packed plan's
     return batch * beams * p.splits * ((int64_t)beams * 8 + 8);
 }
 
@@ -533,7 +633,8 @@ extern "C" int bdm_beam_select(const void *logits, int64_t ld, int64_t batch, in
     if (batch == 0) return BDM_OK;
     if (!logits || !scores || !out_scores || !out_parents || !out_tokens) return BDM_ERR_INVALID;
     const int64_t rows = batch * beams;
-    const BeamPlan p = beam_plan(rows, vocab);
+    const bool vec = (reinterpret_cast<uintptr_t>(logits) & 15) == 0 && (ld * (dtype == BDM_BF16 ? 2 : 4)) % 16 == 0;
+    const BeamPlan p = beam_plan(rows, vocab, vec && dtype == BDM_BF16);
     if (!workspace || workspace_bytes < bdm_beam_select_workspace_bytes(batch, beams, vocab)) return BDM_ERR_WORKSPACE;
     if (rows * p.splits > 0x7fffffff) return BDM_ERR_UNSUPPORTED;
     cudaStream_t st = as_stream(stream);
@@ -542,18 +643,8 @@ extern "C" int bdm_beam_select(const void *logits, int64_t ld, int64_t batch, in
     const unsigned grid = (unsigned)(rows * p.splits);
     BDM_DISPATCH_DTYPE(dtype, T, {
         const T *x = static_cast<const T *>(logits);
-        const bool vec = (reinterpret_cast<uintptr_t>(logits) & 15) == 0 && (ld * (int64_t)sizeof(T)) % 16 == 0;
-        if (p.e == 32) {
-            if (vec)
-                beam_slice_kernel<T, 32, true><<<grid, kThreads, 0, st>>>(x, ld, (int)vocab, beams, p.splits, stat, lists);
-            else
-                beam_slice_kernel<T, 32, false><<<grid, kThreads, 0, st>>>(x, ld, (int)vocab, beams, p.splits, stat, lists);
-        } else {
-            if (vec)
-                beam_slice_kernel<T, 8, true><<<grid, kThreads, 0, st>>>(x, ld, (int)vocab, beams, p.splits, stat, lists);
-            else
-                beam_slice_kernel<T, 8, false><<<grid, kThreads, 0, st>>>(x, ld, (int)vocab, beams, p.splits, stat, lists);
-        }
+        const SliceFn<T> slice = slice_fn(x, vec, p.e);
+        slice<<<grid, kThreads, 0, st>>>(x, ld, (int)vocab, beams, p.splits, stat, lists);
         if (int rc = launch_status()) return rc;
         // a programmatic dependent launch: its start overlaps the slices' end
         cudaLaunchConfig_t cfg{};
