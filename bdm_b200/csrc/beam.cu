@@ -113,15 +113,21 @@ __device__ __forceinline__ float exp2_ftz(float x) {
     return y;
 }
 
-// The slice's maximum and a lower bound of its K-th largest logit: the largest, over the warps, of the K-th
-// largest of a warp's lane maxima (equal ones leave together: the bound is lower then, which is no harm).
+// The slice's maximum and a lower bound of its K-th largest logit.  Every warp draws its K largest lane maxima
+// (equal ones leave together: the bound is lower then, which is no harm).  For K <= 8 the bound is the K-th
+// largest of all warps' together, which hardly more than K logits reach; past that, the largest of the warps'
+// K-th largest, which several times K do.
 __device__ __forceinline__ void slice_bound(float mine, int K, float *redm, float *redk, float &m, float &bound,
                                             TopShared &sh) {
+    constexpr unsigned all = 0xffffffffu;
     const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
-    uint32_t left = mine == mine ? ordered(mine) : 0u, top = __reduce_max_sync(0xffffffffu, left), kth = top;
-    for (int k = 1; k < K; ++k) {
+    uint32_t *drawn = reinterpret_cast<uint32_t *>(sh.list);  // [warp][8], before the list is used
+    uint32_t left = mine == mine ? ordered(mine) : 0u, kth = 0, top = 0;
+    for (int k = 0; k < K; ++k) {
+        kth = __reduce_max_sync(all, left);
+        if (k == 0) top = kth;
+        if (K <= 8 && lane == 0) drawn[warp * 8 + k] = kth;
         if (left == kth) left = 0;
-        kth = __reduce_max_sync(0xffffffffu, left);
     }
     if (lane == 0) {
         redm[warp] = unordered(top ? top : ordered(-INFINITY));
@@ -135,6 +141,16 @@ __device__ __forceinline__ void slice_bound(float mine, int K, float *redm, floa
     for (int w = 1; w < kWarps; ++w) {
         m = fmaxf(m, redm[w]);
         bound = fmaxf(bound, redk[w]);
+    }
+    if (K <= 8) {  // 64 values, two a lane
+        uint32_t a = (lane & 7) < K ? drawn[lane] : 0u, b = (lane & 7) < K ? drawn[lane + 32] : 0u;
+        for (int k = 0; k < K; ++k) {
+            kth = __reduce_max_sync(all, a > b ? a : b);
+            if (a == kth) a = 0;
+            if (b == kth) b = 0;
+        }
+        bound = kth ? unordered(kth) : -INFINITY;
+        __syncthreads();  // the list's memory is free
     }
 }
 
