@@ -1,8 +1,11 @@
-// Decay attention (linear attention with a decay for each head): the walk over a row's tokens on FP32
-// CUDA cores, the sum of shared heads' gradients, and the C entry points.
+// Decay attention (linear attention with a decay for each head): the walk over a row's tokens for FP32 operands
+// and for BF16 ones that TMA cannot address, the sum of shared heads' gradients, and the C entry points.
 //
-// The walk's mathematics is in decay_walk.cuh.  This kernel takes every type and stride: operands are
-// widened to FP32 in shared memory and all products, sums and states are FP32.
+// The walk's mathematics is in decay_walk.cuh.  Operands are widened to FP32 in shared memory.  Every product
+// a b runs on the tensor cores as three TF32 products, a1 b1 + a1 b2 + a2 b1 with a = a1 + a2 + r, |r| <= 2^-22 |a|
+// (the method of splitting an operand into its rounding and the remainder), summed in FP32: about 3e-7 beside
+// FP32's own 1e-7, where plain TF32 gives 5e-4.  Sums and states are FP32.  (On FP32 FMAs, with the same tiles,
+// 2 x 4096 tokens x 16 heads of 128 took 708 us.)
 #include "decay_walk.cuh"
 
 #include <mutex>
@@ -15,12 +18,50 @@ using namespace walk;
 constexpr int kThreads = 256;
 constexpr int kCols = 64;  // columns of c per CTA
 
-// Shared memory (floats): A, B [64][wab+4], Cc [64][64], P [64][68], S [wab][64], powers [65].
-int simt_smem(int wab, bool state_only) {
-    const int pitch = ((wab + 3) & ~3) + 4;
-    int f = kChunk * pitch + kChunk * kCols + kChunk + 4;
-    if (!state_only) f += kChunk * pitch + kChunk * (kChunk + 4) + ((wab + 3) & ~3) * kCols;
+constexpr int kColPitch = kCols + 8;    // C, S: 8 banks from row to row
+constexpr int kScorePitch = kChunk + 4;  // P (as A, B): 4 banks
+__host__ __device__ constexpr int walk_width(int wab) { return (wab + 15) & ~15; }
+
+// Shared memory (floats): B [64][w+4], C [64][72], powers [68], A [64][w+4], P [64][68], S [w][72].
+int walk_smem(int wab, bool state_only) {
+    const int w = walk_width(wab), pitch = w + 4;
+    int f = kChunk * pitch + kChunk * kColPitch + kChunk + 4;
+    if (!state_only) f += kChunk * pitch + kChunk * kScorePitch + w * kColPitch;
     return f * 4;
+}
+
+// x = big + small, both TF32 operands (the tensor core drops the bits of `small` past TF32's).
+struct Split32 {
+    uint32_t big, small;
+};
+__device__ __forceinline__ Split32 split32(float x) {
+    Split32 s;
+    asm("cvt.rna.tf32.f32 %0, %1;\n" : "=r"(s.big) : "f"(x));
+    s.small = __float_as_uint(x - __uint_as_float(s.big));
+    return s;
+}
+__device__ __forceinline__ void mma_tf32(float (&d)[4], const uint32_t (&a)[4], uint32_t b0, uint32_t b1) {
+    asm volatile(
+        "mma.sync.aligned.m16n8k8.row.col.f32.tf32.tf32.f32 {%0, %1, %2, %3}, {%4, %5, %6, %7}, {%8, %9}, {%0, %1, %2, %3};\n"
+        : "+f"(d[0]), "+f"(d[1]), "+f"(d[2]), "+f"(d[3])
+        : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
+}
+// d[n] += a (16 x 8) b (8 x 8, columns 8 n), n < 4.  a(i): element i of this lane's fragment (rows g, g + 8, then
+// the same rows 4 columns on); b(n, i): element i of tile n (rows t, t + 4).  g = lane / 4, t = lane % 4.
+template <typename FA, typename FB> __device__ __forceinline__ void mma_step(float (&d)[4][4], FA a, FB b) {
+    uint32_t big[4], small[4];
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+        const Split32 s = split32(a(i));
+        big[i] = s.big, small[i] = s.small;
+    }
+#pragma unroll
+    for (int n = 0; n < 4; ++n) {
+        const Split32 b0 = split32(b(n, 0)), b1 = split32(b(n, 1));
+        mma_tf32(d[n], small, b0.big, b1.big);
+        mma_tf32(d[n], big, b0.small, b1.small);
+        mma_tf32(d[n], big, b0.big, b1.big);
+    }
 }
 
 // Rows [t0, t0 + 64) of one head into shared memory as FP32; invalid rows and columns are zero.  A warp takes
@@ -46,7 +87,8 @@ __device__ __forceinline__ void load_rows(float *dst, int pitch, const T *src, i
     }
 }
 
-// One CTA walks one segment of one (row, head) for 64 columns of c.
+// One CTA walks one segment of one (row, head) for 64 columns of c.  Warp tiles are 16 x 32: P and the outputs
+// have 4 x 2, one a warp; the state has up to 8 x 2, warp w has tiles w and w + 8.
 template <typename T, typename OT, bool STATE_ONLY>
 __global__ void __launch_bounds__(kThreads) decay_walk_kernel(const Params p) {
     extern __shared__ float sm[];
@@ -60,15 +102,15 @@ __global__ void __launch_bounds__(kThreads) decay_walk_kernel(const Params p) {
     const int64_t bh = id / slices;
     const int64_t b = bh / p.heads;
     const int h = (int)(bh % p.heads);
-    const int wk = (p.wab + 3) & ~3, pitch = wk + 4;
+    const int width = walk_width(p.wab), pitch = width + 4;
     const int n0 = slice * kCols;
 
     float *sB = sm;
     float *sC = sB + kChunk * pitch;
-    float *pw = sC + kChunk * kCols;  // lam^0 .. lam^64
+    float *pw = sC + kChunk * kColPitch;  // lam^0 .. lam^64
     float *sA = pw + kChunk + 4;
     float *sP = sA + kChunk * pitch;
-    float *sS = sP + kChunk * (kChunk + 4);
+    float *sS = sP + kChunk * kScorePitch;
 
     const float g = head_log_decay(p, h);
     for (int i = threadIdx.x; i <= kChunk; i += kThreads) pw[i] = i ? expf(g * (float)i) : 1.f;
@@ -76,33 +118,48 @@ __global__ void __launch_bounds__(kThreads) decay_walk_kernel(const Params p) {
     if (!STATE_ONLY && p.nseg > 1) asm volatile("griddepcontrol.wait;\n" ::: "memory");
 
     const Span sp = span_of(p, row_tokens(p, b), seg);
-    const int tx = threadIdx.x % 16, ty = threadIdx.x / 16;
+    const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, lg = lane >> 2, lt = lane & 3;
+    const int mrow = (warp & 3) * 16, ncol = (warp >> 2) * 32;  // this warp's tile of P and of the outputs
     const T *a = static_cast<const T *>(p.a) + b * p.as[0] + (h / p.ag) * p.as[2];
     const T *bb = static_cast<const T *>(p.b) + b * p.bs[0] + (h / p.bg) * p.bs[2];
     const T *c = static_cast<const T *>(p.c) + b * p.cs[0] + (h / p.cg) * p.cs[2];
     OT *out = static_cast<OT *>(p.out) + b * p.os[0] + h * p.os[2];
-
-    // state elements (ty + 16 r, n0 + 4 tx + e) in registers
     const int64_t size = (int64_t)p.wab * p.wc;
-    const bool before = !STATE_ONLY && p.nseg > 1 && (p.reverse ? seg < p.nseg - 1 : seg > 0);
-    float given = 0.f;
-    if (!STATE_ONLY && p.state_in) {
-        const int64_t end = sp.c1 * kChunk < sp.n ? sp.c1 * kChunk : sp.n;
-        const int64_t far = p.reverse ? sp.n - end : sp.c0 * kChunk;
-        given = (far ? expf(g * (float)far) : 1.f) * p.in_mul;
-    }
-    float S[8][4];
-#pragma unroll
-    for (int r = 0; r < 8; ++r)
-#pragma unroll
-        for (int e = 0; e < 4; ++e) {
-            const int i = ty + 16 * r, j = n0 + 4 * tx + e;
-            S[r][e] = 0.f;
-            if (i >= p.wab || j >= p.wc) continue;
-            if (before) S[r][e] = p.seg[(bh * p.nseg + seg) * size + (int64_t)i * p.wc + j];
-            if (!STATE_ONLY && p.state_in)
-                S[r][e] = fmaf(given, p.state_in[bh * size + (p.in_t ? (int64_t)j * p.wab + i : (int64_t)i * p.wc + j)], S[r][e]);
+
+    // state tile q: rows srow(q) + lg (+ 8), columns scol(q) + 8 n + 2 lt + {0, 1}; element (n, i) is row lg + 8 (i / 2)
+    const int stiles = width / 8;
+    auto srow = [&](int q) { return (warp + 8 * q) / 2 * 16; };
+    auto scol = [&](int q) { return (warp + 8 * q) % 2 * 32; };
+    float S[2][4][4];
+    {
+        const bool before = !STATE_ONLY && p.nseg > 1 && (p.reverse ? seg < p.nseg - 1 : seg > 0);
+        const float *zs = before ? p.seg + (bh * p.nseg + seg) * size : nullptr;
+        const float *x = !STATE_ONLY && p.state_in ? p.state_in + bh * size : nullptr;
+        float given = 0.f;
+        if (x) {
+            const int64_t end = sp.c1 * kChunk < sp.n ? sp.c1 * kChunk : sp.n;
+            const int64_t far = p.reverse ? sp.n - end : sp.c0 * kChunk;
+            given = (far ? expf(g * (float)far) : 1.f) * p.in_mul;
         }
+#pragma unroll
+        for (int q = 0; q < 2; ++q)
+#pragma unroll
+            for (int n = 0; n < 4; ++n)
+#pragma unroll
+                for (int i = 0; i < 4; ++i) {
+                    const int k = srow(q) + lg + 8 * (i >> 1), v = n0 + scol(q) + 8 * n + 2 * lt + (i & 1);
+                    const bool in = k < p.wab && v < p.wc;
+                    S[q][n][i] = 0.f;
+                    if (zs) {
+                        const float f = zs[in ? k * p.wc + v : 0];
+                        S[q][n][i] = in ? f : 0.f;
+                    }
+                    if (x) {
+                        const float f = x[in ? (p.in_t ? v * p.wab + k : k * p.wc + v) : 0];
+                        S[q][n][i] = in ? fmaf(given, f, S[q][n][i]) : 0.f;
+                    }
+                }
+    }
 
     for (int64_t step = 0; step < sp.c1 - sp.c0; ++step) {
         const int64_t ch = p.reverse ? sp.c1 - 1 - step : sp.c0 + step;
@@ -110,123 +167,114 @@ __global__ void __launch_bounds__(kThreads) decay_walk_kernel(const Params p) {
         const int valid = (int)(sp.n - t0 < kChunk ? sp.n - t0 : kChunk);
         __syncthreads();  // the tiles of the previous chunk are done with
         if (!STATE_ONLY) {
-            load_rows<T>(sA, pitch, a, p.as[1], t0, valid, 0, p.wab, wk);
+            load_rows<T>(sA, pitch, a, p.as[1], t0, valid, 0, p.wab, width);
 #pragma unroll
-            for (int r = 0; r < 8; ++r)
-                if (ty + 16 * r < wk) *reinterpret_cast<float4 *>(&sS[(ty + 16 * r) * kCols + 4 * tx]) =
-                    make_float4(S[r][0], S[r][1], S[r][2], S[r][3]);
+            for (int q = 0; q < 2; ++q)
+                if (warp + 8 * q < stiles)
+#pragma unroll
+                    for (int n = 0; n < 4; ++n)
+#pragma unroll
+                        for (int i = 0; i < 4; i += 2)
+                            *reinterpret_cast<float2 *>(&sS[(srow(q) + lg + 4 * i) * kColPitch + scol(q) + 8 * n + 2 * lt]) =
+                                make_float2(S[q][n][i], S[q][n][i + 1]);
         }
-        load_rows<T>(sB, pitch, bb, p.bs[1], t0, valid, 0, p.wab, wk);
-        load_rows<T>(sC, kCols, c, p.cs[1], t0, valid, n0, p.wc, kCols);
+        load_rows<T>(sB, pitch, bb, p.bs[1], t0, valid, 0, p.wab, width);
+        load_rows<T>(sC, kColPitch, c, p.cs[1], t0, valid, n0, p.wc, kCols);
         __syncthreads();
 
         if (!STATE_ONLY) {
-            // P = (A B^T) with the decay between the rows; rows ty + 16 r, columns tx + 16 q
-            float acc[4][4] = {};
-            for (int k = 0; k < wk; k += 4) {
-                float4 x[4], y[4];
-#pragma unroll
-                for (int r = 0; r < 4; ++r) x[r] = *reinterpret_cast<const float4 *>(&sA[(ty + 16 * r) * pitch + k]);
-#pragma unroll
-                for (int q = 0; q < 4; ++q) y[q] = *reinterpret_cast<const float4 *>(&sB[(tx + 16 * q) * pitch + k]);
-#pragma unroll
-                for (int r = 0; r < 4; ++r)
-#pragma unroll
-                    for (int q = 0; q < 4; ++q)
-                        acc[r][q] += x[r].x * y[q].x + x[r].y * y[q].y + x[r].z * y[q].z + x[r].w * y[q].w;
+            // P = A B^T with the decay between the rows; tiles that the mask empties are only cleared
+            float d[4][4] = {};
+            if (p.reverse ? ncol + 31 >= mrow : ncol <= mrow + 15) {
+                const float *fa = sA + (mrow + lg) * pitch + lt, *fb = sB + (ncol + lg) * pitch + lt;
+#pragma unroll 2
+                for (int k = 0; k < width; k += 8)
+                    mma_step(d, [&](int i) { return fa[(i & 1) * 8 * pitch + (i >> 1) * 4 + k]; },
+                             [&](int n, int i) { return fb[n * 8 * pitch + i * 4 + k]; });
             }
 #pragma unroll
-            for (int r = 0; r < 4; ++r)
+            for (int n = 0; n < 4; ++n)
 #pragma unroll
-                for (int q = 0; q < 4; ++q) {
-                    const int i = ty + 16 * r, j = tx + 16 * q;
-                    const int d = p.reverse ? j - i : i - j;
-                    sP[i * (kChunk + 4) + j] = d >= 0 ? acc[r][q] * pw[d] : 0.f;
+                for (int i = 0; i < 4; i += 2) {
+                    const int r = mrow + lg + 4 * i, j = ncol + 8 * n + 2 * lt;
+                    const int e0 = p.reverse ? j - r : r - j, e1 = p.reverse ? e0 + 1 : e0 - 1;
+                    *reinterpret_cast<float2 *>(&sP[r * kScorePitch + j]) =
+                        make_float2(e0 >= 0 ? d[n][i] * pw[e0] : 0.f, e1 >= 0 ? d[n][i + 1] * pw[e1] : 0.f);
                 }
             __syncthreads();
-            // out = scale * (P C + lam^. A S); rows ty + 16 r, columns 4 tx .. 4 tx + 3
+            // out = scale * (lam^. A S + P C)
             float o[4][4] = {};
-            for (int k = 0; k < wk; k += 4) {
-                float4 x[4], y[4];
-#pragma unroll
-                for (int r = 0; r < 4; ++r) x[r] = *reinterpret_cast<const float4 *>(&sA[(ty + 16 * r) * pitch + k]);
-#pragma unroll
-                for (int q = 0; q < 4; ++q) y[q] = *reinterpret_cast<const float4 *>(&sS[(k + q) * kCols + 4 * tx]);
-#pragma unroll
-                for (int r = 0; r < 4; ++r) {
-                    o[r][0] += x[r].x * y[0].x + x[r].y * y[1].x + x[r].z * y[2].x + x[r].w * y[3].x;
-                    o[r][1] += x[r].x * y[0].y + x[r].y * y[1].y + x[r].z * y[2].y + x[r].w * y[3].y;
-                    o[r][2] += x[r].x * y[0].z + x[r].y * y[1].z + x[r].z * y[2].z + x[r].w * y[3].z;
-                    o[r][3] += x[r].x * y[0].w + x[r].y * y[1].w + x[r].z * y[2].w + x[r].w * y[3].w;
-                }
+            {
+                const float *fa = sA + (mrow + lg) * pitch + lt, *fs = sS + lt * kColPitch + ncol + lg;
+#pragma unroll 2
+                for (int k = 0; k < width; k += 8)
+                    mma_step(o, [&](int i) { return fa[(i & 1) * 8 * pitch + (i >> 1) * 4 + k]; },
+                             [&](int n, int i) { return fs[(k + i * 4) * kColPitch + n * 8]; });
             }
 #pragma unroll
-            for (int r = 0; r < 4; ++r) {
-                const int i = ty + 16 * r;
-                const int e = p.reverse ? valid - 1 - i : i + 1;
+            for (int i = 0; i < 4; ++i) {
+                const int r = mrow + lg + 8 * (i >> 1);
+                const int e = p.reverse ? valid - 1 - r : r + 1;
                 const float w = e >= 0 ? pw[e] : 0.f;
 #pragma unroll
-                for (int q = 0; q < 4; ++q) o[r][q] *= w;
+                for (int n = 0; n < 4; ++n) o[n][i] *= w;
             }
-            for (int j = 0; j < kChunk; j += 4) {
-                float4 x[4], y[4];
+            {
+                const float *fp = sP + (mrow + lg) * kScorePitch + lt, *fc = sC + lt * kColPitch + ncol + lg;
+                const int k0 = p.reverse ? mrow : 0, k1 = p.reverse ? kChunk : mrow + 16;  // outside, P is zero
+#pragma unroll 2
+                for (int k = k0; k < k1; k += 8)
+                    mma_step(o, [&](int i) { return fp[(i & 1) * 8 * kScorePitch + (i >> 1) * 4 + k]; },
+                             [&](int n, int i) { return fc[(k + i * 4) * kColPitch + n * 8]; });
+            }
 #pragma unroll
-                for (int r = 0; r < 4; ++r) x[r] = *reinterpret_cast<const float4 *>(&sP[(ty + 16 * r) * (kChunk + 4) + j]);
+            for (int n = 0; n < 4; ++n)
 #pragma unroll
-                for (int q = 0; q < 4; ++q) y[q] = *reinterpret_cast<const float4 *>(&sC[(j + q) * kCols + 4 * tx]);
-#pragma unroll
-                for (int r = 0; r < 4; ++r) {
-                    o[r][0] += x[r].x * y[0].x + x[r].y * y[1].x + x[r].z * y[2].x + x[r].w * y[3].x;
-                    o[r][1] += x[r].x * y[0].y + x[r].y * y[1].y + x[r].z * y[2].y + x[r].w * y[3].y;
-                    o[r][2] += x[r].x * y[0].z + x[r].y * y[1].z + x[r].z * y[2].z + x[r].w * y[3].z;
-                    o[r][3] += x[r].x * y[0].w + x[r].y * y[1].w + x[r].z * y[2].w + x[r].w * y[3].w;
+                for (int i = 0; i < 4; ++i) {
+                    const int r = mrow + lg + 8 * (i >> 1), j = n0 + ncol + 8 * n + 2 * lt + (i & 1);
+                    if (t0 + r < p.time && j < p.wc)
+                        out[(t0 + r) * p.os[1] + j] = Elem<OT>::from_float(r < valid ? p.scale * o[n][i] : 0.f);
                 }
-            }
-#pragma unroll
-            for (int r = 0; r < 4; ++r) {
-                const int i = ty + 16 * r;
-                if (t0 + i >= p.time) continue;
-#pragma unroll
-                for (int q = 0; q < 4; ++q) {
-                    const int j = n0 + 4 * tx + q;
-                    if (j < p.wc)
-                        out[(t0 + i) * p.os[1] + j] = Elem<OT>::from_float(i < valid ? p.scale * o[r][q] : 0.f);
-                }
-            }
         }
         // S = lam^valid S + sum_j lam^. b_j c_j, where anyone asks for it
         if (!STATE_ONLY && step + 1 == sp.c1 - sp.c0 && !(p.state_out && sp.last)) break;
         const float carry = pw[valid];
 #pragma unroll
-        for (int r = 0; r < 8; ++r)
+        for (int q = 0; q < 2; ++q) {
+            if (warp + 8 * q >= stiles) continue;
 #pragma unroll
-            for (int e = 0; e < 4; ++e) S[r][e] *= carry;
-        for (int j = 0; j < valid; ++j) {
-            float4 y = *reinterpret_cast<const float4 *>(&sC[j * kCols + 4 * tx]);
-            const float w = pw[p.reverse ? j + 1 : valid - 1 - j];
-            y.x *= w, y.y *= w, y.z *= w, y.w *= w;
+            for (int n = 0; n < 4; ++n)
 #pragma unroll
-            for (int r = 0; r < 8; ++r) {
-                if (ty + 16 * r >= wk) continue;
-                const float x = sB[j * pitch + ty + 16 * r];
-                S[r][0] += x * y.x, S[r][1] += x * y.y, S[r][2] += x * y.z, S[r][3] += x * y.w;
+                for (int i = 0; i < 4; ++i) S[q][n][i] *= carry;
+            const float *fb = sB + lt * pitch + srow(q) + lg, *fc = sC + lt * kColPitch + scol(q) + lg;
+            for (int k = 0; k < valid; k += 8) {  // rows past `valid` are zero
+                float w[2];
+#pragma unroll
+                for (int i = 0; i < 2; ++i) {
+                    const int e = p.reverse ? k + lt + 4 * i + 1 : valid - 1 - (k + lt + 4 * i);
+                    w[i] = pw[e < 0 ? 0 : e];
+                }
+                mma_step(S[q], [&](int i) { return fb[(k + (i >> 1) * 4) * pitch + (i & 1) * 8]; },
+                         [&](int n, int i) { return w[i] * fc[(k + i * 4) * kColPitch + n * 8]; });
             }
         }
     }
 
     if (STATE_ONLY || (p.state_out && sp.last)) {
+        float *z = STATE_ONLY ? p.seg + (bh * segs + zid) * size : p.state_out + bh * size;
 #pragma unroll
-        for (int r = 0; r < 8; ++r)
+        for (int q = 0; q < 2; ++q)
 #pragma unroll
-            for (int e = 0; e < 4; ++e) {
-                const int i = ty + 16 * r, j = n0 + 4 * tx + e;
-                if (i >= p.wab || j >= p.wc) continue;
-                if (STATE_ONLY)
-                    p.seg[(bh * segs + zid) * size + (int64_t)i * p.wc + j] = S[r][e];
-                else
-                    p.state_out[bh * size + (p.out_t ? (int64_t)j * p.wab + i : (int64_t)i * p.wc + j)] =
-                        S[r][e] * p.out_mul;
-            }
+            for (int n = 0; n < 4; ++n)
+#pragma unroll
+                for (int i = 0; i < 4; ++i) {
+                    const int k = srow(q) + lg + 8 * (i >> 1), v = n0 + scol(q) + 8 * n + 2 * lt + (i & 1);
+                    if (warp + 8 * q >= stiles || k >= p.wab || v >= p.wc) continue;
+                    if (STATE_ONLY)
+                        z[k * p.wc + v] = S[q][n][i];
+                    else
+                        z[p.out_t ? v * p.wab + k : k * p.wc + v] = S[q][n][i] * p.out_mul;
+                }
     }
     if (!STATE_ONLY) {
         // rows of whole chunks past the row's length
@@ -235,8 +283,8 @@ __global__ void __launch_bounds__(kThreads) decay_walk_kernel(const Params p) {
         if (z0 < s0) z0 = s0;
         if (z1 > s1) z1 = s1;
         const int cols = p.wc - n0 < kCols ? p.wc - n0 : kCols;
-        for (int64_t i = threadIdx.x; i < (z1 - z0) * cols; i += kThreads)
-            out[(z0 + i / cols) * p.os[1] + n0 + i % cols] = Elem<OT>::from_float(0.f);
+        for (int64_t t = z0 + warp; t < z1; t += kThreads / 32)
+            for (int j = lane; j < cols; j += 32) out[t * p.os[1] + n0 + j] = Elem<OT>::from_float(0.f);
     }
 }
 
@@ -304,7 +352,7 @@ int device_setup(int &sms) {
             (const void *)decay_walk_kernel<bf16, bf16, true>};
         for (const void *f : fns)
             if (int rc = cuda_status(cudaFuncSetAttribute(f, cudaFuncAttributeMaxDynamicSharedMemorySize,
-                                                          simt_smem(kMaxWidth, false))))
+                                                          walk_smem(kMaxWidth, false))))
                 return rc;
         if (int rc = cuda_status(cudaDeviceGetAttribute(&g_sms[dev], cudaDevAttrMultiProcessorCount, dev))) return rc;
         g_attr[dev] = true;
@@ -314,7 +362,7 @@ int device_setup(int &sms) {
 }
 
 // The state launch, the prefix launch and the walk; each start overlaps the end of the one before.
-template <typename T, typename OT> int simt_launch(Params p, void *workspace, cudaStream_t st) {
+template <typename T, typename OT> int walk_launch(Params p, void *workspace, cudaStream_t st) {
     const int64_t rows = p.batch * p.heads, slices = ceil_div(p.wc, kCols), size = (int64_t)p.wab * p.wc;
     if (rows * slices * p.nseg > 0x7fffffff) return BDM_ERR_UNSUPPORTED;
     cudaLaunchConfig_t cfg{};
@@ -330,21 +378,21 @@ template <typename T, typename OT> int simt_launch(Params p, void *workspace, cu
         Params q = p;
         q.seg = z;
         cfg.gridDim = dim3((unsigned)(rows * slices * (p.nseg - 1)));
-        cfg.dynamicSmemBytes = simt_smem(p.wab, true);
+        cfg.dynamicSmemBytes = walk_smem(p.wab, true);
         if (int rc = cuda_status(cudaLaunchKernelEx(&cfg, decay_walk_kernel<T, T, true>, (const Params)q))) return rc;
         if (int rc = launch_status()) return rc;
         if (int rc = decay_prefix_launch(p, z, 1, p.cps, st)) return rc;
         cfg.numAttrs = 1;
     }
     cfg.gridDim = dim3((unsigned)(rows * slices * p.nseg));
-    cfg.dynamicSmemBytes = simt_smem(p.wab, false);
+    cfg.dynamicSmemBytes = walk_smem(p.wab, false);
     if (int rc = cuda_status(cudaLaunchKernelEx(&cfg, decay_walk_kernel<T, OT, false>, (const Params)p))) return rc;
     return launch_status();
 }
 
-// Segments of the time axis for the CUDA-core walk: three CTAs per SM, down to a chunk each.  A segment more
+// Segments of the time axis for this walk: three CTAs per SM, down to a chunk each.  A segment more
 // costs a second pass over its b and c and half of a chunk's arithmetic, so rows that fill the GPU stay whole.
-int64_t simt_segments(int64_t ctas, int64_t chunks, int sms) {
+int64_t walk_segments(int64_t ctas, int64_t chunks, int sms) {
     if (ctas >= 2 * sms) return 1;
     const int64_t s = 3 * sms / ctas;
     return s > chunks ? chunks : s;
@@ -379,7 +427,7 @@ int plan(const bdm_decay_walk_args &w, Params &p, Split &split, int sms) {
     if (split.tc) {
         decay_walk_tc_split(w.batch * w.heads, chunks, sms, p.nseg, p.cps, split.sub, split.scps);
     } else {
-        const int64_t nseg = simt_segments(w.batch * w.heads * ceil_div(w.width_c, kCols), chunks, sms);
+        const int64_t nseg = walk_segments(w.batch * w.heads * ceil_div(w.width_c, kCols), chunks, sms);
         p.cps = (int)ceil_div(chunks, nseg);
         p.nseg = (int)ceil_div(chunks, p.cps);
     }
@@ -449,9 +497,9 @@ extern "C" int bdm_decay_walk(const bdm_decay_walk_args *w, void *workspace, int
     if (need > workspace_bytes || (need && !workspace)) return BDM_ERR_WORKSPACE;
     cudaStream_t st = as_stream(stream);
     if (split.tc) return decay_walk_tc_launch(*w, p, split.sub, split.scps, workspace, st);
-    if (w->dtype == BDM_F32) return simt_launch<float, float>(p, workspace, st);
-    if (w->out_dtype == BDM_F32) return simt_launch<bf16, float>(p, workspace, st);
-    return simt_launch<bf16, bf16>(p, workspace, st);
+    if (w->dtype == BDM_F32) return walk_launch<float, float>(p, workspace, st);
+    if (w->out_dtype == BDM_F32) return walk_launch<bf16, float>(p, workspace, st);
+    return walk_launch<bf16, bf16>(p, workspace, st);
 }
 
 extern "C" int bdm_decay_group_sum(const float *part, int64_t tokens, int groups, int group, int width, int dtype, void *out,
