@@ -197,12 +197,11 @@ __device__ __forceinline__ void finish_slice(float warp_total, float fix, float 
     if (threadIdx.x < K) dst[threadIdx.x] = sh.best[threadIdx.x];
 }
 
-// One pass over the logits, E per thread in registers: the maximum, then the sum, then the few
-// candidates: the K-th largest of one warp's lane maxima bounds the K-th largest of the slice from below, and the
-// logits at or above the largest such bound (a few times K) go to a list and are ranked there; when the list
-// overflows, K rounds of a CTA-wide maximum take its place.  Bound by HBM where the batch fills the
-// GPU; what it costs beside the load is about 7 instructions per logit (exp as one multiplication and
-// ex2.approx, off by 2^-22 and by |x - max| 2^-24 for terms that are exp(x - max) small).
+// One pass over the logits, E per thread in registers: the maximum, then the sum of exp(x - max) (one
+// multiplication and ex2.approx: off by 2^-22, and by |x - max| 2^-24 for terms that are exp(x - max) small),
+// then the few candidates: the logits at or above slice_bound's bound go to a list and are ranked there; when
+// the list overflows, K rounds of a CTA-wide maximum take its place.  HBM is the floor (5 us for 64 x 8 x 32000
+// BF16), instructions the bound: about 10 per logit and 300 per warp, 14 us.
 // VECTOR: rows start on 16-byte boundaries.
 template <typename T, int E, bool VECTOR>
 __global__ void __launch_bounds__(kThreads)
@@ -359,8 +358,9 @@ __device__ __forceinline__ float candidate(const Row &r, float logit) {
     return c == c ? c : -INFINITY;  // NaN ranks as -inf
 }
 
-// One CTA per batch row: joins the rows' softmax sums, ranks their candidates by (value, lower flat
-// index) and writes the new beams.
+// One CTA per batch row: joins the rows' softmax sums and ranks each row's candidates by (value, lower flat
+// index), a warp for a row, then ranks the rows' against one another by counting and writes the new beams.
+// Latency is all it costs (about 5 us), so its start overlaps the slices' end.
 template <typename T>
 __global__ void __launch_bounds__(kThreads)
     beam_merge_kernel(const T *__restrict__ logits, int64_t ld, const float *__restrict__ scores,
@@ -560,7 +560,8 @@ struct Tensors {
 constexpr int kUnroll = 4;  // columns a thread moves at a time
 
 // In place: each thread owns columns of one group's rows and reads all of them that move before it writes
-// any, so permutations and copies need no second buffer.
+// any, so permutations and copies need no second buffer, and rows that stay cost nothing.  Bound by HBM: 16
+// groups of 4 rows of 12.6 MB, half of them moved, take 129 us (123 at the copy rate), all of them 241 (246);
 template <typename U, int W>
 __global__ void __launch_bounds__(kThreads)
     reorder_rows_kernel(const Tensors t, const int64_t *__restrict__ parents, int beams, int64_t groups, int *status) {
@@ -604,26 +605,66 @@ __global__ void __launch_bounds__(kThreads)
     }
 }
 
+// The same for more than 16 beams, whose columns would take all of a thread's registers: the rows that move pass
+// through shared memory, 1 KB of each at a time (2 groups of 32 rows of 12.6 MB, half of them moved: 156 us, from
+// registers 217; 4 groups of 16: 178, from registers in 8-byte columns 133).
+constexpr int kTileUnits = 64;
+__global__ void __launch_bounds__(kThreads)
+    reorder_tiles_kernel(const Tensors t, const int64_t *__restrict__ parents, int beams, int64_t groups, int *status) {
+    __shared__ uint4 tile[kMaxBeams][kTileUnits];
+    __shared__ int src[kMaxBeams];
+    int k = 0;
+    while (k + 1 < t.count && (int64_t)blockIdx.x >= t.first[k + 1]) ++k;
+    const int64_t at = blockIdx.x - t.first[k];
+    const int64_t group = at % groups, unit = at / groups * kTileUnits + threadIdx.x % kTileUnits;
+    if (threadIdx.x < beams) {
+        const int64_t s = parents[group * beams + threadIdx.x];
+        const bool in = s >= 0 && s < beams;
+        src[threadIdx.x] = in ? (int)s : (int)threadIdx.x;
+        if (!in && status) *(volatile int *)status = 0x8;  // the row keeps its state
+    }
+    __syncthreads();
+    char *base = static_cast<char *>(t.base[k]) + group * beams * t.stride[k] + unit * 16;
+    const int64_t stride = t.stride[k];
+    constexpr int kStep = kThreads / kTileUnits;
+    const int row = threadIdx.x / kTileUnits, u = threadIdx.x % kTileUnits;
+    if (unit < t.units[k])
+#pragma unroll 8
+        for (int i = row; i < beams; i += kStep)
+            if (src[i] != i) tile[i][u] = *reinterpret_cast<const uint4 *>(base + src[i] * stride);
+    __syncthreads();
+    if (unit < t.units[k])
+#pragma unroll 8
+        for (int i = row; i < beams; i += kStep)
+            if (src[i] != i) *reinterpret_cast<uint4 *>(base + i * stride) = tile[i][u];
+}
+
 template <typename U>
 int reorder_launch(Tensors t, const int64_t *row_bytes, const int64_t *parents, int64_t groups, int beams, int *status,
                    cudaStream_t st) {
+    const bool tiled = sizeof(U) == 16 && beams > 16;
     int64_t tiles = 0;
     for (int i = 0; i < t.count; ++i) {
         t.units[i] = row_bytes[i] / (int64_t)sizeof(U);
         t.first[i] = tiles;
-        tiles += groups * ceil_div(t.units[i], kThreads * kUnroll);
+        tiles += groups * ceil_div(t.units[i], tiled ? kTileUnits : kThreads * kUnroll);
     }
     t.first[t.count] = tiles;
     if (tiles > 0x7fffffff) return BDM_ERR_UNSUPPORTED;
     if (tiles == 0) return BDM_OK;
-    if (beams <= 4)
-        reorder_rows_kernel<U, 4><<<(unsigned)tiles, kThreads, 0, st>>>(t, parents, beams, groups, status);
+    const unsigned grid = (unsigned)tiles;
+    if (tiled)
+        reorder_tiles_kernel<<<grid, kThreads, 0, st>>>(t, parents, beams, groups, status);
+    else if (beams <= 4)
+        reorder_rows_kernel<U, 4><<<grid, kThreads, 0, st>>>(t, parents, beams, groups, status);
     else if (beams <= 8)
-        reorder_rows_kernel<U, 8><<<(unsigned)tiles, kThreads, 0, st>>>(t, parents, beams, groups, status);
-    else if (beams <= 16 || sizeof(U) == 16)  // 16-byte columns of 32 rows would not fit the registers
-        reorder_rows_kernel<U, 16><<<(unsigned)tiles, kThreads, 0, st>>>(t, parents, beams, groups, status);
-    else if constexpr (sizeof(U) < 16)
-        reorder_rows_kernel<U, 32><<<(unsigned)tiles, kThreads, 0, st>>>(t, parents, beams, groups, status);
+        reorder_rows_kernel<U, 8><<<grid, kThreads, 0, st>>>(t, parents, beams, groups, status);
+    else if constexpr (sizeof(U) < 16) {
+        if (beams <= 16)
+            reorder_rows_kernel<U, 16><<<grid, kThreads, 0, st>>>(t, parents, beams, groups, status);
+        else if constexpr (sizeof(U) < 8)
+            reorder_rows_kernel<U, 32><<<grid, kThreads, 0, st>>>(t, parents, beams, groups, status);
+    }
     return launch_status();
 }
 
@@ -690,7 +731,7 @@ extern "C" int bdm_reorder_rows(void *const *bases, const int64_t *row_strides, 
     for (int i = 0; i < count; ++i)
         if (row_bytes[i] < 0 || row_strides[i] < row_bytes[i] || (row_bytes[i] && !bases[i])) return BDM_ERR_INVALID;
     cudaStream_t st = as_stream(stream);
-    for (int width : {16, 8, 4, 1}) {  // the widest access each tensor's rows allow, 8 bytes at most past 16 beams
+    for (int width : {16, 8, 4, 1}) {  // the access that a tensor's rows allow
         Tensors t{};
         int64_t bytes[kMaxTensors];
         auto flush = [&]() {
@@ -704,7 +745,8 @@ extern "C" int bdm_reorder_rows(void *const *bases, const int64_t *row_strides, 
         };
         for (int i = 0; i < count; ++i) {
             const uint64_t bits = reinterpret_cast<uintptr_t>(bases[i]) | (uint64_t)row_strides[i] | (uint64_t)row_bytes[i];
-            const int fits = bits % 16 == 0 && beams <= 16 ? 16 : (bits % 8 == 0 ? 8 : (bits % 4 == 0 ? 4 : 1));
+            // 16 bytes, but 8 where the registers are to hold 9 to 16 rows' columns; tensors of odd sizes 4 or 1
+            const int fits = bits % 16 == 0 ? (beams > 8 && beams <= 16 ? 8 : 16) : (bits % 4 == 0 ? 4 : 1);
             if (fits != width || row_bytes[i] == 0) continue;
             t.base[t.count] = bases[i];
             t.stride[t.count] = row_strides[i];
