@@ -81,9 +81,10 @@ def _group_sum(part, kv_heads, dtype):
     return out
 
 
-def _forward(q, k, v, log_decay, initial_state, lengths, scale):
+def _forward(q, k, v, log_decay, initial_state, lengths, scale, want_state):
     heads = q.shape[2]
-    state = torch.empty((q.shape[0], heads, q.shape[3], v.shape[3]), dtype=torch.float32, device=q.device)
+    state = torch.empty((q.shape[0], heads, q.shape[3], v.shape[3]), dtype=torch.float32,
+                        device=q.device) if want_state else None
     with _on(q.device):
         out = _walk(q, k, v, log_decay, lengths, ops._scan_status_of(q.device), heads=heads, scale=scale,
                     state_in=initial_state, state_out=state)
@@ -92,11 +93,11 @@ def _forward(q, k, v, log_decay, initial_state, lengths, scale):
 
 class _DecayAttention(torch.autograd.Function):
     @staticmethod
-    def forward(ctx, q, k, v, log_decay, initial_state, lengths, scale):
+    def forward(ctx, q, k, v, log_decay, initial_state, lengths, scale, want_state):
         ctx.save_for_backward(q, k, v, log_decay, initial_state, lengths)
         ctx.scale = scale
         ctx.set_materialize_grads(False)
-        return _forward(q, k, v, log_decay, initial_state, lengths, scale)
+        return _forward(q, k, v, log_decay, initial_state, lengths, scale, want_state)
 
     @staticmethod
     @torch.autograd.function.once_differentiable
@@ -104,7 +105,7 @@ class _DecayAttention(torch.autograd.Function):
         q, k, v, log_decay, s0, lengths = ctx.saved_tensors
         scale, heads, kv_heads, dt = ctx.scale, q.shape[2], k.shape[2], q.dtype
         if do is None and dstate is None:
-            return (None,) * 7
+            return (None,) * 8
         do = _rows(do) if do is not None else torch.zeros_like(v[:, :, :1]).expand(-1, -1, heads, -1)
         dstate = dstate.contiguous() if dstate is not None else None
         need = ctx.needs_input_grad
@@ -126,7 +127,7 @@ class _DecayAttention(torch.autograd.Function):
                                   device=q.device) if need[4] else None
                 dv = _walk(k, q, do, log_decay, lengths, st, state_out=ds0, state_out_mul=scale, **back)
                 dv = _group_sum(dv, kv_heads, dt) if shared else dv
-        return dq, dk, dv if need[2] else None, None, ds0, None, None
+        return dq, dk, dv if need[2] else None, None, ds0, None, None, None
 
 
 def _check_heads(q, k, v, log_decay, scale):
@@ -189,7 +190,7 @@ def decay_attention(q, k, v, log_decay, *, scale=None, initial_state=None, lengt
     if torch.is_grad_enabled() and (q.requires_grad or k.requires_grad or v.requires_grad
                                     or (initial_state is not None and initial_state.requires_grad)):
         run = _DecayAttention.apply
-    out, state = run(q, k, v, log_decay, initial_state, lengths, scale)
+    out, state = run(q, k, v, log_decay, initial_state, lengths, scale, return_state)
     return (out, state) if return_state else out
 
 

@@ -140,6 +140,48 @@ def test_broadcast_inputs_and_their_gradients(dtype):
     _near(got, ref, (_tol(dtype) + (U if dtype == torch.bfloat16 else 0)) * mag, 'dk')  # one more rounding: the sum over rows
 
 
+@pytest.mark.parametrize('dtype', [torch.float32, torch.bfloat16])
+@pytest.mark.parametrize('size', [(2, 200, 4, 2, 64, 64), (1, 1100, 2, 2, 128, 128)])
+def test_outputs_alone(size, dtype):
+    """Without the state the BF16 walk rounds what it adds to the carried state to 17 bits, not 24: 2^-9 u A,
+    far inside the bound of the outputs, which stays what it is."""
+    from bdm_b200 import decay_attention
+    q, k, v, do, g, s0, _ = _inputs(16, *size, dtype)
+    leaves = [x.requires_grad_(True) for x in (q, k, v)]
+    o = decay_attention(q, k, v, g, initial_state=s0)
+    got = torch.autograd.grad(o, leaves, do)
+    H, sc, tol = size[2], size[4] ** -0.5, _tol(dtype)
+    n = torch.full((size[0],), size[1], device=DEV)
+    _near(o.detach(), walk(q, k, v, g, n, H, sc, s0)[0], tol * walk(q, k, v, g, n, H, sc, s0, absolute=True)[0], 'o')
+    ref, mag = gradients(q, k, v, do, g, n, sc, s0), gradients(q, k, v, do, g, n, sc, s0, absolute=True)
+    for name, x, y, m in zip(('dq', 'dk', 'dv'), got, ref, mag):
+        _near(x, y, tol * m, name)
+
+
+def test_gradient_through_the_state_alone():
+    from bdm_b200 import decay_attention
+    q, k, v, _, g, s0, ds = _inputs(17, 2, 90, 2, 1, 64, 64, torch.float32)
+    leaves = [x.requires_grad_(True) for x in (k, v, s0)]
+    _, s = decay_attention(q, k, v, g, initial_state=s0, return_state=True)
+    got = torch.autograd.grad(s, leaves, ds)
+    n, zero = torch.full((2,), 90, device=DEV), torch.zeros(2, 90, 2, 64, device=DEV)
+    _, *ref = gradients(q, k, v, zero, g, n, 0.125, s0, ds)
+    _, *mag = gradients(q, k, v, zero, g, n, 0.125, s0, ds, absolute=True)
+    for x, y, m in zip(got, ref, mag):
+        _near(x, y, 1e-5 * m, 'gradient')
+
+
+@pytest.mark.parametrize('dtype', [torch.float32, torch.bfloat16])
+def test_many_ragged_rows(dtype):
+    """More rows than fit one wave of CTAs, in every order of length."""
+    B, T = 45, 150
+    q, k, v, do, g, s0, ds = _inputs(18, B, T, 4, 4, 64, 64, dtype)
+    gen = torch.Generator(device=DEV).manual_seed(19)
+    n = torch.randint(0, T + 1, (B,), device=DEV, generator=gen)
+    n[5] = n[6] = n[7]
+    _check(q, k, v, do, g, s0, ds, lengths=n)
+
+
 def test_no_tokens():
     from bdm_b200 import decay_attention
     for dtype in (torch.float32, torch.bfloat16):
