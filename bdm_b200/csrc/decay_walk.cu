@@ -349,6 +349,9 @@ int device_setup(int &sms) {
     int dev = 0;
     if (int rc = cuda_status(cudaGetDevice(&dev))) return rc;
     if (dev < 0 || dev >= kMaxDevices) return BDM_ERR_UNSUPPORTED;
+    // a thread's first call (an autograd worker's) may come before anything has made the context current, which
+    // encoding a tensor map needs
+    if (int rc = cuda_status(cudaSetDevice(dev))) return rc;
     std::lock_guard<std::mutex> lock(g_mu);
     if (!g_attr[dev]) {
         const void *fns[] = {

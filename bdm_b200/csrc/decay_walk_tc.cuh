@@ -16,7 +16,7 @@
 //
 // Roles (22 warps of 24): 0-7 carry the state (a quadrant's value columns, half of the key columns), 8-11 scale V',
 // 12-15 the outputs, 16-19 P, 20 MMA, 21 TMA.  V' is made and T issued in two halves of 32 tokens, so that the
-// scaling of one overlaps the product of the other.  V' is in tensor memory because shared memory's bandwidth
+// scaling of one overlaps the product of the other (in the state launch by two groups, 4-7 and 8-11, at once).  V' is in tensor memory because shared memory's bandwidth
 // is what the products and copies share: as a shared-memory operand it took 768 more of its cycles per chunk.
 // The roles' loops are kept short on purpose: five roles' unrolled code does not fit the instruction cache
 // (measured: 100 us unrolled, 78 us rolled, for the same work).
@@ -248,6 +248,72 @@ __global__ void __launch_bounds__(kTcThreads, 1) decay_walk_tc_kernel(const TcPa
     const uint32_t lanes = (uint32_t)(quad * 32) << 16;
     constexpr int kQuadCols = 16 * kHalves;  // value columns of a quadrant
 
+    // V' of the half chunks half0, half0 + every, ... (32 tokens each), by the four warps of a group
+    auto scale_values = [&](int half0, int every, int ctid) -> bool {
+        // this lane's row of the matrices it loads: two of 8 tokens by two of 8 columns
+        const int mrow = ((lane >> 4) * 8 + (lane & 7)) * 128, mcol = (lane >> 3) & 1;
+        int st = 0, phase = 0;  // stage of the chunk, parity of its barrier
+        for (int hs = half0; hs < 2 * steps; hs += every) {
+            const int n = hs >> 1, hb = hs & 1;
+            const int valid = valid_of(n);
+            if (hb == 0 || every == 2) {
+                if (!wait_warp(&bar.full[st], phase)) return false;
+                if (valid < kChunk && start_of(n) + valid < time) {
+                    // tokens past the row's length may hold anything: zero them for the products over j
+                    if (hb == 0) {
+                        uint4 *kb = reinterpret_cast<uint4 *>(smem + st * kStage + kOffB);
+#pragma unroll 1
+                        for (int i = ctid; i < (DKB + VB) * kBox / 16; i += 128)
+                            if ((i % (kBox / 16)) / 8 >= valid) kb[i] = make_uint4(0, 0, 0, 0);
+                        tc::fence_async_smem();
+                        __syncwarp();
+                        if (lane == 0) tc::mbar_arrive(&bar.zeroed);  // once at most: a row has one such chunk
+                    }
+                    if (!wait_warp(&bar.zeroed, 0)) return false;
+                }
+            }
+            if (n > 0) {
+                if (!wait_warp(&bar.tpart[hb], (n - 1) & 1)) return false;
+                tc::fence_after_sync();
+            }
+            // in the state launch all chunks gather in one T: their distance to the segment's end counts too
+            float far = 1.f;
+            if (STATE_ONLY) {
+                const int64_t last = sp.c1 * kChunk < sp.n ? sp.c1 * kChunk : sp.n;
+                const int64_t gap = p.reverse ? start_of(n) - sp.c0 * kChunk : last - start_of(n) - valid;
+                far = gap ? expf(g * (float)gap) : 1.f;
+            }
+            // 16 tokens by this quadrant's columns at a time: transposed on the way in, scaled, and split into BF16
+            // terms as the fragments that tensor memory takes
+            const float *w = vw + (p.reverse ? 0 : kChunk - valid) + hb * 32 + 2 * (lane & 3);
+            const char *src = smem + st * kStage + kOffC + (VB == 2 ? (quad >> 1) * kBox : 0) + hb * 32 * 128 + mrow;
+            const int c0 = VB == 2 ? (quad & 1) * 4 : quad * 2;
+#pragma unroll (VB == 1 ? 2 : 1)
+            for (int q = 0; q < 2; ++q, src += 16 * 128, w += 16) {
+                const F2 w0 = make2(w[0] * far, w[1] * far), w1 = make2(w[8] * far, w[9] * far);
+                uint32_t r[kHalves][4];
+#pragma unroll
+                for (int d = 0; d < kHalves; ++d)
+                    tc::ldmatrix_x4_trans(src + (((c0 + d * 2 + mcol) ^ (lane & 7)) << 4), r[d]);
+#pragma unroll
+                for (int d = 0; d < kHalves; ++d) {
+                    uint32_t t[3][4];
+#pragma unroll
+                    for (int m = 0; m < 4; ++m) terms<TERMS>(mul2(m < 2 ? w0 : w1, unpack2(r[d][m])), t[0][m], t[1][m], t[2][m]);
+#pragma unroll
+                    for (int u = 0; u < TERMS; ++u) {
+                        const uint32_t at = tmem + lanes + kColV + hb * 48 + u * 16 + q * 8;
+                        tc::tmem_st_16x128b_x2(at + (d << 20), t[u][0], t[u][1], t[u][2], t[u][3]);
+                    }
+                }
+            }
+            if ((hb || every == 2) && ++st == stages) st = 0, phase ^= 1;
+            tc::tmem_wait_st();
+            arrive(&bar.vready[hb]);
+        }
+        return true;
+    };
+
     if (warp < kStateWarps) {
         tc::regs_up<kStateRegs>();
         // ------------------------------------------------------------------ state
@@ -291,7 +357,8 @@ __global__ void __launch_bounds__(kTcThreads, 1) decay_walk_tc_kernel(const TcPa
             if (p.state_in) gather(x, p.in_t, w);
         }
         bool ok = true;
-        for (int n = 0; n <= steps; ++n) {
+        if (STATE_ONLY && warp >= 4) ok = scale_values(1, 2, threadIdx.x - 128);  // nothing else to do until the end
+        for (int n = 0; ok && n <= steps; ++n) {
             if (n > 0) {
                 if (STATE_ONLY && n < steps) continue;  // T gathers all chunks in tensor memory
                 ok = STATE_ONLY ? wait_warp(&bar.tlast, 0) : wait_warp(&bar.tpart[1], (n - 1) & 1);
@@ -343,71 +410,7 @@ __global__ void __launch_bounds__(kTcThreads, 1) decay_walk_tc_kernel(const TcPa
         }
     } else if (warp < kOutWarp) {
         tc::regs_down<kScaleRegs>();
-        // --------------------------------------------------------------------- V'
-        // this lane's row of the matrices it loads: two of 8 tokens by two of 8 columns
-        const int mrow = ((lane >> 4) * 8 + (lane & 7)) * 128, mcol = (lane >> 3) & 1;
-        const int ctid = threadIdx.x - kScaleWarp * 32;
-        int st = 0, phase = 0;  // stage of the chunk, parity of its barrier
-        bool ok = true;
-        for (int hs = 0; hs < 2 * steps; ++hs) {  // half steps, 32 tokens
-            const int n = hs >> 1, hb = hs & 1;
-            const int valid = valid_of(n);
-            if (hb == 0) {
-                ok = wait_warp(&bar.full[st], phase);
-                if (!ok) break;
-                if (valid < kChunk && start_of(n) + valid < time) {
-                    // tokens past the row's length may hold anything: zero them for the products over j
-                    uint4 *kb = reinterpret_cast<uint4 *>(smem + st * kStage + kOffB);
-#pragma unroll 1
-                    for (int i = ctid; i < (DKB + VB) * kBox / 16; i += 128)
-                        if ((i % (kBox / 16)) / 8 >= valid) kb[i] = make_uint4(0, 0, 0, 0);
-                    tc::fence_async_smem();
-                    __syncwarp();
-                    if (lane == 0) tc::mbar_arrive(&bar.zeroed);  // once at most: a row has one such chunk
-                    ok = wait_warp(&bar.zeroed, 0);
-                    if (!ok) break;
-                }
-            }
-            if (n > 0) {
-                ok = wait_warp(&bar.tpart[hb], (n - 1) & 1);
-                if (!ok) break;
-                tc::fence_after_sync();
-            }
-            // in the state launch all chunks gather in one T: their distance to the segment's end counts too
-            float far = 1.f;
-            if (STATE_ONLY) {
-                const int64_t last = sp.c1 * kChunk < sp.n ? sp.c1 * kChunk : sp.n;
-                const int64_t gap = p.reverse ? start_of(n) - sp.c0 * kChunk : last - start_of(n) - valid;
-                far = gap ? expf(g * (float)gap) : 1.f;
-            }
-            // 16 tokens by this quadrant's columns at a time: transposed on the way in, scaled, and split into BF16
-            // terms as the fragments that tensor memory takes
-            const float *w = vw + (p.reverse ? 0 : kChunk - valid) + hb * 32 + 2 * (lane & 3);
-            const char *src = smem + st * kStage + kOffC + (VB == 2 ? (quad >> 1) * kBox : 0) + hb * 32 * 128 + mrow;
-            const int c0 = VB == 2 ? (quad & 1) * 4 : quad * 2;
-#pragma unroll (VB == 1 ? 2 : 1)
-            for (int q = 0; q < 2; ++q, src += 16 * 128, w += 16) {
-                const F2 w0 = make2(w[0] * far, w[1] * far), w1 = make2(w[8] * far, w[9] * far);
-                uint32_t r[kHalves][4];
-#pragma unroll
-                for (int d = 0; d < kHalves; ++d)
-                    tc::ldmatrix_x4_trans(src + (((c0 + d * 2 + mcol) ^ (lane & 7)) << 4), r[d]);
-#pragma unroll
-                for (int d = 0; d < kHalves; ++d) {
-                    uint32_t t[3][4];
-#pragma unroll
-                    for (int m = 0; m < 4; ++m) terms<TERMS>(mul2(m < 2 ? w0 : w1, unpack2(r[d][m])), t[0][m], t[1][m], t[2][m]);
-#pragma unroll
-                    for (int u = 0; u < TERMS; ++u) {
-                        const uint32_t at = tmem + lanes + kColV + hb * 48 + u * 16 + q * 8;
-                        tc::tmem_st_16x128b_x2(at + (d << 20), t[u][0], t[u][1], t[u][2], t[u][3]);
-                    }
-                }
-            }
-            if (hb && ++st == stages) st = 0, phase ^= 1;
-            tc::tmem_wait_st();
-            arrive(&bar.vready[hb]);
-        }
+        scale_values(0, STATE_ONLY ? 2 : 1, threadIdx.x - kScaleWarp * 32);
     } else if (warp < kScoreWarp) {
         // ---------------------------------------------------------------- outputs
         if constexpr (!STATE_ONLY) {

@@ -272,6 +272,35 @@ def test_side_stream_and_repeated_calls_agree():
     assert all(torch.equal(x, y) for x, y in zip(first, second))
 
 
+def test_first_call_of_a_thread():
+    """A new thread (an autograd worker, say) has no current context until something makes it one."""
+    import threading
+    from bdm_b200 import decay_attention
+    q, k, v, _, g, s0, _ = _inputs(20, 2, 200, 2, 2, 64, 64, torch.bfloat16)
+    want = decay_attention(q, k, v, g, initial_state=s0)
+    spare = torch.empty_like(want)
+    del spare  # the allocator has a block for the output: the thread's first driver call is the walk's
+    got = []
+    worker = threading.Thread(target=lambda: got.append(decay_attention(q, k, v, g, initial_state=s0)))
+    worker.start()
+    worker.join()
+    torch.cuda.synchronize()
+    assert got and torch.equal(got[0], want)
+
+
+def test_training_step_in_a_graph():
+    from bdm_b200 import decay_attention
+    q, k, v, do, g, _, _ = _inputs(21, 2, 300, 2, 1, 64, 64, torch.bfloat16, state=False)
+    leaves = [x.requires_grad_(True) for x in (q, k, v)]
+    want = torch.autograd.grad(decay_attention(q, k, v, g), leaves, do)
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        got = torch.autograd.grad(decay_attention(q, k, v, g), leaves, do)
+    graph.replay()
+    torch.cuda.synchronize()
+    assert all(torch.equal(x, y) for x, y in zip(got, want))
+
+
 def test_refusals():
     from bdm_b200 import decay_attention, decay_attention_step
     q, k, v, _, g, s0, _ = _inputs(15, 2, 8, 4, 2, 16, 16, torch.float32)
