@@ -30,7 +30,7 @@ class DecayWalkArgs(ctypes.Structure):
                 + [(n, _i64 * 3) for n in ('a_stride', 'b_stride', 'c_stride', 'out_stride')]
                 + [('batch', _i64), ('time', _i64)]
                 + [(n, _int) for n in ('heads', 'a_heads', 'b_heads', 'c_heads', 'width_ab', 'width_c', 'dtype',
-                                       'out_dtype', 'reverse', 'state_in_transposed', 'state_out_transposed')]
+                                       'out_dtype', 'reverse', 'state_in_transposed', 'state_out_transposed', 'overlap')]
                 + [(n, _flt) for n in ('scale', 'state_in_mul', 'state_out_mul')])
 
 

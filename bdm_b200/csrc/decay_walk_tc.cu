@@ -120,7 +120,7 @@ int decay_walk_tc_launch(const bdm_decay_walk_args &w, Params p, int sub, int sc
         if (int rc = run(tp, maps, kTcState, terms, false, st)) return rc;
         if (int rc = decay_prefix_launch(p, tp.z, sub, scps, st)) return rc;
     }
-    return run(tp, maps, w.out_dtype == BDM_F32 ? kTcFloat : kTcBf16, terms, p.nseg > 1, st);
+    return run(tp, maps, w.out_dtype == BDM_F32 ? kTcFloat : kTcBf16, terms, p.nseg > 1 || w.overlap, st);
 }
 
 }  // namespace bdm

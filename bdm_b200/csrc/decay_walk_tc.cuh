@@ -14,8 +14,8 @@
 // returned: T, and with it the state over any number of chunks, is then exact to FP32.  Where none is, two
 // terms (an error of 2^-17 beside the outputs' 2^-9) are enough.
 //
-// Roles (22 warps of 24): 0-7 carry the state (a quadrant's value columns, half of the key columns), 8-11 scale V',
-// 12-15 the outputs, 16-19 P, 20 MMA, 21 TMA.  V' is made and T issued in two halves of 32 tokens, so that the
+// Roles (23 warps of 24): 0-7 carry the state (a quadrant's value columns, half of the key columns), 8-11 scale V',
+// 12-15 the outputs, 16-19 P, 20 and 22 MMA, 21 TMA.  V' is made and T issued in two halves of 32 tokens, so that the
 // scaling of one overlaps the product of the other (in the state launch by two groups, 4-7 and 8-11, at once).  V' is in tensor memory because shared memory's bandwidth
 // is what the products and copies share: as a shared-memory operand it took 768 more of its cycles per chunk.
 // The roles' loops are kept short on purpose: five roles' unrolled code does not fit the instruction cache
@@ -41,7 +41,8 @@ constexpr int kTcThreads = 768;
 constexpr int kStateRegs = 112, kScaleRegs = 72, kOutRegs = 80, kScoreRegs = 64, kMmaRegs = 40;
 static_assert(2 * kStateRegs + kScaleRegs + kOutRegs + kScoreRegs + kMmaRegs <= 6 * 80, "register shares");
 constexpr int kBox = 64 * 128;  // bytes of a TMA box: 64 tokens x 64 BF16 columns
-constexpr int kStateWarps = 8, kScaleWarp = 8, kOutWarp = 12, kScoreWarp = 16, kMmaWarp = 20, kTmaWarp = 21;
+constexpr int kStateWarps = 8, kScaleWarp = 8, kOutWarp = 12, kScoreWarp = 16, kMmaWarp = 20, kTmaWarp = 21,
+              kOutMmaWarp = 22;
 constexpr int kMaxStages = 8;
 constexpr int kSmemMax = 227 * 1024;
 constexpr long long kWaitCycles = 4000000000ll;  // about 2 s
@@ -65,7 +66,7 @@ struct TcParams {
 // needs something that its waiter gives after the wait (P's two buffers have one barrier each for that reason).
 struct Bars {
     uint64_t full[kMaxStages], empty[kMaxStages];
-    uint64_t vready[2], tpart[2], pfree[2], tlast, tfree, sready, adone, pready, odone, ofree, zeroed, ofull, oempty;
+    uint64_t vready[2], tpart[2], pfree[2], tlast, tfree, sready, adone, pready, odone, ofree, zeroed, ofull, oempty, drain[2];
 };
 
 __device__ __forceinline__ uint32_t pack_bf16(float lo, float hi) {
@@ -204,7 +205,7 @@ __global__ void __launch_bounds__(kTcThreads, 1) decay_walk_tc_kernel(const TcPa
         dead = 0;
         for (int i = 0; i < stages; ++i) {
             tc::mbar_init(&bar.full[i], 1);
-            tc::mbar_init(&bar.empty[i], 1);
+            tc::mbar_init(&bar.empty[i], STATE_ONLY ? 1 : 2);
         }
         for (int i = 0; i < 2; ++i) {
             tc::mbar_init(&bar.vready[i], 4);
@@ -221,6 +222,8 @@ __global__ void __launch_bounds__(kTcThreads, 1) decay_walk_tc_kernel(const TcPa
         tc::mbar_init(&bar.zeroed, 4);
         tc::mbar_init(&bar.ofull, 4);
         tc::mbar_init(&bar.oempty, 1);
+        tc::mbar_init(&bar.drain[0], 1);
+        tc::mbar_init(&bar.drain[1], 1);
         tc::mbar_fence_init();
     }
     if (warp == kMmaWarp) tc::tmem_alloc(&tmem_slot, 512);
@@ -536,33 +539,17 @@ __global__ void __launch_bounds__(kTcThreads, 1) decay_walk_tc_kernel(const TcPa
             }
         }
     } else {
-        // --------------------------------------------------------------- products
         tc::regs_down<kMmaRegs>();
+        // Two issuers, one for the state's products and one for the outputs': a product costs its thread some 40
+        // cycles and a wait 50 and more, and with one thread that chain was longer than the products.
         if (warp == kMmaWarp && tc::elect_one()) {
-            constexpr uint32_t idQK = tc::idesc_bf16(64, 64);
-            constexpr uint32_t idO1 = tc::idesc_bf16(M, 64) | tc::kIdescMnA;
-            constexpr uint32_t idO2 = tc::idesc_bf16(M, 64);
+            // ------------------------------------------------------- products for the state
             constexpr uint32_t idT = tc::idesc_bf16(M, DK) | tc::kIdescMnB;
-            // descriptors of the buffers' starts; an offset adds its bytes / 16 to the low word
-            const uint32_t base = tc::smem_u32(smem);
-            const uint64_t dP = tc::smem_desc_sw128(tc::smem_u32(sP));
-            auto scores = [&](int st) {
-                uint64_t qa = tc::smem_desc_sw128(base + st * kStage), kb = qa + kOffB / 16;
-#pragma unroll 1
-                for (int i = 0; i < DKB; ++i, qa += kBox / 16, kb += kBox / 16)
-#pragma unroll
-                    for (int k = 0; k < 4; ++k) tc::mma_bf16(tmem + kColA, qa + k * 2, kb + k * 2, idQK, i + k > 0);
-                tc::mma_commit(&bar.adone);
-            };
+            uint32_t tile = tc::smem_u32(smem) + kOffB;
             bool ok = true;
-            int done = 0, st = 0, phase = 0;
-            if (!STATE_ONLY && steps > 0) {
-                ok = wait(&bar.full[0], 0);
-                if (ok) scores(0);
-            }
+            int st = 0;
             for (int n = 0; n < steps && ok; ++n) {
-                const uint32_t tile = base + st * kStage;
-                uint64_t kb = tc::smem_desc_sw128_mn(tile + kOffB, kBox);
+                uint64_t kb = tc::smem_desc_sw128_mn(tile, kBox);
                 uint32_t va = tmem + kColV;
                 if (!STATE_ONLY && n > 0 && !(ok = wait(&bar.tfree, (n - 1) & 1))) break;
 #pragma unroll 1
@@ -577,38 +564,63 @@ __global__ void __launch_bounds__(kTcThreads, 1) decay_walk_tc_kernel(const TcPa
                                                 hb + t + k + (STATE_ONLY ? n : 0) > 0);
                     tc::mma_commit(&bar.tpart[hb]);
                 }
-                if (!ok) break;
-                const int st1 = st + 1 == stages ? 0 : st + 1, phase1 = st + 1 == stages ? phase ^ 1 : phase;
-                if (!STATE_ONLY) {
-                    // P(n) is ready, so A is free: the next scores go first, P(n + 1) is what takes longest
-                    if (!(ok = wait(&bar.pready, n & 1))) break;
-                    tc::fence_after_sync();
-                    if (n + 1 < steps) {
-                        if (!(ok = wait(&bar.full[st1], phase1))) break;
-                        scores(st1);
-                    }
-                    if (!(ok = wait(&bar.sready, n & 1))) break;
-                    if (n > 0 && !(ok = wait(&bar.ofree, (n - 1) & 1))) break;
-                    tc::fence_after_sync();
-                    uint64_t qa = tc::smem_desc_sw128(tile);
-                    uint32_t sa = tmem + kColS;
-#pragma unroll 1
-                    for (int i = 0; i < DKB; ++i, qa += kBox / 16, sa += 32)
-#pragma unroll
-                        for (int k = 0; k < 4; ++k) tc::mma_bf16_tmem_a(tmem + kColO2, sa + k * 8, qa + k * 2, idO2, i + k > 0);
-                    const uint64_t vc = tc::smem_desc_sw128_mn(tile + kOffC, kBox), pn = dP + (n & 1) * kBox / 16;
-#pragma unroll
-                    for (int k = 0; k < 4; ++k) tc::mma_bf16(tmem + kColO1, vc + k * 2048 / 16, pn + k * 2, idO1, k > 0);
-                    tc::mma_commit(&bar.odone);
-                    tc::mma_commit(&bar.pfree[n & 1]);
-                }
                 tc::mma_commit(&bar.empty[st]);
-                done = n + 1;
-                st = st1, phase = phase1;
+                tile += kStage;
+                if (++st == stages) st = 0, tile -= stages * kStage;
             }
             if (STATE_ONLY && ok) tc::mma_commit(&bar.tlast);
             // no product may be in flight when the CTA ends, whatever happened to its consumers
-            if (done) tc::mbar_wait(&bar.empty[(done - 1) % stages], ((done - 1) / stages) & 1, kWaitNs);
+            tc::mma_commit(&bar.drain[0]);
+            tc::mbar_wait(&bar.drain[0], 0, kWaitNs);
+        } else if (!STATE_ONLY && warp == kOutMmaWarp && tc::elect_one()) {
+            // ----------------------------------------------------- products for the outputs
+            constexpr uint32_t idQK = tc::idesc_bf16(64, 64);
+            constexpr uint32_t idO1 = tc::idesc_bf16(M, 64) | tc::kIdescMnA;
+            constexpr uint32_t idO2 = tc::idesc_bf16(M, 64);
+            // descriptors of the buffers' starts; an offset adds its bytes / 16 to the low word
+            const uint32_t base = tc::smem_u32(smem);
+            const uint64_t dP = tc::smem_desc_sw128(tc::smem_u32(sP));
+            auto scores = [&](int st) {
+                uint64_t qa = tc::smem_desc_sw128(base + st * kStage), kb = qa + kOffB / 16;
+#pragma unroll 1
+                for (int i = 0; i < DKB; ++i, qa += kBox / 16, kb += kBox / 16)
+#pragma unroll
+                    for (int k = 0; k < 4; ++k) tc::mma_bf16(tmem + kColA, qa + k * 2, kb + k * 2, idQK, i + k > 0);
+                tc::mma_commit(&bar.adone);
+            };
+            int st = 0, phase = 0;
+            if (steps > 0 && wait(&bar.full[0], 0)) scores(0);
+            for (int n = 0; n < steps; ++n) {
+                const uint32_t tile = base + st * kStage;
+                const int st1 = st + 1 == stages ? 0 : st + 1, phase1 = st + 1 == stages ? phase ^ 1 : phase;
+                // P(n) is ready, so A is free: the next scores go first, P(n + 1) is what takes longest
+                if (!wait(&bar.pready, n & 1)) break;
+                tc::fence_after_sync();
+                if (n + 1 < steps) {
+                    if (!wait(&bar.full[st1], phase1)) break;
+                    scores(st1);
+                }
+                if (!wait(&bar.sready, n & 1)) break;
+                if (n > 0 && !wait(&bar.ofree, (n - 1) & 1)) break;
+                const int valid = valid_of(n);
+                if (valid < kChunk && start_of(n) + valid < time && !wait(&bar.zeroed, 0)) break;  // c past the row's end
+                tc::fence_after_sync();
+                uint64_t qa = tc::smem_desc_sw128(tile);
+                uint32_t sa = tmem + kColS;
+#pragma unroll 1
+                for (int i = 0; i < DKB; ++i, qa += kBox / 16, sa += 32)
+#pragma unroll
+                    for (int k = 0; k < 4; ++k) tc::mma_bf16_tmem_a(tmem + kColO2, sa + k * 8, qa + k * 2, idO2, i + k > 0);
+                const uint64_t vc = tc::smem_desc_sw128_mn(tile + kOffC, kBox), pn = dP + (n & 1) * kBox / 16;
+#pragma unroll
+                for (int k = 0; k < 4; ++k) tc::mma_bf16(tmem + kColO1, vc + k * 2048 / 16, pn + k * 2, idO1, k > 0);
+                tc::mma_commit(&bar.odone);
+                tc::mma_commit(&bar.pfree[n & 1]);
+                tc::mma_commit(&bar.empty[st]);
+                st = st1, phase = phase1;
+            }
+            tc::mma_commit(&bar.drain[1]);
+            tc::mbar_wait(&bar.drain[1], 0, kWaitNs);
         } else if (warp == kTmaWarp && tc::elect_one()) {
             // --------------------------------------------------------------- loads
             const int ha = (h / p.ag) * tp.bmul[0], hk = (h / p.bg) * tp.bmul[1], hc = (h / p.cg) * tp.bmul[2];

@@ -41,13 +41,16 @@ def _rows(x):
 
 # bdm_decay_walk_args and bdm_decay_step_args (include/bdm_b200.h), packed in one go: filling a ctypes
 # structure field by field costs several times as much
-_WALK = struct.Struct('9P12q2q11i3f')
+_WALK = struct.Struct('9P12q2q12i3f4x')
 _STEP = struct.Struct('6P6qq5if')
 
 
 def _walk(a, b, c, log_decay, lengths, st, *, heads, scale, reverse=0, out_dtype=None, state_in=None, state_in_mul=1.0,
-          state_in_transposed=0, state_out=None, state_out_mul=1.0):
-    """One bdm_decay_walk over [B, T, heads of the operand, width] tensors; returns out [B, T, heads, width of c]."""
+          state_in_transposed=0, state_out=None, state_out_mul=1.0, after=None):
+    """One bdm_decay_walk over [B, T, heads of the operand, width] tensors; returns out [B, T, heads, width of c].
+
+    ``after``: list of the walks already launched for this backward, independent of this one; it may overlap
+    the last of them when that one had no workspace (whose memory this one's output could otherwise reuse)."""
     batch, time, a_heads, wab = a.shape
     c_heads, wc = c.shape[2:]
     dt = a.dtype
@@ -57,7 +60,8 @@ def _walk(a, b, c, log_decay, lengths, st, *, heads, scale, reverse=0, out_dtype
                    0 if state_out is None else state_out.data_ptr(), st.mapped_ptr,
                    *a.stride()[:3], *b.stride()[:3], *c.stride()[:3], time * heads * wc, heads * wc, wc,
                    batch, time, heads, a_heads, b.shape[2], c_heads, wab, wc, ops._DT[dt], ops._DT[out.dtype],
-                   reverse, state_in_transposed, 0, scale, state_in_mul, state_out_mul)
+                   reverse, state_in_transposed, 0, int(bool(after and after[-1])), scale, state_in_mul,
+                   state_out_mul)
     lib = _lib.load()
     nbytes = lib.bdm_decay_walk_workspace_bytes(w)
     ws = None
@@ -68,6 +72,8 @@ def _walk(a, b, c, log_decay, lengths, st, *, heads, scale, reverse=0, out_dtype
     status = lib.bdm_decay_walk(w, ws.data_ptr() if nbytes else None, nbytes, _raw_stream(a.device))
     if status:
         _lib.check(status, 'bdm_decay_walk')
+    if after is not None:
+        after.append(ws is None)
     return out
 
 
@@ -111,7 +117,7 @@ class _DecayAttention(torch.autograd.Function):
         need = ctx.needs_input_grad
         dq = dk = dv = ds0 = None
         shared = kv_heads != heads
-        walk = dict(heads=heads, scale=scale)
+        walk = dict(heads=heads, scale=scale, after=None if shared else [])
         back = dict(walk, reverse=1, state_in=dstate, state_in_mul=1.0 / scale,
                     out_dtype=torch.float32 if shared else dt)
         with _on(q.device):
