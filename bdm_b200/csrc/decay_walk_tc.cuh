@@ -66,7 +66,7 @@ struct TcParams {
 // needs something that its waiter gives after the wait (P's two buffers have one barrier each for that reason).
 struct Bars {
     uint64_t full[kMaxStages], empty[kMaxStages];
-    uint64_t vready[2], tpart[2], pfree[2], tlast, tfree, sready, adone, pready, odone, ofree, zeroed, ofull, oempty, drain[2];
+    uint64_t vready[2], tpart[2], pfree[2], tlast, tfree, sready, adone, pready, odone, ofree, zeroed, ofull, oempty, drain[2], oissued[2];
 };
 
 __device__ __forceinline__ uint32_t pack_bf16(float lo, float hi) {
@@ -211,6 +211,7 @@ __global__ void __launch_bounds__(kTcThreads, 1) decay_walk_tc_kernel(const TcPa
             tc::mbar_init(&bar.vready[i], 4);
             tc::mbar_init(&bar.tpart[i], 1);
             tc::mbar_init(&bar.pfree[i], 1);
+            tc::mbar_init(&bar.oissued[i], 1);
         }
         tc::mbar_init(&bar.tlast, 1);
         tc::mbar_init(&bar.tfree, kStateWarps);
@@ -551,7 +552,11 @@ __global__ void __launch_bounds__(kTcThreads, 1) decay_walk_tc_kernel(const TcPa
             for (int n = 0; n < steps && ok; ++n) {
                 uint64_t kb = tc::smem_desc_sw128_mn(tile, kBox);
                 uint32_t va = tmem + kColV;
-                if (!STATE_ONLY && n > 0 && !(ok = wait(&bar.tfree, (n - 1) & 1))) break;
+                if (!STATE_ONLY && n > 0) {
+                    if (!(ok = wait(&bar.tfree, (n - 1) & 1))) break;
+                    // long products (N = 128) must not get ahead of the outputs', which more is waiting for
+                    if (DKB == 2 && !(ok = wait(&bar.oissued[(n - 1) & 1], ((n - 1) >> 1) & 1))) break;
+                }
 #pragma unroll 1
                 for (int hb = 0; hb < 2; ++hb, kb += 2 * 2048 / 16, va += 48) {
                     if (!(ok = wait(&bar.vready[hb], n & 1))) break;
@@ -614,6 +619,7 @@ __global__ void __launch_bounds__(kTcThreads, 1) decay_walk_tc_kernel(const TcPa
                 const uint64_t vc = tc::smem_desc_sw128_mn(tile + kOffC, kBox), pn = dP + (n & 1) * kBox / 16;
 #pragma unroll
                 for (int k = 0; k < 4; ++k) tc::mma_bf16(tmem + kColO1, vc + k * 2048 / 16, pn + k * 2, idO1, k > 0);
+                tc::mbar_arrive(&bar.oissued[n & 1]);
                 tc::mma_commit(&bar.odone);
                 tc::mma_commit(&bar.pfree[n & 1]);
                 tc::mma_commit(&bar.empty[st]);
