@@ -1,6 +1,7 @@
 // Decay attention, one token per row: S <- lam S + k v^T (in place, FP32), o = scale q S.
 //
-// The state is read and written once (8 dk dv bytes per head) and nothing else matters: the bound is HBM.
+// The state is read and written once (8 dk dv bytes per head) and nothing else matters: the bound is HBM (256
+// rows of 8 heads of 128: 44 us, 41 at the copy rate).
 // A CTA owns one (row, head) and a slice of dv columns; a thread holds 4 columns (one 16-byte access) of
 // every 8th..32nd state row, all its loads are issued before the first use, and the partial sums of o over
 // the state's rows are joined in shared memory in a fixed order.

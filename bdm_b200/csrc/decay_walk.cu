@@ -4,8 +4,9 @@
 // The walk's mathematics is in decay_walk.cuh.  Operands are widened to FP32 in shared memory.  Every product
 // a b runs on the tensor cores as three TF32 products, a1 b1 + a1 b2 + a2 b1 with a = a1 + a2 + r, |r| <= 2^-22 |a|
 // (the method of splitting an operand into its rounding and the remainder), summed in FP32: about 3e-7 beside
-// FP32's own 1e-7, where plain TF32 gives 5e-4.  Sums and states are FP32.  (On FP32 FMAs, with the same tiles,
-// 2 x 4096 tokens x 16 heads of 128 took 708 us.)
+// FP32's own 1e-7, where plain TF32 gives 5e-4.  Sums and states are FP32.  Bound: the TF32 products' rate and
+// the latency of a chunk's phases (2 x 4096 tokens x 8 heads of 128: 440 us; on FP32 FMAs with the same tiles,
+// whose operands shared memory could not deliver, about 700).
 #include "decay_walk.cuh"
 
 #include <mutex>
