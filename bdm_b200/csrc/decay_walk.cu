@@ -5,8 +5,8 @@
 // a b runs on the tensor cores as three TF32 products, a1 b1 + a1 b2 + a2 b1 with a = a1 + a2 + r, |r| <= 2^-22 |a|
 // (the method of splitting an operand into its rounding and the remainder), summed in FP32: about 3e-7 beside
 // FP32's own 1e-7, where plain TF32 gives 5e-4.  Sums and states are FP32.  Bound: the TF32 products' rate and
-// the latency of a chunk's phases (2 x 4096 tokens x 8 heads of 128: 440 us; on FP32 FMAs with the same tiles,
-// whose operands shared memory could not deliver, about 700).
+// the latency of a chunk's phases (2 x 4096 tokens x 8 heads of 128: 440 us; 3 x 777 x 6 heads of 40 / 72: 48 us
+// in three launches, on FP32 FMAs with the same tiles 72).
 #include "decay_walk.cuh"
 
 #include <mutex>

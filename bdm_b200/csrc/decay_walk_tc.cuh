@@ -15,9 +15,10 @@
 // terms (an error of 2^-17 beside the outputs' 2^-9) are enough.
 //
 // Roles (23 warps of 24): 0-7 carry the state (a quadrant's value columns, half of the key columns), 8-11 scale V',
-// 12-15 the outputs, 16-19 P, 20 and 22 MMA, 21 TMA.  V' is made and T issued in two halves of 32 tokens, so that the
-// scaling of one overlaps the product of the other (in the state launch by two groups, 4-7 and 8-11, at once).  V' is in tensor memory because shared memory's bandwidth
-// is what the products and copies share: as a shared-memory operand it took 768 more of its cycles per chunk.
+// 12-15 the outputs, 16-19 P, 20 and 22 MMA, 21 TMA.  V' is made and T issued in two halves of 32 tokens, so that
+// the scaling of one overlaps the product of the other (in the state launch by two groups, 4-7 and 8-11, at once).
+// V' is in tensor memory because shared memory's bandwidth is what the products and copies share: as a
+// shared-memory operand it took 768 more of its cycles per chunk.
 // The roles' loops are kept short on purpose: five roles' unrolled code does not fit the instruction cache
 // (2048 tokens x 148 heads of 128: 100 us unrolled, 78 us rolled, with one set of roles).
 // The scores, and value widths up to 64, use M = 64 products, whose 64 rows are 16 lanes of each quadrant, so
@@ -40,8 +41,9 @@ namespace walk {
 constexpr int kTcThreads = 768;
 // Registers: 6 groups of 4 warps, 80 per thread at launch (480 in all), dealt out as 2 x 112 (state) + 72 (V') + 80
 // (outputs) + 64 (P) + 40 (loads and products).
+constexpr int kLaunchRegs = 80;
 constexpr int kStateRegs = 112, kScaleRegs = 72, kOutRegs = 80, kScoreRegs = 64, kMmaRegs = 40;
-static_assert(2 * kStateRegs + kScaleRegs + kOutRegs + kScoreRegs + kMmaRegs <= 6 * 80, "register shares");
+static_assert(2 * kStateRegs + kScaleRegs + kOutRegs + kScoreRegs + kMmaRegs <= 6 * kLaunchRegs, "register shares");
 constexpr int kBox = 64 * 128;  // bytes of a TMA box: 64 tokens x 64 BF16 columns
 constexpr int kStateWarps = 8, kScaleWarp = 8, kOutWarp = 12, kScoreWarp = 16, kMmaWarp = 20, kTmaWarp = 21,
               kOutMmaWarp = 22;
@@ -68,7 +70,9 @@ struct TcParams {
 // needs something that its waiter gives after the wait (P's two buffers have one barrier each for that reason).
 struct Bars {
     uint64_t full[kMaxStages], empty[kMaxStages];
-    uint64_t vready[2], tpart[2], pfree[2], tlast, tfree, sready, adone, pready, odone, ofree, zeroed, ofull, oempty, drain[2], oissued[2];
+    uint64_t vready[2], tpart[2], tlast, tfree, sready;       // V' halves, T halves, all T, T read, S written
+    uint64_t adone, pready, pfree[2], odone, oissued[2], ofree;  // A, P, P read, O, O issued, O read
+    uint64_t zeroed, ofull, oempty, drain[2];                 // row's end cleared, output buffers, issuers' last products
 };
 
 __device__ __forceinline__ uint32_t pack_bf16(float lo, float hi) {
@@ -128,7 +132,6 @@ __device__ __forceinline__ bool wait_slow(uint64_t *m, unsigned parity, volatile
     *dead = 1;
     return false;
 }
-
 
 // Stages of the load pipeline: what shared memory holds beside two buffers of P and of outputs.
 template <int DKB, int VB, bool STATE_ONLY> constexpr int stages_of() {
@@ -698,6 +701,10 @@ int tc_launch(const TcParams &tp, const Maps &maps, bool dependent, cudaStream_t
         std::lock_guard<std::mutex> lock(mu);
         if (!set[dev]) {
             if (int rc = cuda_status(cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, smem))) return rc;
+            // the state warps wait for the registers that the others give up: never launch with fewer than are dealt out
+            cudaFuncAttributes fa;
+            if (int rc = cuda_status(cudaFuncGetAttributes(&fa, kernel))) return rc;
+            if (fa.numRegs < kLaunchRegs) return BDM_ERR_UNSUPPORTED;
             set[dev] = true;
         }
     }
