@@ -407,12 +407,7 @@ int64_t walk_segments(int64_t ctas, int64_t chunks, int sms) {
     return s > chunks ? chunks : s;
 }
 
-struct Split {
-    bool tc;        // the tensor-core walk takes it
-    int sub, scps;  // its state launch's sub-segments and their chunks
-};
-
-int plan(const bdm_decay_walk_args &w, Params &p, Split &split, int sms) {
+int plan(const bdm_decay_walk_args &w, Params &p, WalkSplit &split, bool &tc, int sms) {
     p.a = w.a, p.b = w.b, p.c = w.c, p.out = w.out;
     for (int i = 0; i < 3; ++i) {
         p.as[i] = w.a_stride[i];
@@ -432,13 +427,16 @@ int plan(const bdm_decay_walk_args &w, Params &p, Split &split, int sms) {
     p.status = w.status;
     p.seg = nullptr;
     const int64_t chunks = ceil_div(w.time, kChunk) > 0 ? ceil_div(w.time, kChunk) : 1;
-    split = Split{decay_walk_tc_takes(w), 1, 1};
-    if (split.tc) {
-        decay_walk_tc_split(w.batch * w.heads, chunks, sms, p.nseg, p.cps, split.sub, split.scps);
+    tc = decay_walk_tc_takes(w);
+    if (tc) {
+        split = decay_walk_tc_split(w.batch * w.heads, chunks, w.width_c, sms);
+        p.nseg = split.nseg;
+        p.cps = split.cps;
     } else {
         const int64_t nseg = walk_segments(w.batch * w.heads * ceil_div(w.width_c, kCols), chunks, sms);
         p.cps = (int)ceil_div(chunks, nseg);
         p.nseg = (int)ceil_div(chunks, p.cps);
+        split = WalkSplit{p.nseg, p.cps, 1, p.cps, 1};
     }
     return BDM_OK;
 }
@@ -455,7 +453,7 @@ int check_args(const bdm_decay_walk_args &w) {
     return BDM_OK;
 }
 
-int64_t seg_bytes(const Params &p, const Split &split) {
+int64_t seg_bytes(const Params &p, const WalkSplit &split) {
     return p.nseg > 1 ? p.batch * p.heads * ((int64_t)p.nseg + (int64_t)(p.nseg - 1) * split.sub) * p.wab * p.wc * 4 : 0;
 }
 
@@ -486,8 +484,9 @@ extern "C" int64_t bdm_decay_walk_workspace_bytes(const bdm_decay_walk_args *w) 
     int sms = 0;
     if (device_setup(sms)) return -1;
     Params p{};
-    Split split{};
-    if (plan(*w, p, split, sms)) return -1;
+    WalkSplit split{};
+    bool tc = false;
+    if (plan(*w, p, split, tc, sms)) return -1;
     return seg_bytes(p, split);
 }
 
@@ -500,12 +499,13 @@ extern "C" int bdm_decay_walk(const bdm_decay_walk_args *w, void *workspace, int
     int sms = 0;
     if (int rc = device_setup(sms)) return rc;
     Params p{};
-    Split split{};
-    if (int rc = plan(*w, p, split, sms)) return rc;
+    WalkSplit split{};
+    bool tc = false;
+    if (int rc = plan(*w, p, split, tc, sms)) return rc;
     const int64_t need = seg_bytes(p, split);
     if (need > workspace_bytes || (need && !workspace)) return BDM_ERR_WORKSPACE;
     cudaStream_t st = as_stream(stream);
-    if (split.tc) return decay_walk_tc_launch(*w, p, split.sub, split.scps, workspace, st);
+    if (tc) return decay_walk_tc_launch(*w, p, split, workspace, st);
     if (w->dtype == BDM_F32) return walk_launch<float, float>(p, workspace, st);
     if (w->out_dtype == BDM_F32) return walk_launch<bf16, float>(p, workspace, st);
     return walk_launch<bf16, bf16>(p, workspace, st);

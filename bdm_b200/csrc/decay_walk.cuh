@@ -77,13 +77,20 @@ __device__ __forceinline__ Span span_of(const Params &p, int64_t n, int seg) {
 
 }  // namespace walk
 
+// How a walk is cut up: segments of a row and their chunks, sub-segments of one in the state launch and theirs,
+// CTAs that share a row's value columns.
+struct WalkSplit {
+    int nseg, cps, sub, scps, vsplit;
+};
+
 // Sums the segments' start states from z, [batch*heads, (nseg - 1) * sub, wab * wc], the own states of the
 // sub-segments (scps chunks each, sub in a segment) of all segments but the last one walked.
 int decay_prefix_launch(const walk::Params &p, const float *z, int sub, int scps, cudaStream_t st);
 
 // The tensor-core walk (decay_walk_tc.cu): BF16 operands that TMA can address.
 bool decay_walk_tc_takes(const bdm_decay_walk_args &w);
-void decay_walk_tc_split(int64_t rows, int64_t chunks, int sms, int &nseg, int &cps, int &sub, int &scps);
-int decay_walk_tc_launch(const bdm_decay_walk_args &w, walk::Params p, int sub, int scps, void *workspace, cudaStream_t st);
+WalkSplit decay_walk_tc_split(int64_t rows, int64_t chunks, int width_c, int sms);
+int decay_walk_tc_launch(const bdm_decay_walk_args &w, walk::Params p, const WalkSplit &split, void *workspace,
+                         cudaStream_t st);
 
 }  // namespace bdm

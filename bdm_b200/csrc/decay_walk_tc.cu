@@ -72,25 +72,33 @@ bool decay_walk_tc_takes(const bdm_decay_walk_args &w) {
     return encode_tiled() != nullptr;
 }
 
-// Segments of the time axis: the split that makes the launches shortest, in units of a chunk of the main walk
-// (about a microsecond).  A CTA has an SM to itself; its start and end cost about three chunks, a chunk of the
-// state launch 0.6, the prefix launch and the dependent starts about six in all.
-void decay_walk_tc_split(int64_t rows, int64_t chunks, int sms, int &nseg, int &cps, int &sub, int &scps) {
-    nseg = 1, cps = (int)chunks, sub = 1, scps = (int)chunks;
+// Segments of the time axis, and CTAs to a row's value columns: the split that makes the launches shortest, in
+// units of a chunk of the main walk (1.7 us).  A CTA has an SM to itself; its start and end cost about three
+// chunks, a chunk of half the columns 0.75, one of the state launch 0.6 of the walk's, the prefix launch and the
+// dependent starts about six in all.  (8 x 4096 tokens x 8 heads of 128: two segments 104 us, two halves of the
+// columns 91; halves also read a and b twice, but from L2.)
+WalkSplit decay_walk_tc_split(int64_t rows, int64_t chunks, int width_c, int sms) {
+    WalkSplit best{1, (int)chunks, 1, (int)chunks, 1};
     double cost = (double)ceil_div(rows, sms) * (chunks + 3.0);
-    for (int64_t s = 2; s <= chunks / 4 && s <= 128 && rows * (s - 1) < 2 * sms; ++s) {
-        const int64_t c0 = ceil_div(chunks, s);
-        int64_t u = sms / (rows * (s - 1));
-        if (u > c0 / 2) u = c0 / 2;
-        if (u < 1) u = 1;
-        const int64_t sc = ceil_div(c0, u), c = sc * u, n = ceil_div(chunks, c);
-        if (n < 2) continue;
-        const double t = ceil_div(rows * n, sms) * (c + 3.0) + ceil_div(rows * (n - 1) * u, sms) * (0.6 * sc + 3.0) + 6.0;
-        if (t < cost) cost = t, nseg = (int)n, cps = (int)c, sub = (int)u, scps = (int)sc;
+    for (int v = 1; v <= (width_c > 64 ? 2 : 1); ++v) {
+        const double chunk = v == 2 ? 0.75 : 1.0;
+        const int64_t r = rows * v;
+        for (int64_t s = 1; s <= chunks / 4 + 1 && s <= 128 && r * (s - 1) < 2 * sms; ++s) {
+            const int64_t c0 = ceil_div(chunks, s);
+            int64_t u = s > 1 ? sms / (r * (s - 1)) : 1;
+            if (u > c0 / 2) u = c0 / 2;
+            if (u < 1) u = 1;
+            const int64_t sc = ceil_div(c0, u), c = sc * u, n = ceil_div(chunks, c);
+            if (s > 1 && n < 2) continue;
+            double t = ceil_div(r * n, sms) * (chunk * c + 3.0);
+            if (n > 1) t += ceil_div(r * (n - 1) * u, sms) * (0.6 * chunk * sc + 3.0) + 6.0;
+            if (t < cost) cost = t, best = WalkSplit{(int)n, (int)c, (int)u, (int)sc, v};
+        }
     }
+    return best;
 }
 
-int decay_walk_tc_launch(const bdm_decay_walk_args &w, Params p, int sub, int scps, void *workspace, cudaStream_t st) {
+int decay_walk_tc_launch(const bdm_decay_walk_args &w, Params p, const WalkSplit &split, void *workspace, cudaStream_t st) {
     EncodeTiled fn = encode_tiled();
     if (!fn) return BDM_ERR_UNSUPPORTED;
     TcParams tp{};
@@ -108,17 +116,19 @@ int decay_walk_tc_launch(const bdm_decay_walk_args &w, Params p, int sub, int sc
     }
     p.seg = static_cast<float *>(workspace);
     tp.p = p;
-    tp.sub = sub;
-    tp.scps = scps;
+    tp.sub = split.sub;
+    tp.scps = split.scps;
+    tp.vsplit = split.vsplit;
     tp.z = p.seg + p.batch * p.heads * p.nseg * (int64_t)p.wab * p.wc;
     // ragged rows in more than one wave (24 x 1333, 192 CTAs: 62 us in the order of the batch, 43 us sorted); a
     // CTA's sort is a loop over the batch, so large batches, whose many waves level out by themselves, go without
-    tp.longest_first = p.lengths && p.batch > 1 && p.batch <= 256 && p.batch * p.heads * p.nseg > kNumSMs;
+    tp.longest_first = p.lengths && p.batch > 1 && p.batch <= 256 && p.batch * p.heads * p.nseg * split.vsplit > kNumSMs;
     const int terms = p.state_out ? 3 : 2;
-    auto run = p.wab > 64 ? (p.wc > 64 ? tc_launch_22 : tc_launch_21) : (p.wc > 64 ? tc_launch_12 : tc_launch_11);
+    const bool wide = p.wc > 64 && split.vsplit == 1;
+    auto run = p.wab > 64 ? (wide ? tc_launch_22 : tc_launch_21) : (wide ? tc_launch_12 : tc_launch_11);
     if (p.nseg > 1) {
         if (int rc = run(tp, maps, kTcState, terms, false, st)) return rc;
-        if (int rc = decay_prefix_launch(p, tp.z, sub, scps, st)) return rc;
+        if (int rc = decay_prefix_launch(p, tp.z, split.sub, split.scps, st)) return rc;
     }
     return run(tp, maps, w.out_dtype == BDM_F32 ? kTcFloat : kTcBf16, terms, p.nseg > 1 || w.overlap, st);
 }

@@ -21,6 +21,7 @@
 // shared-memory operand it took 768 more of its cycles per chunk.
 // The roles' loops are kept short on purpose: five roles' unrolled code does not fit the instruction cache
 // (2048 tokens x 148 heads of 128: 100 us unrolled, 78 us rolled, with one set of roles).
+// Wider values than 64 take one CTA with 128 lanes, or, where rows are few, two with 64 columns each.
 // The scores, and value widths up to 64, use M = 64 products, whose 64 rows are 16 lanes of each quadrant, so
 // that all four schedulers share the work; wider values use all 128 lanes.
 // Every wait is bounded; one that gives up sets the status word and lets the CTA drain.
@@ -63,6 +64,7 @@ struct TcParams {
     int amul[3], bmul[3];  // 0 where the operand's batch (head) is shared by all: a, b, c
     int sub, scps;         // state launch: sub-segments of a segment, chunks of one
     int longest_first;     // rows are dealt out by length
+    int vsplit;            // CTAs that share a row's value columns, 64 each (1: one has them all)
     float *z;              // its states, [batch*heads, (nseg - 1) * sub, wc * wab]
 };
 
@@ -162,6 +164,8 @@ __global__ void __launch_bounds__(kTcThreads, 1) decay_walk_tc_kernel(const TcPa
     char *sP = smem + stages * kStage;
 
     int64_t id = blockIdx.x;
+    const int voff = tp.vsplit > 1 ? (int)(id % tp.vsplit) * 64 : 0;  // neighbours read the same a and b
+    id /= tp.vsplit;
     const int segs = STATE_ONLY ? (p.nseg - 1) * tp.sub : p.nseg;
     const int seg = (int)(id % segs);
     int64_t bh = id / segs;
@@ -329,7 +333,7 @@ __global__ void __launch_bounds__(kTcThreads, 1) decay_walk_tc_kernel(const TcPa
         // Fragments: S[d][4 b + 2 r + e] is key column k0 + 8 b + 2 (lane % 4) + e of value column
         // quad * kQuadCols + 16 d + 8 r + lane / 4.
         constexpr int KC = DK / 2;
-        const int k0 = (warp >> 2) * KC, kl = k0 + 2 * (lane & 3), v0 = quad * kQuadCols + (lane >> 2);
+        const int k0 = (warp >> 2) * KC, kl = k0 + 2 * (lane & 3), v0 = voff + quad * kQuadCols + (lane >> 2);
         const int64_t size = (int64_t)p.wab * p.wc;
         F2 S[kHalves][KC / 4];
 #pragma unroll
@@ -476,7 +480,7 @@ __global__ void __launch_bounds__(kTcThreads, 1) decay_walk_tc_kernel(const TcPa
                     } else {
 #pragma unroll
                         for (int e = 0; e < 8; ++e) {
-                            const int r = r0 + e / 2 * 8, c = quad * kQuadCols + d * 16 + (e & 1) * 8 + (lane >> 2);
+                            const int r = r0 + e / 2 * 8, c = voff + quad * kQuadCols + d * 16 + (e & 1) * 8 + (lane >> 2);
                             const float2 v = split2(x[e]);
                             OT *o = out + (int64_t)(t0 + r) * p.os[1] + c;
                             if (c < p.wc && t0 + r < time) o[0] = r < valid ? v.x : 0.f;
@@ -495,7 +499,7 @@ __global__ void __launch_bounds__(kTcThreads, 1) decay_walk_tc_kernel(const TcPa
                     if (!wait_warp(&bar.ofull, n & 1)) break;
                     if (lane == 0) {
 #pragma unroll
-                        for (int i = 0; i < VB; ++i) tc::tma_store_4d(&maps.out, stage + i * kBox, i * 64, t0, h, (int)b);
+                        for (int i = 0; i < VB; ++i) tc::tma_store_4d(&maps.out, stage + i * kBox, voff + i * 64, t0, h, (int)b);
                         tc::tma_store_commit();
                     }
                 }
@@ -648,7 +652,7 @@ __global__ void __launch_bounds__(kTcThreads, 1) decay_walk_tc_kernel(const TcPa
                     tc::tma_load_4d(dst + kOffB + i * kBox, &maps.b, i * 64, t0, hk, bb, &bar.full[st]);
                 }
 #pragma unroll
-                for (int i = 0; i < VB; ++i) tc::tma_load_4d(dst + kOffC + i * kBox, &maps.c, i * 64, t0, hc, bc, &bar.full[st]);
+                for (int i = 0; i < VB; ++i) tc::tma_load_4d(dst + kOffC + i * kBox, &maps.c, voff + i * 64, t0, hc, bc, &bar.full[st]);
                 issued = n + 1;
                 if (++st == stages) st = 0, phase ^= 1;
             }
@@ -666,9 +670,9 @@ __global__ void __launch_bounds__(kTcThreads, 1) decay_walk_tc_kernel(const TcPa
         const int64_t s0 = (int64_t)seg * p.cps * kChunk, s1 = s0 + (int64_t)p.cps * kChunk;
         if (z0 < s0) z0 = s0;
         if (z1 > s1) z1 = s1;
-        OT *out = static_cast<OT *>(p.out) + b * p.os[0] + h * p.os[2];
+        OT *out = static_cast<OT *>(p.out) + b * p.os[0] + h * p.os[2] + voff;
         constexpr int kLane = sizeof(OT) == 2 ? 8 : 1;  // BF16 rows are whole 16-byte units (TMA writes them too)
-        const int units = p.wc / kLane, per = kTcThreads / units;
+        const int cols = tp.vsplit > 1 ? min(p.wc - voff, 64) : p.wc, units = cols / kLane, per = kTcThreads / units;
         const int row = threadIdx.x / units, unit = threadIdx.x % units;
         if (row < per)
             for (int64_t t = z0 + row; t < z1; t += per) {
@@ -708,7 +712,7 @@ int tc_launch(const TcParams &tp, const Maps &maps, bool dependent, cudaStream_t
             set[dev] = true;
         }
     }
-    const int64_t blocks = tp.p.batch * tp.p.heads * (STATE_ONLY ? (int64_t)(tp.p.nseg - 1) * tp.sub : (int64_t)tp.p.nseg);
+    const int64_t blocks = tp.p.batch * tp.p.heads * tp.vsplit * (STATE_ONLY ? (int64_t)(tp.p.nseg - 1) * tp.sub : (int64_t)tp.p.nseg);
     if (blocks > 0x7fffffff) return BDM_ERR_UNSUPPORTED;
     cudaLaunchConfig_t cfg{};
     cfg.gridDim = dim3((unsigned)blocks);
