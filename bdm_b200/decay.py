@@ -36,7 +36,7 @@ def _raw_stream(device) -> int:
 
 def _rows(x):
     """Columns of a head contiguous; every other stride is free."""
-    return x if x.stride(-1) == 1 or x.shape[-1] == 1 else x.contiguous()
+    return x if x.stride(-1) == 1 else x.contiguous()
 
 
 # bdm_decay_walk_args and bdm_decay_step_args (include/bdm_b200.h), packed in one go: filling a ctypes
@@ -137,17 +137,18 @@ class _DecayAttention(torch.autograd.Function):
 
 
 def _check_heads(q, k, v, log_decay, scale):
-    dev, dt = q.device, q.dtype
-    if not (q.is_cuda and k.is_cuda and v.is_cuda and log_decay.is_cuda):
+    """Shapes [..., heads, width] with the same leading sizes (1 or 2); returns the scale."""
+    dt, at = q.dtype, q.get_device()
+    if at < 0 or k.get_device() != at or v.get_device() != at or log_decay.get_device() != at:
         ops._cuda(q, k, v, log_decay)
+        raise ValueError('q, k, v and log_decay must be on one device')
     if k.dtype != dt or v.dtype != dt:
         raise ValueError('q, k and v must share one dtype')
     ops.dtype_code(dt)
-    if k.device != dev or v.device != dev or log_decay.device != dev:
-        raise ValueError('q, k, v and log_decay must be on one device')
     qs, ks, vs = q.shape, k.shape, v.shape
     heads, kv_heads, dk = qs[-2], ks[-2], qs[-1]
-    if ks[-1] != dk or vs[-2] != kv_heads or ks[:-2] != qs[:-2] or vs[:-2] != qs[:-2]:
+    if (ks[-1] != dk or vs[-2] != kv_heads or ks[0] != qs[0] or vs[0] != qs[0]
+            or (len(qs) == 4 and (ks[1] != qs[1] or vs[1] != qs[1]))):
         raise ValueError('k must be [..., kv_heads, key width of q] and v [..., kv_heads, value width], '
                          'with the leading sizes of q')
     if heads < 1 or kv_heads < 1 or dk < 1 or vs[-1] < 1 or heads % kv_heads:
@@ -156,14 +157,17 @@ def _check_heads(q, k, v, log_decay, scale):
         raise ValueError(f'log_decay must be a contiguous float32 [{heads}] tensor')
     if log_decay.requires_grad and torch.is_grad_enabled():
         raise ValueError('log_decay is a constant: it gets no gradient')
-    scale = dk ** -0.5 if scale is None else float(scale)
+    if scale is None:
+        return dk ** -0.5
+    scale = float(scale)
     if not math.isfinite(scale) or scale == 0.0:
         raise ValueError('scale must be finite and not 0')
     return scale
 
 
 def _check_state(name, state, shape, device):
-    if state.dtype != torch.float32 or tuple(state.shape) != shape or state.device != device or not state.is_contiguous():
+    if (state.dtype != torch.float32 or state.shape != shape or state.get_device() != device.index
+            or not state.is_contiguous()):
         raise ValueError(f'{name} must be a contiguous float32 {list(shape)} tensor on {device}')
 
 
@@ -185,7 +189,7 @@ def decay_attention(q, k, v, log_decay, *, scale=None, initial_state=None, lengt
     batch = q.shape[0]
     if initial_state is not None:
         _check_state('initial_state', initial_state, (batch, q.shape[2], q.shape[3], v.shape[3]), q.device)
-    if lengths is not None and (lengths.dtype != torch.int64 or tuple(lengths.shape) != (batch,)
+    if lengths is not None and (lengths.dtype != torch.int64 or lengths.shape != (batch,)
                                 or lengths.device != q.device or not lengths.is_contiguous()):
         raise ValueError(f'lengths must be a contiguous int64 [{batch}] tensor on {q.device}')
     if q.shape[3] > 128 or v.shape[3] > 128:
@@ -219,7 +223,8 @@ def decay_attention_step(q, k, v, log_decay, state, *, scale=None):
     q, k, v = _rows(q), _rows(k), _rows(v)
     out = torch.empty((batch, heads, dv), dtype=q.dtype, device=q.device)
     a = _STEP.pack(q.data_ptr(), k.data_ptr(), v.data_ptr(), log_decay.data_ptr(), state.data_ptr(), out.data_ptr(),
-                   *q.stride()[:2], *k.stride()[:2], *v.stride()[:2], batch, heads, k.shape[1], dk, dv,
+                   q.stride(0), q.stride(1), k.stride(0), k.stride(1), v.stride(0), v.stride(1), batch, heads,
+                   k.shape[1], dk, dv,
                    ops._DT[q.dtype], scale)
     with _on(q.device):
         status = _lib.load().bdm_decay_step(a, _raw_stream(q.device))
