@@ -5,7 +5,7 @@
 // a b runs on the tensor cores as three TF32 products, a1 b1 + a1 b2 + a2 b1 with a = a1 + a2 + r, |r| <= 2^-22 |a|
 // (the method of splitting an operand into its rounding and the remainder), summed in FP32: about 3e-7 beside
 // FP32's own 1e-7, where plain TF32 gives 5e-4.  Sums and states are FP32.  Bound: the TF32 products' rate and
-// the latency of a chunk's phases (2 x 4096 tokens x 8 heads of 128: 440 us; 3 x 777 x 6 heads of 40 / 72: 48 us
+// the latency of a chunk's phases (2 x 4096 tokens x 8 heads of 128: 365 us; 3 x 777 x 6 heads of 40 / 72: 48 us
 // in three launches, on FP32 FMAs with the same tiles 72).
 #include "decay_walk.cuh"
 
@@ -16,7 +16,6 @@ namespace {
 
 using namespace walk;
 
-constexpr int kThreads = 256;
 constexpr int kCols = 64;  // columns of c per CTA
 
 constexpr int kColPitch = kCols + 8;    // C, S: 8 banks from row to row
@@ -47,9 +46,9 @@ __device__ __forceinline__ void mma_tf32(float (&d)[4], const uint32_t (&a)[4], 
         : "+f"(d[0]), "+f"(d[1]), "+f"(d[2]), "+f"(d[3])
         : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
 }
-// d[n] += a (16 x 8) b (8 x 8, columns 8 n), n < 4.  a(i): element i of this lane's fragment (rows g, g + 8, then
+// d[n] += a (16 x 8) b (8 x 8, columns 8 n), n < N.  a(i): element i of this lane's fragment (rows g, g + 8, then
 // the same rows 4 columns on); b(n, i): element i of tile n (rows t, t + 4).  g = lane / 4, t = lane % 4.
-template <typename FA, typename FB> __device__ __forceinline__ void mma_step(float (&d)[4][4], FA a, FB b) {
+template <int N, typename FA, typename FB> __device__ __forceinline__ void mma_step(float (&d)[N][4], FA a, FB b) {
     uint32_t big[4], small[4];
 #pragma unroll
     for (int i = 0; i < 4; ++i) {
@@ -57,7 +56,7 @@ template <typename FA, typename FB> __device__ __forceinline__ void mma_step(flo
         big[i] = s.big, small[i] = s.small;
     }
 #pragma unroll
-    for (int n = 0; n < 4; ++n) {
+    for (int n = 0; n < N; ++n) {
         const Split32 b0 = split32(b(n, 0)), b1 = split32(b(n, 1));
         // The tensor core cuts its sums off rather than rounding them: over a long sum that is a drift (2.5e-6 after
         // 20000 tokens).  So its sums are of 8 products, and they are added up by FP32 additions.
@@ -71,8 +70,8 @@ template <typename FA, typename FB> __device__ __forceinline__ void mma_step(flo
 }
 
 // Rows [t0, t0 + 64) of one head into shared memory as FP32; invalid rows and columns are zero.  A warp takes
-// every 8th row, its lanes neighbouring columns; four rows' loads are in flight at a time.
-template <typename T>
+// every WARPS-th row, its lanes neighbouring columns; four rows' loads are in flight at a time.
+template <int WARPS, typename T>
 __device__ __forceinline__ void load_rows(float *dst, int pitch, const T *src, int64_t st, int64_t t0, int valid, int first,
                                           int width, int cols) {
     const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
@@ -80,23 +79,27 @@ __device__ __forceinline__ void load_rows(float *dst, int pitch, const T *src, i
         const bool in = first + d < width;
         const T *p = src + t0 * st + first + d;
 #pragma unroll
-        for (int u0 = 0; u0 < kChunk / 8; u0 += 4) {
+        for (int u0 = 0; u0 < kChunk / WARPS; u0 += 4) {
             float x[4];
 #pragma unroll
             for (int u = 0; u < 4; ++u) {
-                const int r = warp + (u0 + u) * 8;
+                const int r = warp + (u0 + u) * WARPS;
                 x[u] = in && r < valid ? Elem<T>::to_float(p[r * st]) : 0.f;
             }
 #pragma unroll
-            for (int u = 0; u < 4; ++u) dst[(warp + (u0 + u) * 8) * pitch + d] = x[u];
+            for (int u = 0; u < 4; ++u) dst[(warp + (u0 + u) * WARPS) * pitch + d] = x[u];
         }
     }
 }
 
-// One CTA walks one segment of one (row, head) for 64 columns of c.  Warp tiles are 16 x 32: P and the outputs
-// have 4 x 2, one a warp; the state has up to 8 x 2, warp w has tiles w and w + 8.
-template <typename T, typename OT, bool STATE_ONLY>
-__global__ void __launch_bounds__(kThreads) decay_walk_kernel(const Params p) {
+// One CTA walks one segment of one (row, head) for 64 columns of c.  With 8 warps, P and the outputs are 4 x 2
+// warp tiles of 16 x 32 and a warp has two of the state's up to 8 x 2 tiles of that size; with 16 warps, 4 x 4 of
+// 16 x 16 and one of the state's.  Shared memory decides: up to 80 columns of a and b two or three CTAs of 8 warps
+// share an SM (3 x 777 x 6 heads of 40 / 72: 48 us, with 16 warps 62), past that one of 16 hides more latency than
+// one of 8 (2 x 4096 x 8 heads of 128: 365 us, with 8 warps 441, issuing in 38 % of the cycles).
+template <int WARPS, typename T, typename OT, bool STATE_ONLY>
+__global__ void __launch_bounds__(WARPS * 32) decay_walk_kernel(const Params p) {
+    constexpr int kThreads = WARPS * 32, N = 32 / WARPS, ST = 16 / WARPS;
     extern __shared__ float sm[];
     const int slices = (p.wc + kCols - 1) / kCols;
     int64_t id = blockIdx.x;
@@ -125,18 +128,17 @@ __global__ void __launch_bounds__(kThreads) decay_walk_kernel(const Params p) {
 
     const Span sp = span_of(p, row_tokens(p, b), seg);
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, lg = lane >> 2, lt = lane & 3;
-    const int mrow = (warp & 3) * 16, ncol = (warp >> 2) * 32;  // this warp's tile of P and of the outputs
+    const int mrow = (warp & 3) * 16, ncol = (warp >> 2) * 8 * N;  // this warp's tile of P and of the outputs
     const T *a = static_cast<const T *>(p.a) + b * p.as[0] + (h / p.ag) * p.as[2];
     const T *bb = static_cast<const T *>(p.b) + b * p.bs[0] + (h / p.bg) * p.bs[2];
     const T *c = static_cast<const T *>(p.c) + b * p.cs[0] + (h / p.cg) * p.cs[2];
     OT *out = static_cast<OT *>(p.out) + b * p.os[0] + h * p.os[2];
     const int64_t size = (int64_t)p.wab * p.wc;
 
-    // state tile q: rows srow(q) + lg (+ 8), columns scol(q) + 8 n + 2 lt + {0, 1}; element (n, i) is row lg + 8 (i / 2)
-    const int stiles = width / 8;
-    auto srow = [&](int q) { return (warp + 8 * q) / 2 * 16; };
-    auto scol = [&](int q) { return (warp + 8 * q) % 2 * 32; };
-    float S[2][4][4];
+    // state tile q: rows srow(q) + lg (+ 8), columns scol + 8 n + 2 lt + {0, 1}; element (n, i) is row lg + 8 (i / 2)
+    const int scol = warp % 2 * 32;
+    auto srow = [&](int q) { return (warp + WARPS * q) / 2 * 16; };
+    float S[ST][4][4];
     {
         const bool before = !STATE_ONLY && p.nseg > 1 && (p.reverse ? seg < p.nseg - 1 : seg > 0);
         const float *zs = before ? p.seg + (bh * p.nseg + seg) * size : nullptr;
@@ -148,12 +150,12 @@ __global__ void __launch_bounds__(kThreads) decay_walk_kernel(const Params p) {
             given = (far ? expf(g * (float)far) : 1.f) * p.in_mul;
         }
 #pragma unroll
-        for (int q = 0; q < 2; ++q)
+        for (int q = 0; q < ST; ++q)
 #pragma unroll
             for (int n = 0; n < 4; ++n)
 #pragma unroll
                 for (int i = 0; i < 4; ++i) {
-                    const int k = srow(q) + lg + 8 * (i >> 1), v = n0 + scol(q) + 8 * n + 2 * lt + (i & 1);
+                    const int k = srow(q) + lg + 8 * (i >> 1), v = n0 + scol + 8 * n + 2 * lt + (i & 1);
                     const bool in = k < p.wab && v < p.wc;
                     S[q][n][i] = 0.f;
                     if (zs) {
@@ -173,25 +175,25 @@ __global__ void __launch_bounds__(kThreads) decay_walk_kernel(const Params p) {
         const int valid = (int)(sp.n - t0 < kChunk ? sp.n - t0 : kChunk);
         __syncthreads();  // the tiles of the previous chunk are done with
         if (!STATE_ONLY) {
-            load_rows<T>(sA, pitch, a, p.as[1], t0, valid, 0, p.wab, width);
+            load_rows<WARPS, T>(sA, pitch, a, p.as[1], t0, valid, 0, p.wab, width);
 #pragma unroll
-            for (int q = 0; q < 2; ++q)
-                if (warp + 8 * q < stiles)
+            for (int q = 0; q < ST; ++q)
+                if (srow(q) < width)
 #pragma unroll
                     for (int n = 0; n < 4; ++n)
 #pragma unroll
                         for (int i = 0; i < 4; i += 2)
-                            *reinterpret_cast<float2 *>(&sS[(srow(q) + lg + 4 * i) * kColPitch + scol(q) + 8 * n + 2 * lt]) =
+                            *reinterpret_cast<float2 *>(&sS[(srow(q) + lg + 4 * i) * kColPitch + scol + 8 * n + 2 * lt]) =
                                 make_float2(S[q][n][i], S[q][n][i + 1]);
         }
-        load_rows<T>(sB, pitch, bb, p.bs[1], t0, valid, 0, p.wab, width);
-        load_rows<T>(sC, kColPitch, c, p.cs[1], t0, valid, n0, p.wc, kCols);
+        load_rows<WARPS, T>(sB, pitch, bb, p.bs[1], t0, valid, 0, p.wab, width);
+        load_rows<WARPS, T>(sC, kColPitch, c, p.cs[1], t0, valid, n0, p.wc, kCols);
         __syncthreads();
 
         if (!STATE_ONLY) {
             // P = A B^T with the decay between the rows; tiles that the mask empties are only cleared
-            float d[4][4] = {};
-            if (p.reverse ? ncol + 31 >= mrow : ncol <= mrow + 15) {
+            float d[N][4] = {};
+            if (p.reverse ? ncol + 8 * N - 1 >= mrow : ncol <= mrow + 15) {
                 const float *fa = sA + (mrow + lg) * pitch + lt, *fb = sB + (ncol + lg) * pitch + lt;
 #pragma unroll 2
                 for (int k = 0; k < width; k += 8)
@@ -199,7 +201,7 @@ __global__ void __launch_bounds__(kThreads) decay_walk_kernel(const Params p) {
                              [&](int n, int i) { return fb[n * 8 * pitch + i * 4 + k]; });
             }
 #pragma unroll
-            for (int n = 0; n < 4; ++n)
+            for (int n = 0; n < N; ++n)
 #pragma unroll
                 for (int i = 0; i < 4; i += 2) {
                     const int r = mrow + lg + 4 * i, j = ncol + 8 * n + 2 * lt;
@@ -209,7 +211,7 @@ __global__ void __launch_bounds__(kThreads) decay_walk_kernel(const Params p) {
                 }
             __syncthreads();
             // out = scale * (lam^. A S + P C)
-            float o[4][4] = {};
+            float o[N][4] = {};
             {
                 const float *fa = sA + (mrow + lg) * pitch + lt, *fs = sS + lt * kColPitch + ncol + lg;
 #pragma unroll 2
@@ -223,7 +225,7 @@ __global__ void __launch_bounds__(kThreads) decay_walk_kernel(const Params p) {
                 const int e = p.reverse ? valid - 1 - r : r + 1;
                 const float w = e >= 0 ? pw[e] : 0.f;
 #pragma unroll
-                for (int n = 0; n < 4; ++n) o[n][i] *= w;
+                for (int n = 0; n < N; ++n) o[n][i] *= w;
             }
             {
                 const float *fp = sP + (mrow + lg) * kScorePitch + lt, *fc = sC + lt * kColPitch + ncol + lg;
@@ -234,7 +236,7 @@ __global__ void __launch_bounds__(kThreads) decay_walk_kernel(const Params p) {
                              [&](int n, int i) { return fc[(k + i * 4) * kColPitch + n * 8]; });
             }
 #pragma unroll
-            for (int n = 0; n < 4; ++n)
+            for (int n = 0; n < N; ++n)
 #pragma unroll
                 for (int i = 0; i < 4; ++i) {
                     const int r = mrow + lg + 8 * (i >> 1), j = n0 + ncol + 8 * n + 2 * lt + (i & 1);
@@ -246,13 +248,13 @@ __global__ void __launch_bounds__(kThreads) decay_walk_kernel(const Params p) {
         if (!STATE_ONLY && step + 1 == sp.c1 - sp.c0 && !(p.state_out && sp.last)) break;
         const float carry = pw[valid];
 #pragma unroll
-        for (int q = 0; q < 2; ++q) {
-            if (warp + 8 * q >= stiles) continue;
+        for (int q = 0; q < ST; ++q) {
+            if (srow(q) >= width) continue;
 #pragma unroll
             for (int n = 0; n < 4; ++n)
 #pragma unroll
                 for (int i = 0; i < 4; ++i) S[q][n][i] *= carry;
-            const float *fb = sB + lt * pitch + srow(q) + lg, *fc = sC + lt * kColPitch + scol(q) + lg;
+            const float *fb = sB + lt * pitch + srow(q) + lg, *fc = sC + lt * kColPitch + scol + lg;
             for (int k = 0; k < valid; k += 8) {  // rows past `valid` are zero
                 float w[2];
 #pragma unroll
@@ -269,13 +271,13 @@ __global__ void __launch_bounds__(kThreads) decay_walk_kernel(const Params p) {
     if (STATE_ONLY || (p.state_out && sp.last)) {
         float *z = STATE_ONLY ? p.seg + (bh * segs + zid) * size : p.state_out + bh * size;
 #pragma unroll
-        for (int q = 0; q < 2; ++q)
+        for (int q = 0; q < ST; ++q)
 #pragma unroll
             for (int n = 0; n < 4; ++n)
 #pragma unroll
                 for (int i = 0; i < 4; ++i) {
-                    const int k = srow(q) + lg + 8 * (i >> 1), v = n0 + scol(q) + 8 * n + 2 * lt + (i & 1);
-                    if (warp + 8 * q >= stiles || k >= p.wab || v >= p.wc) continue;
+                    const int k = srow(q) + lg + 8 * (i >> 1), v = n0 + scol + 8 * n + 2 * lt + (i & 1);
+                    if (k >= p.wab || v >= p.wc) continue;
                     if (STATE_ONLY)
                         z[k * p.wc + v] = S[q][n][i];
                     else
@@ -356,9 +358,10 @@ int device_setup(int &sms) {
     std::lock_guard<std::mutex> lock(g_mu);
     if (!g_attr[dev]) {
         const void *fns[] = {
-            (const void *)decay_walk_kernel<float, float, false>, (const void *)decay_walk_kernel<float, float, true>,
-            (const void *)decay_walk_kernel<bf16, bf16, false>, (const void *)decay_walk_kernel<bf16, float, false>,
-            (const void *)decay_walk_kernel<bf16, bf16, true>};
+            (const void *)decay_walk_kernel<8, float, float, false>, (const void *)decay_walk_kernel<16, float, float, false>,
+            (const void *)decay_walk_kernel<8, bf16, bf16, false>,   (const void *)decay_walk_kernel<16, bf16, bf16, false>,
+            (const void *)decay_walk_kernel<8, bf16, float, false>,  (const void *)decay_walk_kernel<16, bf16, float, false>,
+            (const void *)decay_walk_kernel<8, float, float, true>,  (const void *)decay_walk_kernel<8, bf16, bf16, true>};
         for (const void *f : fns)
             if (int rc = cuda_status(cudaFuncSetAttribute(f, cudaFuncAttributeMaxDynamicSharedMemorySize,
                                                           walk_smem(kMaxWidth, false))))
@@ -375,7 +378,7 @@ template <typename T, typename OT> int walk_launch(Params p, void *workspace, cu
     const int64_t rows = p.batch * p.heads, slices = ceil_div(p.wc, kCols), size = (int64_t)p.wab * p.wc;
     if (rows * slices * p.nseg > 0x7fffffff) return BDM_ERR_UNSUPPORTED;
     cudaLaunchConfig_t cfg{};
-    cfg.blockDim = dim3(kThreads);
+    cfg.blockDim = dim3(256);
     cfg.stream = st;
     cudaLaunchAttribute attr{};
     attr.id = cudaLaunchAttributeProgrammaticStreamSerialization;
@@ -388,14 +391,17 @@ template <typename T, typename OT> int walk_launch(Params p, void *workspace, cu
         q.seg = z;
         cfg.gridDim = dim3((unsigned)(rows * slices * (p.nseg - 1)));
         cfg.dynamicSmemBytes = walk_smem(p.wab, true);
-        if (int rc = cuda_status(cudaLaunchKernelEx(&cfg, decay_walk_kernel<T, T, true>, (const Params)q))) return rc;
+        if (int rc = cuda_status(cudaLaunchKernelEx(&cfg, decay_walk_kernel<8, T, T, true>, (const Params)q))) return rc;
         if (int rc = launch_status()) return rc;
         if (int rc = decay_prefix_launch(p, z, 1, p.cps, st)) return rc;
         cfg.numAttrs = 1;
     }
     cfg.gridDim = dim3((unsigned)(rows * slices * p.nseg));
     cfg.dynamicSmemBytes = walk_smem(p.wab, false);
-    if (int rc = cuda_status(cudaLaunchKernelEx(&cfg, decay_walk_kernel<T, OT, false>, (const Params)p))) return rc;
+    const bool wide = p.wab > 80;  // shared memory holds one CTA
+    cfg.blockDim = dim3(wide ? 512 : 256);
+    auto kernel = wide ? decay_walk_kernel<16, T, OT, false> : decay_walk_kernel<8, T, OT, false>;
+    if (int rc = cuda_status(cudaLaunchKernelEx(&cfg, kernel, (const Params)p))) return rc;
     return launch_status();
 }
 
