@@ -682,6 +682,9 @@ __global__ void __launch_bounds__(kTcThreads, 1) decay_walk_tc_kernel(const TcPa
                     out[t * p.os[1] + unit] = 0.f;
             }
     }
+    // A walk that overlaps the one before it does not end before that one has: what follows in the stream waits for
+    // this walk only.
+    if (!STATE_ONLY) asm volatile("griddepcontrol.wait;\n" ::: "memory");
     if (threadIdx.x == 0 && dead && p.status) *(volatile int *)p.status = 0x4;
     if (warp == kMmaWarp) {
         tc::fence_after_sync();

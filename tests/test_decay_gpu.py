@@ -301,6 +301,20 @@ def test_training_step_in_a_graph():
     assert all(torch.equal(x, y) for x, y in zip(got, want))
 
 
+def test_gradients_are_whole_when_the_next_kernel_starts():
+    """dk and dv may start under dq's end; what follows in the stream must still see all three."""
+    from bdm_b200 import decay_attention
+    q, k, v, do, g, _, _ = _inputs(22, 24, 700, 8, 8, 64, 64, torch.bfloat16, state=False)
+    leaves = [x.requires_grad_(True) for x in (q, k, v)]
+    o = decay_attention(q, k, v, g)
+    torch.cuda.synchronize()
+    want = [x.clone() for x in torch.autograd.grad(o, leaves, do, retain_graph=True)]
+    torch.cuda.synchronize()
+    for _ in range(5):
+        got = [x + 0 for x in torch.autograd.grad(o, leaves, do, retain_graph=True)]
+        assert all(torch.equal(x, y) for x, y in zip(got, want))
+
+
 def test_refusals():
     from bdm_b200 import decay_attention, decay_attention_step
     q, k, v, _, g, s0, _ = _inputs(15, 2, 8, 4, 2, 16, 16, torch.float32)
