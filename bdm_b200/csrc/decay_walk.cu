@@ -30,7 +30,8 @@ int walk_smem(int wab, bool state_only) {
     return f * 4;
 }
 
-// x = big + small, both TF32 operands (the tensor core drops the bits of `small` past TF32's).
+// x = big + small, both TF32 operands (the tensor core drops the bits of `small` past TF32's).  An infinite x gives
+// NaN, as it would in the products of the next chunk anyway.
 struct Split32 {
     uint32_t big, small;
 };
