@@ -113,6 +113,28 @@ __device__ __forceinline__ float exp2_ftz(float x) {
     return y;
 }
 
+// Two FP32 values in one register pair, for the packed FP32 instructions.
+__device__ __forceinline__ u64 pair(float x, float y) {
+    u64 r;
+    asm("mov.b64 %0, {%1, %2};\n" : "=l"(r) : "f"(x), "f"(y));
+    return r;
+}
+__device__ __forceinline__ float2 halves(u64 a) {
+    float2 r;
+    asm("mov.b64 {%0, %1}, %2;\n" : "=f"(r.x), "=f"(r.y) : "l"(a));
+    return r;
+}
+__device__ __forceinline__ u64 add2(u64 a, u64 b) {
+    u64 r;
+    asm("add.rn.f32x2 %0, %1, %2;\n" : "=l"(r) : "l"(a), "l"(b));
+    return r;
+}
+__device__ __forceinline__ u64 mul2(u64 a, u64 b) {
+    u64 r;
+    asm("mul.rn.f32x2 %0, %1, %2;\n" : "=l"(r) : "l"(a), "l"(b));
+    return r;
+}
+
 // The slice's maximum and a lower bound of its K-th largest logit.  Every warp draws its K largest lane maxima
 // (equal ones leave together: the bound is lower then, which is no harm).  For K <= 8 the bound is the K-th
 // largest of all warps' together, which hardly more than K logits reach; past that, the largest of the warps'
@@ -157,7 +179,7 @@ __device__ __forceinline__ void slice_bound(float mine, int K, float *redm, floa
 // Joins the warps' sums, collects the candidates that hot(use) names by index (a logit is read again: registers
 // have no index) and writes the K largest.
 template <typename T, typename F>
-__device__ __forceinline__ void finish_slice(float warp_total, float fix, float m, F hot, TopShared &sh, const T *src,
+__device__ __forceinline__ void finish_slice(float warp_total, float m, F hot, TopShared &sh, const T *src,
                                              int base, int count, int vocab, int K, Slice *stat, u64 *dst) {
     __shared__ float reds[kWarps];
     if ((threadIdx.x & 31) == 0) reds[threadIdx.x >> 5] = warp_total;
@@ -171,7 +193,6 @@ __device__ __forceinline__ void finish_slice(float warp_total, float fix, float 
         float t = 0.f;
 #pragma unroll
         for (int w = 0; w < kWarps; ++w) t += reds[w];
-        t *= fix;
         *stat = Slice{t == t ? m : NAN, t};
     }
     const int n = sh.count;
@@ -252,7 +273,7 @@ __global__ void __launch_bounds__(kThreads)
 #pragma unroll
         for (int e = 0; e < E; ++e) s0 += x[e] == -INFINITY ? 0.f : NAN;
     }
-    finish_slice<T>(warp_sum(s0 + s1), 1.f, m, [&](auto &&use) {
+    finish_slice<T>(warp_sum(s0 + s1), m, [&](auto &&use) {
         if (mine < bound) return;
         uint32_t hot = 0;
 #pragma unroll
@@ -262,8 +283,8 @@ __global__ void __launch_bounds__(kThreads)
 }
 
 // The same for BF16 rows that start on 16-byte boundaries, which stay packed: the maximum and the comparisons
-// take two logits an instruction, and exp(x - max) is one packed multiply-add and ex2 (the rounding of
-// max * log2 e, which all terms share, is taken out of the sum at the end).
+// take two logits an instruction, as do the subtraction of the maximum, the multiplication by log2 e and the sum.
+// The subtraction comes first: a slice whose every logit is masked by a large finite value has weights of 1.
 template <int E>
 __global__ void __launch_bounds__(kThreads)
     beam_slice_bf16_kernel(const bf16 *__restrict__ logits, int64_t ld, int vocab, int K, int splits,
@@ -302,25 +323,24 @@ __global__ void __launch_bounds__(kThreads)
     const float mine = fmaxf(__low2float(top2), __high2float(top2));
     float m, bound;
     slice_bound(mine, K, redm, redk, m, bound, sh);
-    float sum = 0.f, fix = 1.f;
+    float sum = 0.f;
     if (m > -INFINITY && m < INFINITY) {
-        constexpr float kLog2e = 1.4426950408889634f;
-        const float c = m * kLog2e;
-        fix = exp2_ftz(-fmaf(m, kLog2e, -c));
-        float s0 = 0.f, s1 = 0.f;
+        const u64 minus = pair(-m, -m), log2e = pair(1.4426950408889634f, 1.4426950408889634f);
+        u64 total = 0;  // two zeros
 #pragma unroll
         for (int i = 0; i < E / 2; ++i) {
-            s0 += exp2_ftz(fmaf(__uint_as_float(r[i] << 16), kLog2e, -c));
-            s1 += exp2_ftz(fmaf(__uint_as_float(r[i] & 0xffff0000u), kLog2e, -c));
+            const float2 y = halves(mul2(add2(pair(__uint_as_float(r[i] << 16), __uint_as_float(r[i] & 0xffff0000u)), minus), log2e));
+            total = add2(total, pair(exp2_ftz(y.x), exp2_ftz(y.y)));
         }
-        sum = s0 + s1;
+        const float2 t = halves(total);
+        sum = t.x + t.y;
     } else if (m == -INFINITY) {  // all -inf, or NaN
 #pragma unroll
         for (int i = 0; i < E / 2; ++i) sum += __hbeq2(two(r[i]), __bfloat162bfloat162(__float2bfloat16_rn(-INFINITY))) ? 0.f : NAN;
     } else {
         sum = NAN;
     }
-    finish_slice<bf16>(warp_sum(sum), fix, m, [&](auto &&use) {
+    finish_slice<bf16>(warp_sum(sum), m, [&](auto &&use) {
         if (mine < bound) return;
         const __nv_bfloat162 b2 = __bfloat162bfloat162(__float2bfloat16_rn(bound));  // a logit: exact
 #pragma unroll
