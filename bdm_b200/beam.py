@@ -17,6 +17,7 @@ from . import _lib, ops
 from .decay import _on, _raw_stream
 
 MAX_BEAMS = 32
+MAX_VOCAB = 2 ** 31 - 2 ** 16
 
 
 class BeamStep(NamedTuple):
@@ -52,8 +53,9 @@ def beam_select(logits, scores, *, finished=None, eos_token=None, stable_slots=F
         raise ValueError('eos_token is outside the vocabulary')
     if scores.device != dev or (finished is not None and finished.device != dev):
         raise ValueError('logits, scores and finished must be on one device')
-    if beams > MAX_BEAMS or beams * vocab >= 2 ** 32 - 1:
-        raise NotImplementedError(f'beam_select supports up to {MAX_BEAMS} beams and beams * vocab < 2^32')
+    if beams > MAX_BEAMS or vocab > MAX_VOCAB or beams * vocab >= 2 ** 32 - 1:
+        raise NotImplementedError(f'beam_select supports up to {MAX_BEAMS} beams, vocab <= {MAX_VOCAB} and '
+                                  f'beams * vocab < 2^32 - 1')
     rows = logits.reshape(batch * beams, vocab)
     if rows.stride(1) != 1 and vocab > 1:
         rows = rows.contiguous()

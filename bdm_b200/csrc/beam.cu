@@ -7,6 +7,7 @@ namespace {
 constexpr int kThreads = 256;
 constexpr int kWarps = kThreads / 32;
 constexpr int kMaxBeams = 32;
+constexpr int64_t kMaxVocab = 0x7fff0000;  // token indices, rounded up to a whole slice, are ints
 constexpr int kList = 1024;  // candidates a CTA collects before it falls back to repeated maxima
 
 using u64 = unsigned long long;
@@ -693,7 +694,9 @@ int reorder_launch(Tensors t, const int64_t *row_bytes, const int64_t *parents, 
 
 extern "C" int64_t bdm_beam_select_workspace_bytes(int64_t batch, int beams, int64_t vocab) {
     using namespace bdm;
-    if (batch < 0 || beams <= 0 || vocab <= 0 || beams > kMaxBeams || vocab * beams >= 0xffffffffll) return -1;
+    if (batch < 0 || beams <= 0 || vocab <= 0 || beams > kMaxBeams || vocab > kMaxVocab ||
+        vocab * beams >= 0xffffffffll)
+        return -1;
     const BeamPlan p = beam_plan(batch * beams, vocab, false);  // never fewer splits than the packed plan's
     return batch * beams * p.splits * ((int64_t)beams * 8 + 8);
 }
@@ -706,7 +709,7 @@ extern "C" int bdm_beam_select(const void *logits, int64_t ld, int64_t batch, in
     if (batch < 0 || beams <= 0 || vocab <= 0 || ld < 0 || eos_token < -1 || eos_token >= vocab) return BDM_ERR_INVALID;
     if (finished && eos_token < 0) return BDM_ERR_INVALID;
     if (!valid_dtype(dtype)) return BDM_ERR_DTYPE;
-    if (beams > kMaxBeams || vocab * beams >= 0xffffffffll) return BDM_ERR_UNSUPPORTED;
+    if (beams > kMaxBeams || vocab > kMaxVocab || vocab * beams >= 0xffffffffll) return BDM_ERR_UNSUPPORTED;
     if (batch == 0) return BDM_OK;
     if (!logits || !scores || !out_scores || !out_parents || !out_tokens) return BDM_ERR_INVALID;
     const int64_t rows = batch * beams;

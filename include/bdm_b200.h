@@ -532,7 +532,7 @@ BDM_API int bdm_decay_step(const bdm_decay_step_args *args, void *stream);
  * `beams` best per batch row, ties to the lower w * vocab + t, in descending order; with stable_slots the
  * best child of each parent takes the parent's place and the others the free places in turn.
  * finished (optional, bytes) needs eos_token >= 0; out_finished (optional) = the parent's | (token == eos).
- * beams <= 32, beams * vocab < 2^32.
+ * beams <= 32, vocab <= 2^31 - 2^16, beams * vocab < 2^32 - 1.
  */
 BDM_API int64_t bdm_beam_select_workspace_bytes(int64_t batch, int beams, int64_t vocab);
 BDM_API int bdm_beam_select(const void *logits, int64_t ld, int64_t batch, int beams, int64_t vocab, int dtype,
