@@ -46,15 +46,18 @@ _STEP = struct.Struct('6P6qq5if')
 
 
 def _walk(a, b, c, log_decay, lengths, st, *, heads, scale, reverse=0, out_dtype=None, state_in=None, state_in_mul=1.0,
-          state_in_transposed=0, state_out=None, state_out_mul=1.0, after=None):
+          state_in_transposed=0, state_out=None, state_out_mul=1.0, out=None, after=None):
     """One bdm_decay_walk over [B, T, heads of the operand, width] tensors; returns out [B, T, heads, width of c].
 
     ``after``: list of the walks already launched for this backward, independent of this one; it may overlap
-    the last of them when that one had no workspace (whose memory this one's output could otherwise reuse)."""
+    the launch before it when the last of them had no workspace.  That launch may be another thread's on the same
+    stream, and what it uses may have been freed since: a walk that may overlap writes only to an ``out`` and a
+    ``state_out`` that were allocated before the backward's first walk, which waits for all earlier launches."""
     batch, time, a_heads, wab = a.shape
     c_heads, wc = c.shape[2:]
     dt = a.dtype
-    out = torch.empty((batch, time, heads, wc), dtype=out_dtype or dt, device=a.device)
+    if out is None:
+        out = torch.empty((batch, time, heads, wc), dtype=out_dtype or dt, device=a.device)
     w = _WALK.pack(a.data_ptr(), b.data_ptr(), c.data_ptr(), out.data_ptr(), log_decay.data_ptr(),
                    0 if lengths is None else lengths.data_ptr(), 0 if state_in is None else state_in.data_ptr(),
                    0 if state_out is None else state_out.data_ptr(), st.mapped_ptr,
@@ -123,15 +126,19 @@ class _DecayAttention(torch.autograd.Function):
         with _on(q.device):
             st = ops._scan_status_of(q.device)
             ops.check_mapped_status(st)
+            # all that overlapping walks write is allocated before the first launch (see _walk)
+            if need[4]:
+                ds0 = torch.empty((q.shape[0], heads, q.shape[3], v.shape[3]), dtype=torch.float32, device=q.device)
+            if not shared:
+                dk = torch.empty(k.shape, dtype=dt, device=q.device) if need[1] else None
+                dv = torch.empty(v.shape, dtype=dt, device=q.device) if need[2] or need[4] else None
             if need[0]:
                 dq = _walk(do, v, k, log_decay, lengths, st, state_in=s0, state_in_transposed=1, **walk)
             if need[1]:
-                dk = _walk(v, do, q, log_decay, lengths, st, state_in_transposed=1, **back)
+                dk = _walk(v, do, q, log_decay, lengths, st, state_in_transposed=1, out=dk, **back)
                 dk = _group_sum(dk, kv_heads, dt) if shared else dk
             if need[2] or need[4]:
-                ds0 = torch.empty((q.shape[0], heads, q.shape[3], v.shape[3]), dtype=torch.float32,
-                                  device=q.device) if need[4] else None
-                dv = _walk(k, q, do, log_decay, lengths, st, state_out=ds0, state_out_mul=scale, **back)
+                dv = _walk(k, q, do, log_decay, lengths, st, state_out=ds0, state_out_mul=scale, out=dv, **back)
                 dv = _group_sum(dv, kv_heads, dt) if shared else dv
         return dq, dk, dv if need[2] else None, None, ds0, None, None, None
 

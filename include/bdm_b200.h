@@ -477,8 +477,10 @@ BDM_API int bdm_decode_token_step(const void *proj, int64_t batch, int64_t ld, i
  * Strides are in elements, in the order batch, token, head; columns are contiguous.  Head h uses head
  * h / (heads / x_heads) of operand x.  States are FP32 [batch, heads, width_ab, width_c], or with
  * *_transposed [batch, heads, width_c, width_ab].  Products, sums and states are FP32.
- * overlap = 1: where the walk is one launch, it may start while the walk launched before it in the stream still
- * runs; the caller knows that neither reads or overwrites what the other writes (dk after dq, dv after dk).
+ * overlap = 1: where the walk is one launch, it may start while the launch before it in the stream still runs, and so
+ * beside everything back to the last walk (or other kernel) that did not overlap, whoever launched it.  The caller
+ * knows that it neither writes what those use nor reads what they write (dk after dq, dv after dk, with all three
+ * outputs allocated before dq is launched).  It ends after the launch before it.
  * width_ab, width_c <= 128.  status (optional, an int the device can write, mapped host
  * memory included): set to 0x4 if a bounded wait gave up; the outputs are then unspecified.
  */
@@ -497,7 +499,7 @@ typedef struct bdm_decay_walk_args {
     int dtype, out_dtype; /* out_dtype: dtype, or BDM_F32 */
     int reverse;
     int state_in_transposed, state_out_transposed;
-    int overlap; /* 1: see below */
+    int overlap; /* 1: see above */
     float scale, state_in_mul, state_out_mul;
 } bdm_decay_walk_args;
 
