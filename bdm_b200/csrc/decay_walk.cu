@@ -30,8 +30,8 @@ int walk_smem(int wab, bool state_only) {
     return f * 4;
 }
 
-// x = big + small, both TF32 operands (the tensor core drops the bits of `small` past TF32's).  An infinite x gives
-// NaN, as it would in the products of the next chunk anyway.
+// x = big + small, both TF32 operands (the tensor core drops the bits of `small` past TF32's).  An infinite x makes
+// its products NaN: what it reaches is not finite either way.
 struct Split32 {
     uint32_t big, small;
 };
@@ -70,12 +70,16 @@ template <int N, typename FA, typename FB> __device__ __forceinline__ void mma_s
     }
 }
 
+__device__ __forceinline__ bool finite(float x) { return fabsf(x) < INFINITY; }
+
 // Rows [t0, t0 + 64) of one head into shared memory as FP32; invalid rows and columns are zero.  A warp takes
-// every WARPS-th row, its lanes neighbouring columns; four rows' loads are in flight at a time.
+// every WARPS-th row, its lanes neighbouring columns; four rows' loads are in flight at a time.  Returns NaN
+// where one of this thread's values is infinite or NaN, else 0.
 template <int WARPS, typename T>
-__device__ __forceinline__ void load_rows(float *dst, int pitch, const T *src, int64_t st, int64_t t0, int valid, int first,
+__device__ __forceinline__ float load_rows(float *dst, int pitch, const T *src, int64_t st, int64_t t0, int valid, int first,
                                           int width, int cols) {
     const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+    float odd = 0.f;
     for (int d = lane; d < cols; d += 32) {
         const bool in = first + d < width;
         const T *p = src + t0 * st + first + d;
@@ -88,9 +92,12 @@ __device__ __forceinline__ void load_rows(float *dst, int pitch, const T *src, i
                 x[u] = in && r < valid ? Elem<T>::to_float(p[r * st]) : 0.f;
             }
 #pragma unroll
+            for (int u = 0; u < 4; ++u) odd = fmaf(x[u], 0.f, odd);
+#pragma unroll
             for (int u = 0; u < 4; ++u) dst[(warp + (u0 + u) * WARPS) * pitch + d] = x[u];
         }
     }
+    return odd;
 }
 
 // One CTA walks one segment of one (row, head) for 64 columns of c.  With 8 warps, P and the outputs are 4 x 2
@@ -102,6 +109,8 @@ template <int WARPS, typename T, typename OT, bool STATE_ONLY>
 __global__ void __launch_bounds__(WARPS * 32) decay_walk_kernel(const Params p) {
     constexpr int kThreads = WARPS * 32, N = 32 / WARPS, ST = 16 / WARPS;
     extern __shared__ float sm[];
+    __shared__ int odd_step;         // the last step that met a c that is not finite
+    __shared__ int odd_from[kCols];  // of a chunk where c is not finite: each column's first such row (reverse: last)
     const int slices = (p.wc + kCols - 1) / kCols;
     int64_t id = blockIdx.x;
     const int segs = STATE_ONLY ? p.nseg - 1 : p.nseg;
@@ -170,6 +179,7 @@ __global__ void __launch_bounds__(WARPS * 32) decay_walk_kernel(const Params p) 
                 }
     }
 
+    if (threadIdx.x == 0) odd_step = -1;
     for (int64_t step = 0; step < sp.c1 - sp.c0; ++step) {
         const int64_t ch = p.reverse ? sp.c1 - 1 - step : sp.c0 + step;
         const int64_t t0 = ch * kChunk;
@@ -188,8 +198,26 @@ __global__ void __launch_bounds__(WARPS * 32) decay_walk_kernel(const Params p) 
                                 make_float2(S[q][n][i], S[q][n][i + 1]);
         }
         load_rows<WARPS, T>(sB, pitch, bb, p.bs[1], t0, valid, 0, p.wab, width);
-        load_rows<WARPS, T>(sC, kColPitch, c, p.cs[1], t0, valid, n0, p.wc, kCols);
+        const float odd = load_rows<WARPS, T>(sC, kColPitch, c, p.cs[1], t0, valid, n0, p.wc, kCols);
+        if (!STATE_ONLY && odd != odd) odd_step = (int)step;
         __syncthreads();
+        const bool odd_chunk = !STATE_ONLY && odd_step == (int)step;
+        if (odd_chunk) {
+            // c has values that are not finite, which a masked score of zero would turn into NaN: they count as zero in
+            // the product with the scores.  What they do reach, the column's outputs from there on, is set to NaN after
+            // it, and so is the value that the state takes in.
+            if (threadIdx.x < kCols) {
+                float *col = sC + threadIdx.x;
+                int from = p.reverse ? -1 : kChunk;
+                for (int r = 0; r < kChunk; ++r)
+                    if (!finite(col[r * kColPitch])) {
+                        from = p.reverse ? r : min(from, r);
+                        col[r * kColPitch] = 0.f;
+                    }
+                odd_from[threadIdx.x] = from;
+            }
+            __syncthreads();
+        }
 
         if (!STATE_ONLY) {
             // P = A B^T with the decay between the rows; tiles that the mask empties are only cleared
@@ -244,6 +272,16 @@ __global__ void __launch_bounds__(WARPS * 32) decay_walk_kernel(const Params p) 
                     if (t0 + r < p.time && j < p.wc)
                         out[(t0 + r) * p.os[1] + j] = Elem<OT>::from_float(r < valid ? p.scale * o[n][i] : 0.f);
                 }
+            if (odd_chunk) {
+                __syncthreads();
+                const int col = threadIdx.x, from = col < kCols ? odd_from[col] : -1;
+                if (from >= 0 && from < valid) {
+                    sC[from * kColPitch + col] = NAN;
+                    for (int r = p.reverse ? 0 : from; r < (p.reverse ? from + 1 : valid); ++r)
+                        out[(t0 + r) * p.os[1] + n0 + col] = Elem<OT>::from_float(NAN);
+                }
+                __syncthreads();
+            }
         }
         // S = lam^valid S + sum_j lam^. b_j c_j, where anyone asks for it
         if (!STATE_ONLY && step + 1 == sp.c1 - sp.c0 && !(p.state_out && sp.last)) break;
