@@ -125,6 +125,16 @@ template <int N> __device__ __forceinline__ void terms(F2 x, uint32_t &hi, uint3
     }
 }
 
+// Running maximum of BF16 pairs that keeps a NaN, and whether it has met one.
+__device__ __forceinline__ uint32_t max_nan(uint32_t a, uint32_t b) {
+    uint32_t r;
+    asm("max.NaN.bf16x2 %0, %1, %2;\n" : "=r"(r) : "r"(a), "r"(b));
+    return r;
+}
+__device__ __forceinline__ bool met_nan(uint32_t a) {  // such a NaN is 0x7fff
+    return ((a & 0x7fff7fffu) + 0x00010001u) & 0x80008000u;
+}
+
 __device__ __forceinline__ bool wait_slow(uint64_t *m, unsigned parity, volatile int *dead) {
     const long long t0 = clock64();
     for (int i = 0; i < (1 << 28); ++i) {
@@ -444,6 +454,7 @@ __global__ void __launch_bounds__(kTcThreads, 1) decay_walk_tc_kernel(const TcPa
                 if (!wait_warp(&bar.odone, n & 1)) break;
                 tc::fence_after_sync();
                 const float *w0 = ow + (p.reverse ? kChunk - valid : 0) + 2 * (lane & 3);
+                uint32_t seen = 0;
                 // 16 columns by 32 tokens at a time.  Fragments: this lane has tokens 8 b + 2 (lane % 4) + {0, 1} of
                 // column 16 d + lane / 4 (+ 8).
 #pragma unroll 1
@@ -473,6 +484,8 @@ __global__ void __launch_bounds__(kTcThreads, 1) decay_walk_tc_kernel(const TcPa
                                 const int r = r0 + e / 2 * 8;
                                 v[e] &= (r < valid ? 0xffffu : 0u) | (r + 1 < valid ? 0xffff0000u : 0u);
                             }
+#pragma unroll
+                        for (int e = 0; e < 8; ++e) seen = max_nan(seen, v[e]);
                         char *dst = stage + (VB == 2 ? (quad >> 1) * kBox : 0) + i * 32 * 128 + mtok +
                                     (((c0 + d * 2 + mcol) ^ (lane & 7)) << 4);
                         tc::stmatrix_x4_trans(dst, v[0], v[1], v[2], v[3]);
@@ -481,11 +494,52 @@ __global__ void __launch_bounds__(kTcThreads, 1) decay_walk_tc_kernel(const TcPa
 #pragma unroll
                         for (int e = 0; e < 8; ++e) {
                             const int r = r0 + e / 2 * 8, c = voff + quad * kQuadCols + d * 16 + (e & 1) * 8 + (lane >> 2);
-                            const float2 v = split2(x[e]);
+                            float2 v = split2(x[e]);
+                            v.x = r < valid ? v.x : 0.f;
+                            v.y = r + 1 < valid ? v.y : 0.f;
+                            seen = max_nan(seen, pack_bf16(v.x, v.y));
                             OT *o = out + (int64_t)(t0 + r) * p.os[1] + c;
-                            if (c < p.wc && t0 + r < time) o[0] = r < valid ? v.x : 0.f;
-                            if (c < p.wc && t0 + r + 1 < time) o[p.os[1]] = r + 1 < valid ? v.y : 0.f;
+                            if (c < p.wc && t0 + r < time) o[0] = v.x;
+                            if (c < p.wc && t0 + r + 1 < time) o[p.os[1]] = v.y;
                         }
+                    }
+                }
+                if (__builtin_expect(__any_sync(0xffffffffu, met_nan(seen)), 0)) {
+                    // A masked score of zero times a value that is not finite, or a zero weight times such a score, is
+                    // NaN.  The outputs that hold one although what they read of the state is finite are summed again,
+                    // over the tokens before them only: a lane has a column.
+                    __syncwarp();
+                    const bf16 *pa = static_cast<const bf16 *>(p.a) + b * p.as[0] + (h / p.ag) * p.as[2] + t0 * p.as[1];
+                    const bf16 *pb = static_cast<const bf16 *>(p.b) + b * p.bs[0] + (h / p.bg) * p.bs[2] + t0 * p.bs[1];
+                    const bf16 *pc = static_cast<const bf16 *>(p.c) + b * p.cs[0] + (h / p.cg) * p.cs[2] + t0 * p.cs[1];
+                    const int c = quad * kQuadCols + lane;
+                    const bool mine = lane < kQuadCols && voff + c < p.wc;
+#pragma unroll 1
+                    for (int i = 0; i < valid; ++i) {
+                        const float y = tc::tmem_ld1(tmem + lanes + kColO2 + i), z = tc::tmem_ld1(tmem + lanes + kColO1 + i);
+                        tc::tmem_wait_ld();
+                        const float read = ow[(p.reverse ? kChunk - valid : 0) + i] * y, sum = read + z;
+                        const bool redo = mine && sum != sum && read == read;
+                        if (!__any_sync(0xffffffffu, redo)) continue;
+                        const int j0 = p.reverse ? i : 0, j1 = p.reverse ? valid : i + 1;
+                        float o = read;
+#pragma unroll 1
+                        for (int j = j0; j < j1; ++j) {
+                            float s = 0.f;
+#pragma unroll 1
+                            for (int k = lane; k < p.wab; k += 32)
+                                s = fmaf(__bfloat162float(pa[i * p.as[1] + k]), __bfloat162float(pb[j * p.bs[1] + k]), s);
+                            s = warp_sum(s) * wt[kChunk + (p.reverse ? j - i : i - j)];
+                            if (mine) o = fmaf(__bfloat162float(__float2bfloat16_rn(s)), __bfloat162float(pc[j * p.cs[1] + voff + c]), o);
+                        }
+                        if (redo) {
+                            if constexpr (kTma)
+                                *reinterpret_cast<bf16 *>(stage + c / 64 * kBox + i * 128 + (((c & 63) >> 3 ^ (i & 7)) << 4) +
+                                                          (c & 7) * 2) = __float2bfloat16_rn(o);
+                            else
+                                out[(int64_t)(t0 + i) * p.os[1] + voff + c] = o;
+                        }
+                        __syncwarp();
                     }
                 }
                 if (kTma) tc::fence_async_smem();

@@ -165,6 +165,12 @@ __device__ __forceinline__ void tmem_ld8(uint32_t taddr, float (&v)[8]) {
 #pragma unroll
     for (int i = 0; i < 8; ++i) v[i] = __uint_as_float(r[i]);
 }
+// One column: this lane's own word.
+__device__ __forceinline__ float tmem_ld1(uint32_t taddr) {
+    uint32_t r;
+    asm volatile("tcgen05.ld.sync.aligned.32x32b.x1.b32 {%0}, [%1];\n" : "=r"(r) : "r"(taddr));
+    return __uint_as_float(r);
+}
 // Fragment forms: 16 lanes (16 * k from the warp's first), the layout of the mma.sync fragments.
 // 32 consecutive columns: registers 4 b .. 4 b + 3 hold columns 8 b + 2 (l % 4) + {0, 1} of lane l / 4, then of
 // lane l / 4 + 8.

@@ -188,7 +188,8 @@ def decay_attention(q, k, v, log_decay, *, scale=None, initial_state=None, lengt
 
     Returns o [B, T, H, dv] in q's dtype, and with ``return_state`` (o, state [B, H, dk, dv] float32), the
     state after each row's last valid token, starting from ``initial_state`` (zero if None).
-    Differentiable in q, k, v and initial_state, through o and the state.
+    An infinity or NaN makes what the recurrence lets it reach infinite or NaN (an infinity may arrive as NaN) and
+    leaves everything else, the tokens before it among it, as it is.  Differentiable in q, k, v and initial_state, through o and the state.
     """
     if q.ndim != 4 or k.ndim != 4 or v.ndim != 4:
         raise ValueError('q, k and v must be [batch, time, heads, width]')

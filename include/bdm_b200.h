@@ -474,6 +474,7 @@ BDM_API int bdm_decode_token_step(const void *proj, int64_t batch, int64_t ld, i
  *   X = state_in * state_in_mul (0 if null), state_out = Y * state_out_mul (skipped if null).
  * The attention is the forward walk of (q, k, v); its gradients are dq = forward(do, v, k),
  * dk = reverse(v, do, q) and dv = reverse(k, q, do).  Outputs of rows past n are 0; nothing is read there.
+ * Infinities and NaN stay with what these sums let them reach, where an infinity may arrive as NaN.
  * Strides are in elements, in the order batch, token, head; columns are contiguous.  Head h uses head
  * h / (heads / x_heads) of operand x.  States are FP32 [batch, heads, width_ab, width_c], or with
  * *_transposed [batch, heads, width_c, width_ab].  Products, sums and states are FP32.
