@@ -35,9 +35,10 @@ def beam_select(logits, scores, *, finished=None, eos_token=None, stable_slots=F
     candidate, ``eos_token`` at its score.  Logits of -inf are banned tokens.  A row with NaN, +inf or no
     finite logit has no candidate above -inf.  Ties go to the lower w, then the lower t.  Beams come in
     descending order, or with ``stable_slots`` each parent's best child in the parent's place and the other
-    children in the free places in turn.  W <= 32.
+    children in the free places in turn.  W <= 32.  Not differentiable.
     """
     ops._cuda(logits, scores, finished)
+    ops._no_tangents('beam_select', logits, scores)
     if logits.ndim != 3 or tuple(scores.shape) != tuple(logits.shape[:2]) or scores.dtype != torch.float32:
         raise ValueError('logits must be [batch, beams, vocab] and scores float32 [batch, beams]')
     batch, beams, vocab = logits.shape
@@ -89,6 +90,7 @@ def reorder_states(states, parents):
     status that ``ops.check_scan_status`` reports.  Returns ``states``.
     """
     ops._cuda(parents, *states)
+    ops._no_tangents('reorder_states', *states)
     if parents.ndim != 2 or parents.dtype != torch.int64 or parents.shape[1] < 1:
         raise ValueError('parents must be int64 [batch, beams]')
     batch, beams = parents.shape

@@ -189,11 +189,13 @@ def decay_attention(q, k, v, log_decay, *, scale=None, initial_state=None, lengt
     Returns o [B, T, H, dv] in q's dtype, and with ``return_state`` (o, state [B, H, dk, dv] float32), the
     state after each row's last valid token, starting from ``initial_state`` (zero if None).
     An infinity or NaN makes what the recurrence lets it reach infinite or NaN (an infinity may arrive as NaN) and
-    leaves everything else, the tokens before it among it, as it is.  Differentiable in q, k, v and initial_state, through o and the state.
+    leaves everything else, the tokens before it among it, as it is.
+    Differentiable (in reverse mode, once) in q, k, v and initial_state, through o and the state.
     """
     if q.ndim != 4 or k.ndim != 4 or v.ndim != 4:
         raise ValueError('q, k and v must be [batch, time, heads, width]')
     scale = _check_heads(q, k, v, log_decay, scale)
+    ops._no_tangents('decay_attention', q, k, v, log_decay, initial_state)
     batch = q.shape[0]
     if initial_state is not None:
         _check_state('initial_state', initial_state, (batch, q.shape[2], q.shape[3], v.shape[3]), q.device)
@@ -221,6 +223,7 @@ def decay_attention_step(q, k, v, log_decay, state, *, scale=None):
     if q.ndim != 3 or k.ndim != 3 or v.ndim != 3:
         raise ValueError('q, k and v must be [batch, heads, width]')
     scale = _check_heads(q, k, v, log_decay, scale)
+    ops._no_tangents('decay_attention_step', q, k, v, log_decay, state)
     if torch.is_grad_enabled() and (q.requires_grad or k.requires_grad or v.requires_grad or state.requires_grad):
         raise RuntimeError('decay_attention_step requires no_grad or inference_mode')
     batch, heads, dk = q.shape

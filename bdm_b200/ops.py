@@ -28,6 +28,7 @@ from __future__ import annotations
 import ctypes
 
 import torch
+from torch.autograd import forward_ad
 
 from . import _lib
 from .config import near_square_factors
@@ -47,6 +48,13 @@ def _cuda(*tensors):
     for t in tensors:
         if t is not None and not t.is_cuda:
             raise ValueError('bdm_b200 ops require CUDA tensors (there is no CPU path)')
+
+
+def _no_tangents(what, *tensors):
+    """Raises where one of the tensors carries a forward-mode tangent, which a kernel would drop."""
+    if forward_ad._current_level >= 0 and any(t is not None and forward_ad.unpack_dual(t).tangent is not None
+                                              for t in tensors):
+        raise NotImplementedError(f'{what} has no forward-mode derivative')
 
 
 def _ptr(t):
