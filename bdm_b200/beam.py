@@ -39,6 +39,8 @@ def beam_select(logits, scores, *, finished=None, eos_token=None, stable_slots=F
     """
     ops._cuda(logits, scores, finished)
     ops._no_tangents('beam_select', logits, scores)
+    if torch.is_grad_enabled() and (logits.requires_grad or scores.requires_grad):
+        raise RuntimeError('beam_select requires no_grad or inference_mode for logits and scores that need gradients')
     if logits.ndim != 3 or tuple(scores.shape) != tuple(logits.shape[:2]) or scores.dtype != torch.float32:
         raise ValueError('logits must be [batch, beams, vocab] and scores float32 [batch, beams]')
     batch, beams, vocab = logits.shape

@@ -43,3 +43,13 @@ def test_a_layer_refuses_tangents():
     x = torch.randn(1, 10, 64, device=DEV)
     with torch.no_grad(), forward_ad.dual_level(), pytest.raises(NotImplementedError):
         m(forward_ad.make_dual(x, torch.ones_like(x)))
+
+
+def test_selection_refuses_to_cut_a_graph():
+    from bdm_b200 import beam_select
+    logits, scores = torch.randn(2, 3, 10, device=DEV), torch.zeros(2, 3, device=DEV)
+    for args in ((logits.clone().requires_grad_(True), scores), (logits, scores.clone().requires_grad_(True))):
+        with pytest.raises(RuntimeError):
+            beam_select(*args)
+        with torch.no_grad():
+            beam_select(*args)
