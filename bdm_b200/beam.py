@@ -129,6 +129,7 @@ def reorder_states(states, parents):
                                                 (ctypes.c_int64 * n)(*sizes), n, parents.data_ptr(), batch, beams,
                                                 ops._scan_status_of(dev).mapped_ptr + 4, _raw_stream(dev)),
                    'bdm_reorder_rows')
+    ops._changed(*states)
     return states
 
 

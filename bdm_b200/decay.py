@@ -241,6 +241,7 @@ def decay_attention_step(q, k, v, log_decay, state, *, scale=None):
         status = _lib.load().bdm_decay_step(a, _raw_stream(q.device))
     if status:
         _lib.check(status, 'bdm_decay_step')
+    ops._changed(state)
     return out
 
 

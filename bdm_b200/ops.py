@@ -29,6 +29,7 @@ import ctypes
 
 import torch
 from torch.autograd import forward_ad
+from torch.autograd.graph import increment_version
 
 from . import _lib
 from .config import near_square_factors
@@ -55,6 +56,13 @@ def _no_tangents(what, *tensors):
     if forward_ad._current_level >= 0 and any(t is not None and forward_ad.unpack_dual(t).tangent is not None
                                               for t in tensors):
         raise NotImplementedError(f'{what} has no forward-mode derivative')
+
+
+def _changed(*tensors):
+    """Tells autograd that a kernel writes to these tensors, as torch's own in-place operations do."""
+    for t in tensors:
+        if not t.is_inference():
+            increment_version(t)
 
 
 def _ptr(t):
