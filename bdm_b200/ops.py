@@ -165,9 +165,14 @@ def check_mapped_status(st: _ScanStatus) -> None:
 
 
 def reset_scan_status(device=None) -> None:
+    """Clears the device status, after what was launched before on the current stream (waiting for it, except
+    inside a capture, where the clearing becomes part of the graph)."""
     st = _scan_status_of(device)
     st.word.zero_()
-    st.mapped.zero_()
+    for i in range(2):  # the mapped words too in stream order: a kernel still running may yet set them
+        st.mapped[i:i + 1].copy_(st.word, non_blocking=True)
+    if not torch.cuda.is_current_stream_capturing():
+        torch.cuda.current_stream(st.word.device).synchronize()
     if st.event is not None:
         st.event.synchronize()
         st.event = None
