@@ -83,6 +83,11 @@ def beam_select(logits, scores, *, finished=None, eos_token=None, stable_slots=F
     return BeamStep(out_scores, parents, tokens, done)
 
 
+def _overlap(spans):
+    spans.sort()
+    return any(b[0] < a[1] for a, b in zip(spans, spans[1:]))
+
+
 def reorder_states(states, parents):
     """In place, for every tensor of ``states`` ([B * W, ...]): row (b, w) becomes row (b, parents[b, w]).
 
@@ -119,8 +124,9 @@ def reorder_states(states, parents):
         strides.append(stride)
         sizes.append(size)
         extents.append((s.data_ptr(), s.data_ptr() + stride * (s.shape[0] - 1) + size))
-    extents.sort()
-    if any(b[0] < a[1] for a, b in zip(extents, extents[1:])):
+    if _overlap(extents) and _overlap([(base + i * stride, base + i * stride + size)  # rows may lie between other rows
+                                       for base, stride, size in zip(bases, strides, sizes)
+                                       for i in range(batch * beams)]):
         raise ValueError('the states must not overlap')
     parents = parents.contiguous()
     n = len(bases)
