@@ -96,6 +96,9 @@ def reorder_states(states, parents):
     (unless another row takes them).  A parent outside [0, W) leaves its row as it is and sets the device
     status that ``ops.check_scan_status`` reports.  Returns ``states``.
     """
+    if isinstance(states, torch.Tensor):
+        raise ValueError('states must be a list of tensors')
+    given, states = states, list(states)
     ops._cuda(parents, *states)
     ops._no_tangents('reorder_states', *states)
     if parents.ndim != 2 or parents.dtype != torch.int64 or parents.shape[1] < 1:
@@ -136,7 +139,7 @@ def reorder_states(states, parents):
                                                 ops._scan_status_of(dev).mapped_ptr + 4, _raw_stream(dev)),
                    'bdm_reorder_rows')
     ops._changed(*states)
-    return states
+    return given
 
 
 def beam_search(model, prompt, *, beams, max_new_tokens, eos_token=None):

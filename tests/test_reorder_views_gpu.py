@@ -34,3 +34,14 @@ def test_views_that_do_overlap_are_refused():
                    [x.flatten().as_strided((2, 4), (8, 1)), x.flatten().as_strided((2, 4), (12, 1))]):
         with pytest.raises(ValueError):
             reorder_states(states, parents)
+
+
+def test_states_of_any_iterable_and_single_tensors():
+    from bdm_b200 import reorder_states
+    parents = torch.tensor([[1, 0]], device=DEV)
+    x = torch.arange(8.0, device=DEV).reshape(2, 4)
+    want = x.flip(0)
+    reorder_states((s for s in [x]), parents)
+    assert torch.equal(x, want)
+    with pytest.raises(ValueError):
+        reorder_states(torch.zeros(2, 2, device=DEV), parents)  # a tensor is not a list of states
