@@ -11,7 +11,6 @@ model can interleave the two (``HybridLanguageModel``).  There is no reference c
 """
 from __future__ import annotations
 
-import math
 import struct
 from contextlib import nullcontext
 
@@ -167,8 +166,8 @@ def _check_heads(q, k, v, log_decay, scale):
     if scale is None:
         return dk ** -0.5
     scale = float(scale)
-    if not math.isfinite(scale) or scale == 0.0:
-        raise ValueError('scale must be finite and not 0')
+    if not 1e-38 <= abs(scale) <= 1e38:  # its reciprocal is an FP32 number too: the backward pass divides by it
+        raise ValueError('scale must be between 1e-38 and 1e38 in magnitude')
     return scale
 
 
