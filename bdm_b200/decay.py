@@ -249,7 +249,7 @@ class DecayAttention(nn.Module):
 
     One projection gives q, k (SiLU, unit norm per head), v and an output gate; the heads' outputs are
     RMS-normalised per head, gated by a sigmoid and projected back.  The decays are fixed: 1 - 2^-e with e
-    spread evenly over [min_exponent, max_exponent] across the heads.  ``forward`` / ``prefill`` / ``step``
+    spread evenly over [min_exponent, max_exponent] across the heads (buffer ``log_decays``).  ``forward`` / ``prefill`` / ``step``
     / ``create_state`` mirror the bank memory layer's; the state is FP32 [B, H, key width, value width].
     """
 
@@ -272,9 +272,11 @@ class DecayAttention(nn.Module):
             self.in_proj = nn.Linear(dim, sum(self._splits), bias=False)
             self.o_proj = nn.Linear(num_heads * self.value_width, dim, bias=False)
         self.norm_weight = nn.Parameter(torch.ones(num_heads * self.value_width))
-        exponent = torch.linspace(float(min_exponent), float(max_exponent), num_heads, dtype=torch.float64)
-        self._log_decay = torch.log1p(-torch.exp2(-exponent)).float()  # a constant: FP32 whatever the module's dtype
-        self._decay_on = {}
+        with torch.inference_mode(False):  # backward passes save them
+            exponent = torch.linspace(float(min_exponent), float(max_exponent), num_heads, dtype=torch.float64, device='cpu')
+            log_decays = torch.log1p(-torch.exp2(-exponent)).float()
+            at = self.in_proj.weight.device
+            self.register_buffer('log_decays', log_decays if at.type == 'meta' else log_decays.to(at))
         self.init_weights(initialization_seed=seed)
 
     def init_weights(self, *, initialization_seed=0):
@@ -284,12 +286,22 @@ class DecayAttention(nn.Module):
                 nn.init.trunc_normal_(w, std=w.shape[1] ** -0.5, a=-3 * w.shape[1] ** -0.5, b=3 * w.shape[1] ** -0.5)
         nn.init.ones_(self.norm_weight)
 
+    def _apply(self, fn, recurse=True):
+        # the decays follow the module's device, but are FP32 whatever its dtype
+        log_decays = self.log_decays
+        super()._apply(fn, recurse)
+        with torch.inference_mode(False):
+            self.log_decays = log_decays.to(self.log_decays.device)
+        return self
+
+    def _load_from_state_dict(self, state_dict, prefix, *args, **kwargs):
+        # checkpoints of before the decays were part of them
+        state_dict.setdefault(prefix + 'log_decays', self.log_decays)
+        super()._load_from_state_dict(state_dict, prefix, *args, **kwargs)
+
     def log_decay(self, device):
-        """The heads' log-decays [H] on ``device`` (uploaded once per device)."""
-        if device not in self._decay_on:
-            with torch.inference_mode(False):
-                self._decay_on[device] = self._log_decay.to(device)
-        return self._decay_on[device]
+        """The heads' log-decays [H] on ``device``."""
+        return self.log_decays if self.log_decays.device == device else self.log_decays.to(device)
 
     def create_state(self, batch, *, device=None):
         """A zero state for ``batch`` rows."""
