@@ -11,12 +11,13 @@
 //   out  = O1 + scale lam^. O2,    S <- lam^n S + T
 // The state itself stays in registers in FP32.  Roundings to BF16: P and the copy of S that is read (one
 // rounding each, as large as the output's own).  V' is split into three terms (24 bits) where a state is
-// returned: T, and with it the state over any number of chunks, is then exact to FP32.  Where none is, two
-// terms (an error of 2^-17 beside the outputs' 2^-9) are enough.
+// returned: the state is then as near as an FP32 sum, over any number of chunks (65536 to 400000 tokens of one sign
+// without decay: 1.5e-6 at the worst element).  Where none is, two terms (an error of 2^-17 beside the outputs' 2^-9)
+// are enough.
 //
 // Roles (23 warps of 24): 0-7 carry the state (a quadrant's value columns, half of the key columns), 8-11 scale V',
 // 12-15 the outputs, 16-19 P, 20 and 22 MMA, 21 TMA.  V' is made and T issued in two halves of 32 tokens, so that
-// the scaling of one overlaps the product of the other (in the state launch by two groups, 4-7 and 8-11, at once).
+// the scaling of one overlaps the product of the other (in the state launch by two groups, 8-11 and 12-15, at once).
 // V' is in tensor memory because shared memory's bandwidth is what the products and copies share: as a
 // shared-memory operand it took 768 more of its cycles per chunk.
 // The roles' loops are kept short on purpose: five roles' unrolled code does not fit the instruction cache
@@ -55,6 +56,12 @@ constexpr unsigned long long kWaitNs = 2000000000ull;
 
 // tensor memory columns
 constexpr uint32_t kColA = 0, kColO1 = 64, kColO2 = 128, kColT = 192, kColS = 320, kColV = 384;
+// State launch: the chunks whose products gather in one T before it is added to the FP32 state.  Tensor-core sums are
+// cut off, not rounded, and a long one drifts: of 65536 tokens of one sign x 74 heads of 64, 3.4e-5 of the state was lost
+// with whole sub-segments in one T, and 1e-8 is in groups of 4 (1.5e-6 at the worst element, as in FP32).  Two T's, so
+// that one is read while the next group gathers (1 x 65536 x 8 x 128: 179 us, with one sum 177.5).
+constexpr int kGroup = 4;
+constexpr uint32_t kColT2 = 0;
 
 struct Maps {
     CUtensorMap a, b, c, out;
@@ -72,7 +79,8 @@ struct TcParams {
 // needs something that its waiter gives after the wait (P's two buffers have one barrier each for that reason).
 struct Bars {
     uint64_t full[kMaxStages], empty[kMaxStages];
-    uint64_t vready[2], tpart[2], tlast, tfree, sready;       // V' halves, T halves, all T, T read, S written
+    uint64_t vready[2], tpart[2], tfree, sready;              // V' halves, T halves, T read, S written
+    uint64_t tgroup[2], tdrained[2];                          // state launch: a group's T whole, read
     uint64_t adone, pready, pfree[2], odone, oissued[2], ofree;  // A, P, P read, O, O issued, O read
     uint64_t zeroed, ofull, oempty, drain[2];                 // row's end cleared, output buffers, issuers' last products
 };
@@ -229,10 +237,11 @@ __global__ void __launch_bounds__(kTcThreads, 1) decay_walk_tc_kernel(const TcPa
         for (int i = 0; i < 2; ++i) {
             tc::mbar_init(&bar.vready[i], 4);
             tc::mbar_init(&bar.tpart[i], 1);
+            tc::mbar_init(&bar.tgroup[i], 1);
+            tc::mbar_init(&bar.tdrained[i], kStateWarps);
             tc::mbar_init(&bar.pfree[i], 1);
             tc::mbar_init(&bar.oissued[i], 1);
         }
-        tc::mbar_init(&bar.tlast, 1);
         tc::mbar_init(&bar.tfree, kStateWarps);
         tc::mbar_init(&bar.sready, kStateWarps);
         tc::mbar_init(&bar.adone, 1);
@@ -299,7 +308,7 @@ __global__ void __launch_bounds__(kTcThreads, 1) decay_walk_tc_kernel(const TcPa
                 if (!wait_warp(&bar.tpart[hb], (n - 1) & 1)) return false;
                 tc::fence_after_sync();
             }
-            // in the state launch all chunks gather in one T: their distance to the segment's end counts too
+            // in the state launch chunks are added up without a carry: their distance to the segment's end counts too
             float far = 1.f;
             if (STATE_ONLY) {
                 const int64_t last = sp.c1 * kChunk < sp.n ? sp.c1 * kChunk : sp.n;
@@ -379,33 +388,41 @@ __global__ void __launch_bounds__(kTcThreads, 1) decay_walk_tc_kernel(const TcPa
             if (before) gather(zs, true, 1.f);
             if (p.state_in) gather(x, p.in_t, w);
         }
+        auto add_products = [&](uint32_t col, F2 carry) {
+#pragma unroll
+            for (int d = 0; d < kHalves; ++d)
+#pragma unroll
+                for (int i = 0; i < KC; i += 32) {
+                    float t[16];
+                    tc::tmem_ld_16x256b_x4(tmem + lanes + (d << 20) + col + k0 + i, t);
+                    tc::tmem_wait_ld();
+#pragma unroll
+                    for (int e = 0; e < 8; ++e) S[d][i / 4 + e] = fma2(carry, S[d][i / 4 + e], make2(t[2 * e], t[2 * e + 1]));
+                }
+        };
         bool ok = true;
-        if (STATE_ONLY && warp >= 4) ok = scale_values(1, 2, threadIdx.x - 128);  // nothing else to do until the end
-        for (int n = 0; ok && n <= steps; ++n) {
-            if (n > 0) {
-                if (STATE_ONLY && n < steps) continue;  // T gathers all chunks in tensor memory
-                ok = STATE_ONLY ? wait_warp(&bar.tlast, 0) : wait_warp(&bar.tpart[1], (n - 1) & 1);
+        if constexpr (STATE_ONLY)
+            for (int i = 0; ok && i * kGroup < steps; ++i) {
+                ok = wait_warp(&bar.tgroup[i & 1], (i >> 1) & 1);
                 if (!ok) break;
                 tc::fence_after_sync();
-                const float f = STATE_ONLY ? 0.f : pw[valid_of(n - 1)];
-                const F2 carry = make2(f, f);
-#pragma unroll
-                for (int d = 0; d < kHalves; ++d)
-#pragma unroll
-                    for (int i = 0; i < KC; i += 32) {
-                        float t[16];
-                        tc::tmem_ld_16x256b_x4(tmem + lanes + (d << 20) + kColT + k0 + i, t);
-                        tc::tmem_wait_ld();
-#pragma unroll
-                        for (int e = 0; e < 8; ++e) S[d][i / 4 + e] = fma2(carry, S[d][i / 4 + e], make2(t[2 * e], t[2 * e + 1]));
-                    }
+                add_products(i & 1 ? kColT2 : kColT, make2(1.f, 1.f));
+                arrive(&bar.tdrained[i & 1]);
+            }
+        for (int n = 0; !STATE_ONLY && ok && n <= steps; ++n) {
+            if (n > 0) {
+                ok = wait_warp(&bar.tpart[1], (n - 1) & 1);
+                if (!ok) break;
+                tc::fence_after_sync();
+                const float f = pw[valid_of(n - 1)];
+                add_products(kColT, make2(f, f));
                 if (n == steps) break;
                 arrive(&bar.tfree);
                 ok = wait_warp(&bar.odone, (n - 1) & 1);  // the last chunk's reads of S are over
                 if (!ok) break;
                 tc::fence_after_sync();
             }
-            if (!STATE_ONLY && n < steps) {
+            if (n < steps) {
 #pragma unroll
                 for (int d = 0; d < kHalves; ++d)
 #pragma unroll
@@ -559,6 +576,8 @@ __global__ void __launch_bounds__(kTcThreads, 1) decay_walk_tc_kernel(const TcPa
                 }
             }
             if (kTma && warp == kOutWarp && lane == 0) tc::tma_store_wait();
+        } else {
+            scale_values(1, 2, threadIdx.x - kOutWarp * 32);  // the halves that the other group leaves out
         }
     } else if (warp < kMmaWarp) {
         tc::regs_down<kScoreRegs>();
@@ -615,7 +634,12 @@ __global__ void __launch_bounds__(kTcThreads, 1) decay_walk_tc_kernel(const TcPa
             for (int n = 0; n < steps && ok; ++n) {
                 uint64_t kb = tc::smem_desc_sw128_mn(tile, kBox);
                 uint32_t va = tmem + kColV;
-                if (!STATE_ONLY && n > 0) {
+                uint32_t to = tmem + kColT;
+                if (STATE_ONLY) {
+                    const int i = n / kGroup;
+                    to = tmem + (i & 1 ? kColT2 : kColT);
+                    if (n % kGroup == 0 && i > 1 && !(ok = wait(&bar.tdrained[i & 1], ((i >> 1) - 1) & 1))) break;
+                } else if (n > 0) {
                     if (!(ok = wait(&bar.tfree, (n - 1) & 1))) break;
                     // long products (N = 128) must not get ahead of the outputs', which more is waiting for
                     if (DKB == 2 && !(ok = wait(&bar.oissued[(n - 1) & 1], ((n - 1) >> 1) & 1))) break;
@@ -628,15 +652,15 @@ __global__ void __launch_bounds__(kTcThreads, 1) decay_walk_tc_kernel(const TcPa
                     for (int t = 0; t < TERMS; ++t)
 #pragma unroll
                         for (int k = 0; k < 2; ++k)
-                            tc::mma_bf16_tmem_a(tmem + kColT, va + t * 16 + k * 8, kb + k * 2048 / 16, idT,
-                                                hb + t + k + (STATE_ONLY ? n : 0) > 0);
+                            tc::mma_bf16_tmem_a(to, va + t * 16 + k * 8, kb + k * 2048 / 16, idT,
+                                                hb + t + k + (STATE_ONLY ? n % kGroup : 0) > 0);
                     tc::mma_commit(&bar.tpart[hb]);
                 }
+                if (STATE_ONLY && ok && (n % kGroup == kGroup - 1 || n + 1 == steps)) tc::mma_commit(&bar.tgroup[n / kGroup & 1]);
                 tc::mma_commit(&bar.empty[st]);
                 tile += kStage;
                 if (++st == stages) st = 0, tile -= stages * kStage;
             }
-            if (STATE_ONLY && ok) tc::mma_commit(&bar.tlast);
             // no product may be in flight when the CTA ends, whatever happened to its consumers
             tc::mma_commit(&bar.drain[0]);
             tc::mbar_wait(&bar.drain[0], 0, kWaitNs);
