@@ -249,8 +249,9 @@ class DecayAttention(nn.Module):
 
     One projection gives q, k (SiLU, unit norm per head), v and an output gate; the heads' outputs are
     RMS-normalised per head, gated by a sigmoid and projected back.  The decays are fixed: 1 - 2^-e with e
-    spread evenly over [min_exponent, max_exponent] across the heads (buffer ``log_decays``).  ``forward`` / ``prefill`` / ``step``
-    / ``create_state`` mirror the bank memory layer's; the state is FP32 [B, H, key width, value width].
+    spread evenly over [min_exponent, max_exponent] across the heads (buffer ``log_decays``).  ``forward`` /
+    ``prefill`` / ``step`` / ``create_state`` mirror the bank memory layer's; the state is FP32 [B, H, key width,
+    value width].
     """
 
     def __init__(self, dim, num_heads, *, key_width=None, value_width=None, kv_heads=None, min_exponent=3.0,
@@ -311,7 +312,8 @@ class DecayAttention(nn.Module):
     def _heads(self, hidden):
         q, k, v, gate = self.in_proj(hidden).split(self._splits, -1)
         lead = hidden.shape[:-1]
-        unit = lambda x, n: F.normalize(F.silu(x.reshape(*lead, n, self.key_width)), dim=-1, eps=1e-6)  # noqa: E731
+        unit = lambda x, n: F.normalize(F.silu(x.reshape(*lead, n, self.key_width)), dim=-1,  # noqa: E731
+                                        eps=1e-6).to(v.dtype)  # autocast leaves norms in FP32
         return unit(q, self.num_heads), unit(k, self.kv_heads), v.reshape(*lead, self.kv_heads, self.value_width), gate
 
     def _output(self, o, gate):
