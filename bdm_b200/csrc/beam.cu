@@ -582,7 +582,7 @@ constexpr int kUnroll = 4;  // columns a thread moves at a time
 
 // In place: each thread owns columns of one group's rows and reads all of them that move before it writes
 // any, so permutations and copies need no second buffer, and rows that stay cost nothing.  Bound by HBM: 16
-// groups of 4 rows of 12.6 MB, half of them moved, take 129 us (123 at the copy rate), all of them 241 (246);
+// groups of 4 rows of 12.6 MB, half of them moved, take 132 us (127 at the copy rate), all of them 248 (254).
 template <typename U, int W>
 __global__ void __launch_bounds__(kThreads)
     reorder_rows_kernel(const Tensors t, const int64_t *__restrict__ parents, int beams, int64_t groups, int *status) {
@@ -627,7 +627,7 @@ __global__ void __launch_bounds__(kThreads)
 }
 
 // The same for more than 16 beams, whose columns would take all of a thread's registers: the rows that move pass
-// through shared memory, 1 KB of each at a time (2 groups of 32 rows of 12.6 MB, half of them moved: 156 us, from
+// through shared memory, 1 KB of each at a time (2 groups of 32 rows of 12.6 MB, half of them moved: 156 to 171 us, from
 // registers 217; 4 groups of 16: 178, from registers in 8-byte columns 133).
 constexpr int kTileUnits = 64;
 __global__ void __launch_bounds__(kThreads)

@@ -5,7 +5,7 @@
 // a b runs on the tensor cores as three TF32 products, a1 b1 + a1 b2 + a2 b1 with a = a1 + a2 + r, |r| <= 2^-22 |a|
 // (the method of splitting an operand into its rounding and the remainder), summed in FP32: about 3e-7 beside
 // FP32's own 1e-7, where plain TF32 gives 5e-4.  Sums and states are FP32.  Bound: the TF32 products' rate and
-// the latency of a chunk's phases (2 x 4096 tokens x 8 heads of 128: 365 us; 3 x 777 x 6 heads of 40 / 72: 48 us
+// the latency of a chunk's phases (2 x 4096 tokens x 8 heads of 128: 354 us; 3 x 777 x 6 heads of 40 / 72: 48 us
 // in three launches, on FP32 FMAs with the same tiles 72).
 #include "decay_walk.cuh"
 
@@ -103,8 +103,8 @@ __device__ __forceinline__ float load_rows(float *dst, int pitch, const T *src, 
 // One CTA walks one segment of one (row, head) for 64 columns of c.  With 8 warps, P and the outputs are 4 x 2
 // warp tiles of 16 x 32 and a warp has two of the state's up to 8 x 2 tiles of that size; with 16 warps, 4 x 4 of
 // 16 x 16 and one of the state's.  Shared memory decides: up to 80 columns of a and b two or three CTAs of 8 warps
-// share an SM (3 x 777 x 6 heads of 40 / 72: 48 us, with 16 warps 62), past that one of 16 hides more latency than
-// one of 8 (2 x 4096 x 8 heads of 128: 365 us, with 8 warps 441, issuing in 38 % of the cycles).
+// share an SM (3 x 777 x 6 heads of 40 / 72: 48 us, with 16 warps 55), past that one of 16 hides more latency than
+// one of 8 (2 x 4096 x 8 heads of 128: 354 us, with 8 warps 430, issuing in 38 % of the cycles).
 template <int WARPS, typename T, typename OT, bool STATE_ONLY>
 __global__ void __launch_bounds__(WARPS * 32) decay_walk_kernel(const Params p) {
     constexpr int kThreads = WARPS * 32, N = 32 / WARPS, ST = 16 / WARPS;

@@ -75,8 +75,8 @@ bool decay_walk_tc_takes(const bdm_decay_walk_args &w) {
 // Segments of the time axis, and CTAs to a row's value columns: the split that makes the launches shortest, in
 // units of a chunk of the main walk (1.7 us).  A CTA has an SM to itself; its start and end cost about three
 // chunks, a chunk of half the columns 0.75, one of the state launch 0.6 of the walk's, the prefix launch and the
-// dependent starts about six in all.  (8 x 4096 tokens x 8 heads of 128: two segments 104 us, two halves of the
-// columns 91; halves also read a and b twice, but from L2.)
+// dependent starts about six in all.  (8 x 4096 tokens x 8 heads of 128 with the state: two segments 103 us, two
+// halves of the columns 83; halves also read a and b twice, but from L2.)
 WalkSplit decay_walk_tc_split(int64_t rows, int64_t chunks, int width_c, int sms) {
     WalkSplit best{1, (int)chunks, 1, (int)chunks, 1};
     double cost = (double)ceil_div(rows, sms) * (chunks + 3.0);

@@ -190,6 +190,9 @@ def decay_attention(q, k, v, log_decay, *, scale=None, initial_state=None, lengt
     An infinity or NaN makes what the recurrence lets it reach infinite or NaN (an infinity may arrive as NaN) and
     leaves everything else, the tokens before it among it, as it is.
     Differentiable (in reverse mode, once) in q, k, v and initial_state, through o and the state.
+    Sums and the state are FP32.  With bfloat16 inputs the decayed scores and the copy of the state that o reads are
+    rounded to bfloat16 once each, as o is; without ``return_state``, and in gradients, the terms of the state that is
+    not returned have 17 bits instead of 24, so that o may differ by a rounding.
     """
     if q.ndim != 4 or k.ndim != 4 or v.ndim != 4:
         raise ValueError('q, k and v must be [batch, time, heads, width]')

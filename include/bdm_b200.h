@@ -477,7 +477,10 @@ BDM_API int bdm_decode_token_step(const void *proj, int64_t batch, int64_t ld, i
  * Infinities and NaN stay with what these sums let them reach, where an infinity may arrive as NaN.
  * Strides are in elements, in the order batch, token, head; columns are contiguous.  Head h uses head
  * h / (heads / x_heads) of operand x.  States are FP32 [batch, heads, width_ab, width_c], or with
- * *_transposed [batch, heads, width_c, width_ab].  Products, sums and states are FP32.
+ * *_transposed [batch, heads, width_c, width_ab].  Sums and states are FP32, and so are the products of FP32 operands
+ * (three TF32 products for one).  BF16 operands that TMA can address (16-byte aligned base and strides) run on the BF16
+ * tensor cores: there the decayed scores and the copy of the state that the outputs read are rounded to BF16 once each,
+ * whatever out_dtype is, and the terms of the state have 24 bits where state_out is given, 17 where it is not.
  * overlap = 1: where the walk is one launch, it may start while the launch before it in the stream still runs, and so
  * beside everything back to the last walk (or other kernel) that did not overlap, whoever launched it.  The caller
  * knows that it neither writes what those use nor reads what they write (dk after dq, dv after dk, with all three
