@@ -527,7 +527,8 @@ __global__ void __launch_bounds__(kTcThreads, 1) decay_walk_tc_kernel(const TcPa
                 if (__builtin_expect(__any_sync(0xffffffffu, met_nan(seen)), 0)) {
                     // A masked score of zero times a value that is not finite, or a zero weight times such a score, is
                     // NaN.  The outputs that hold one although what they read of the state is finite are summed again,
-                    // over the tokens before them only: a lane has a column.
+                    // over the tokens that reach them only: a lane has a column.  Slow (up to 1 ms a chunk), but a chunk
+                    // where this happens turns columns or rows of the state bad, which then need it no more.
                     __syncwarp();
                     const bf16 *pa = static_cast<const bf16 *>(p.a) + b * p.as[0] + (h / p.ag) * p.as[2] + t0 * p.as[1];
                     const bf16 *pb = static_cast<const bf16 *>(p.b) + b * p.bs[0] + (h / p.bg) * p.bs[2] + t0 * p.bs[1];
